@@ -58,11 +58,13 @@ typedef enum {
     ST_ERR_OOM = 7
 } st_status;
 
-typedef enum { ST_F32 = 0, ST_F16 = 1, ST_BF16 = 2 } st_dtype;
+typedef enum { ST_F32 = 0, ST_F16 = 1, ST_BF16 = 2, ST_I8 = 3 } st_dtype;
 
 /* flags */
 #define ST_FLAG_ZEROS_PLUS_ONE 0x1u /* qzeros hold z - 1 (AutoGPTQ v1 files) */
 #define ST_FLAG_TILED 0x2u          /* weights in the tiled layout of st_gptq_i4_repack / st_int8_repack */
+#define ST_FLAG_NORM_PLUS_ONE 0x4u  /* st_qk_norm_rope_store: norm weights hold w - 1 (the reference's rmsnorm multiplies by 1 + w) */
+#define ST_FLAG_ROPE_PAIRS 0x8u     /* st_qk_norm_rope_store: rotates dims (2j, 2j + 1), not (j, j + rot / 2) */
 
 /* ------------------------------------------------------------ runtime */
 
@@ -344,6 +346,123 @@ int st_int8_gemm(st_context *ctx, const uint16_t *a, const int8_t *w, const floa
  * st_int8_tiled_bytes(K, N) bytes; pass ST_FLAG_TILED to st_int8_matvec. */
 size_t st_int8_tiled_bytes(int K, int N);
 int st_int8_repack(st_context *ctx, const int8_t *w, int8_t *w_tiled, int K, int N);
+
+/* ----------------------------------------- key-value cache and attention */
+
+/* A paged key-value cache of one layer (device pointers, owned by the caller).
+ * Slot s is place s % page_size of page s / page_size; tokens lie in tiles of
+ * 16 places, so that the attention's matrix instructions take 16-byte (f16)
+ * or 8-byte (int8) pieces as they are, and whole tiles are contiguous:
+ *   k  [num_pages][n_kv_heads][page_size / 16][head_dim / 8][16][8]
+ *      eight dims of a token side by side
+ *   v  [num_pages][n_kv_heads][page_size / 16][2][head_dim][8]
+ *      eight places of a dim side by side: half h holds places 4 h .. 4 h + 3
+ *      and 8 + 4 h .. 8 + 4 h + 3 of the tile, in this order
+ *   k_scale, v_scale  f32 [num_pages][n_kv_heads][page_size], ST_I8 only: a
+ *      token's head is its int8 values times its scale
+ * dtype ST_F16 or ST_I8; page_size 16, 32, 64, 128 or 256; head_dim 64, 128
+ * or 256; every pointer 16-byte aligned. The reference keeps one contiguous
+ * f32 cache per sequence (fused_split_qknorm_kvstore.wgsl, src/model.rs:971-1029). */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int dtype;
+    int num_pages, page_size, n_kv_heads, head_dim;
+} st_kv_cache;
+
+/* RMS norms of the queries and keys of each head, their rotation, and the
+ * write of keys and values into the cache, in one launch: replaces
+ * fused_split_qknorm_kvstore.wgsl:1-230 (dispatched between q|k|v and the
+ * attention, src/model.rs:715-726).
+ *   q, k, v   T tokens of x_dtype (ST_F32 or ST_F16); *_stride elements from
+ *             one token to the next (the three may be parts of one q|k|v
+ *             row); heads of k and v side by side, those of q q_head_stride
+ *             elements apart (2 head_dim where each head's query is followed
+ *             by its gate, as the reference's gated q). q and q_out NULL:
+ *             keys and values only.
+ *   q_weight, k_weight  f32 [head_dim] or NULL (no norm):
+ *             y = x / sqrt(mean(x^2) + eps) * w (1 + w: ST_FLAG_NORM_PLUS_ONE)
+ *   cos, sin  f32 [n_pos][rot / 2] or both NULL (no rotation): the first rot
+ *             dims (a multiple of 16) of q and k at the token's position,
+ *             dims (j, j + rot / 2), or (2j, 2j + 1) with ST_FLAG_ROPE_PAIRS:
+ *             (a, b) -> (a c - b s, b c + a s). Positions of several axes:
+ *             tables of one row per token.
+ *   positions int32 [T] (NULL without rotation); a token whose position is
+ *             not in [0, n_pos) gets NaN queries and is not stored
+ *   slots     int32 [T]; a slot outside the cache (a negative one: padding)
+ *             is not written
+ *   q_out     [T][n_heads][head_dim] of q_dtype (ST_F32 or ST_F16)
+ * f32 arithmetic, one rounding to what is stored. An int8 cache gets, for
+ * each token and head, scale = max|y| / 127 and round(y / scale). Two tokens
+ * of one call with one slot: which of them stays is undefined. Pointers and
+ * strides in whole 16 bytes. */
+int st_qk_norm_rope_store(st_context *ctx, const st_kv_cache *cache, const void *q, const void *k, const void *v,
+                          int x_dtype, int64_t q_stride, int64_t k_stride, int64_t v_stride, int q_head_stride,
+                          const float *q_weight, const float *k_weight, float eps, const float *cos,
+                          const float *sin, int rot, int n_pos, const int32_t *positions, const int32_t *slots,
+                          void *q_out, int q_dtype, int T, int n_heads, uint32_t flags);
+
+/* Cached tokens read back, dequantised: k_out and v_out [T][n_kv_heads]
+ * [head_dim] of out_dtype (ST_F32 or ST_F16, int8 values times their scale
+ * rounded once). A slot outside the cache reads as zeros. For a prefix taken
+ * out of a cache or moved to another (the reference copies whole cache
+ * buffers, src/model.rs:1021-1029). */
+int st_kv_read(st_context *ctx, const st_kv_cache *cache, const int32_t *slots, void *k_out, void *v_out,
+               int out_dtype, int T);
+
+/* Attention of new rows over the cache: rows of sequence b are q_start[b] ..
+ * q_start[b + 1] (NULL: one row for each sequence, T == B), the newest of its
+ * kv_len[b] tokens, all of them in the cache already (so row i of n has
+ * position kv_len - n + i). Replaces gqa_attention_head.wgsl:1-124,
+ * gqa_reduce.wgsl:1-65 and sigmoid_mul.wgsl (src/model.rs:540-592).
+ *   s_j = scale q . k_j, capped cap tanh(s_j / cap) where cap > 0, plus
+ *   slopes[head] (j - position) where slopes (f32 [n_heads]) is given;
+ *   key j is visible if j <= position and, where window > 0, j > position -
+ *   window; out = sum_j softmax(s)_j v_j over the visible keys (a row that
+ *   sees none: zeros), times sigmoid(gate) where gate is given
+ *   q, out    [T][n_heads][head_dim] of q_dtype, out_dtype (ST_F32 or ST_F16);
+ *             n_heads a multiple of the cache's heads, head h reads key head
+ *             h / (n_heads / n_kv_heads)
+ *   table     int32 [B][table_stride]: page of tokens page_size i ..; entries
+ *             past a sequence's last token are not read; tokens of a page
+ *             outside the cache are never read and count as not visible
+ *   kv_len    int32 [B], q_start int32 [B + 1]: device arrays; a captured
+ *             graph may be replayed after they, table and the cache changed
+ *             (out-of-range values are clamped to the table and to T; if
+ *             q_start decreases anywhere, out may be left as it is)
+ *   gate      gate_dtype, gate_stride elements between tokens,
+ *             gate_head_stride between heads (the gates of the reference's
+ *             gated q lie beside its queries)
+ * Rows of q and out outside every sequence are left alone. f32 scores,
+ * softmax and sums. With f32 q or out the products keep 22 bits of q and of
+ * the softmax weights; with f16 both, the weights are rounded to f16. Chunks
+ * of a long cache meet in the context workspace, in a fixed order. */
+int st_paged_attention(st_context *ctx, const st_kv_cache *cache, const void *q, int q_dtype, const int32_t *table,
+                       int table_stride, const int32_t *kv_len, const int32_t *q_start, float scale, float cap,
+                       int window, const float *slopes, const void *gate, int gate_dtype, int64_t gate_stride,
+                       int gate_head_stride, void *out, int out_dtype, int T, int B, int n_heads);
+
+/* ------------------------------------------------------------ logits */
+
+/* Log probabilities of given tokens, their rank, the entropy and the top
+ * alternatives of M rows of logits, in one pass. The reference reads its
+ * logits back and samples on the CPU (src/model.rs:836-968).
+ *   logits    [M] rows of V, `stride` elements apart, dtype ST_F32 or ST_F16
+ *   tokens    int32 [M] or NULL (then neither logprob nor rank)
+ *   logprob   f32 [M] or NULL: log softmax(logits)[token], natural logarithm;
+ *             NaN for a token outside the vocabulary
+ *   entropy   f32 [M] or NULL: -sum p log p
+ *   rank      int32 [M] or NULL: how many tokens come before the given one by
+ *             (value, lower index first); -1 for one outside the vocabulary
+ *   top_ids   int32 [M][top], top_logprobs f32 [M][top] or NULL: the `top`
+ *             first tokens in that order; top 0..32, at most V
+ * -inf logits are tokens of probability 0. A row with a NaN, a +inf or
+ * nothing but -inf has no distribution: its log probabilities and entropy
+ * are NaN (a NaN orders as +inf). V <= 2^20. f32 arithmetic; a likely
+ * token's log probability keeps f32's relative precision down to 0. */
+int st_token_logprobs(st_context *ctx, const void *logits, int dtype, int64_t stride, const int32_t *tokens,
+                      float *logprob, float *entropy, int32_t *rank, int32_t *top_ids, float *top_logprobs,
+                      int M, int V, int top);
 
 #ifdef __cplusplus
 }

@@ -16,9 +16,11 @@ HEADER = os.path.join(ROOT, "include", "shady_hip.h")
 
 ST_OK = 0
 ST_ERR_WORKSPACE = 6
-ST_F32, ST_F16, ST_BF16 = 0, 1, 2
+ST_F32, ST_F16, ST_BF16, ST_I8 = 0, 1, 2, 3
 ST_FLAG_ZEROS_PLUS_ONE = 0x1
 ST_FLAG_TILED = 0x2
+ST_FLAG_NORM_PLUS_ONE = 0x4
+ST_FLAG_ROPE_PAIRS = 0x8
 
 # st_tune (include/shady_hip.h): kernel-path overrides of one context
 TUNE_KNOBS = ("DECODE_KERNEL", "STAGE_MODE", "STAGE_ROUNDS", "WAVES", "NO_COOP", "ONE_TILE", "NO_CHUNK", "NO_KSPLIT",
@@ -47,6 +49,16 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _U32 = ctypes.c_uint32
 _SZ = ctypes.c_size_t
+_I64 = ctypes.c_int64
+_F = ctypes.c_float
+
+
+class KvCacheStruct(ctypes.Structure):
+    """st_kv_cache."""
+
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("dtype", _I), ("num_pages", _I),
+                ("page_size", _I), ("n_kv_heads", _I), ("head_dim", _I)]
+
 
 _SIGNATURES = {
     "st_last_error": (ctypes.c_char_p, []),
@@ -84,6 +96,11 @@ _SIGNATURES = {
     "st_int8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _U32]),
     "st_int8_tiled_bytes": (_SZ, [_I, _I]),
     "st_int8_repack": (_I, [_P, _P, _P, _I, _I]),
+    "st_qk_norm_rope_store": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P, _I,
+                                   _I, _I, _U32]),
+    "st_kv_read": (_I, [_P, _P, _P, _P, _P, _I, _I]),
+    "st_paged_attention": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _F, _F, _I, _P, _P, _I, _I64, _I, _P, _I, _I, _I, _I]),
+    "st_token_logprobs": (_I, [_P, _P, _I, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _I]),
 }
 
 _lib = None

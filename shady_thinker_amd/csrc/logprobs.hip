@@ -1,0 +1,368 @@
+// Log probabilities of given tokens, with their rank, the entropy and the top
+// alternatives of rows of logits (st_token_logprobs), in one pass. The
+// reference reads the logits back and samples on the CPU (src/model.rs:836-968).
+//
+// Of a row x with maximum m and S = sum exp(x - m) over all but one maximum:
+//   log p_j = (x_j - m) - log1p(S),   H = log1p(S) - T / (1 + S),
+//   T = sum exp(x - m) (x - m)
+// (leaving the maximum's own 1 out of the sum keeps a likely token's small
+// -log p exact to f32's last bits, not to 2^-24).
+// Bound by HBM (each logit once). A workgroup takes a chunk of a row into
+// registers; each wave has (m, S, T) of its own and they meet in LDS. The top
+// tokens: of 64 lanes' largest values the k-th is a lower bound of the wave's
+// k-th largest logit, so only logits from the largest such bound of the four
+// waves on (k and a few more) are candidates; these are ranked among each
+// other by value, then index. The last chunk of a row to count in joins the
+// chunks (the counter protocol of the split-K kernels, see qmv_kernel.hpp),
+// its top tokens found in the same way among the chunks'.
+#include "common.hpp"
+
+#include <algorithm>
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxTop = 32;
+constexpr int kMergeEach = 16;                        // of the joined chunks' top tokens, per thread
+constexpr int kMaxMerged = kMergeEach * kThreads;     // chunks times top
+constexpr int kCandidates = 512;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
+constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
+
+struct Args {
+    const void *x;
+    int64_t stride;
+    const int32_t *tokens;
+    float *logprob, *entropy;
+    int32_t *rank, *top_ids;
+    float *top_logprobs;
+    int V, top, chunks;
+    float *part;       // [row][chunk] of part_words(top)
+    unsigned *cnt;     // [row]
+};
+
+// A chunk's partial result: m, S, T, rank, then `top` keys of two words.
+__host__ __device__ constexpr int part_words(int top) { return 4 + 2 * top; }
+
+// Order of (value, index) as an unsigned: larger value first, then lower
+// index. Equal zeros of both signs.
+__device__ __forceinline__ unsigned order_of(float v) {
+    const unsigned u = __float_as_uint(v + 0.0f);
+    return (int)u < 0 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float((int)o < 0 ? o & 0x7FFFFFFFu : ~o); }
+
+struct Sums {
+    float m, s, t;  // t in units of log 2
+};
+
+// The sums of two disjoint parts (m -inf: nothing in it).
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    if (b.m > a.m) {
+        const Sums c = a;
+        a = b, b = c;
+    }
+    if (b.m == -INFINITY) return a;
+    const float d = (b.m - a.m) * kLog2e, f = __builtin_amdgcn_exp2f(d), w = f * (1.0f + b.s);
+    a.s += w;
+    a.t += f * b.t + (w > 0.0f ? w * d : 0.0f);
+    return a;
+}
+
+// The top `k` of a workgroup's elements (value x[j], index idx(j), present
+// where idx(j) >= 0), as keys in order in `out`, which has room for k; fewer
+// than k present: keys 0 after them.
+struct TopShared {
+    unsigned long long cand[kCandidates];
+    unsigned long long best[kWaves];
+    unsigned bound[kWaves];
+    int n;
+};
+template <int E, typename Idx>
+__device__ void top_of_block(const float (&x)[E], Idx idx, int k, TopShared &sh, unsigned long long *out) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    unsigned mine = 0;  // this lane's largest (0: none present)
+#pragma unroll
+    for (int j = 0; j < E; ++j) mine = max(mine, idx(j) >= 0 ? order_of(x[j]) : 0u);
+    // the largest 20-bit bound that k lanes reach
+    unsigned bound = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 12; --bit) {
+        const unsigned b = bound | 1u << bit;
+        if (__popcll(__ballot(mine >= b)) >= k) bound = b;
+    }
+    __syncthreads();  // (sh and out may be read from before)
+    if (lane == 0) sh.bound[wave] = bound;
+    if (tid == 0) sh.n = 0;
+    for (int i = tid; i < k; i += kThreads) out[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) bound = max(bound, sh.bound[w]);
+    if (mine >= bound && mine) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int i = idx(j);
+            const unsigned o = order_of(x[j]);
+            if (i >= 0 && o >= bound) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kCandidates) sh.cand[at] = (unsigned long long)o << 32 | ~(unsigned)i;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= kCandidates) {
+        for (int c = tid; c < n; c += kThreads) {
+            const unsigned long long key = sh.cand[c];
+            int r = 0;
+            for (int i = 0; i < n; ++i) r += sh.cand[i] > key;
+            if (r < k) out[r] = key;
+        }
+        __syncthreads();
+        return;
+    }
+    // very many equal values (rows of few distinct logits): one at a time
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < k; ++r) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int i = idx(j);
+            const unsigned long long key = i >= 0 ? (unsigned long long)order_of(x[j]) << 32 | ~(unsigned)i : 0ull;
+            if (key < last && key > best) best = key;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned long long o = __shfl_xor(best, d);
+            best = o > best ? o : best;
+        }
+        __syncthreads();
+        if (lane == 0) sh.best[wave] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        if (tid == 0) out[r] = best;
+        last = best;
+    }
+    __syncthreads();
+}
+
+template <bool F16, int E>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
+    constexpr int VEC = F16 ? 8 : 4, NL = E / VEC;
+    using X = std::conditional_t<F16, _Float16, float>;
+    __shared__ TopShared sh;
+    __shared__ Sums s_sums[kWaves];
+    __shared__ int s_rank[kWaves];
+    __shared__ unsigned long long s_top[kMaxTop];
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.y, chunk = blockIdx.x;
+    const X *const xr = static_cast<const X *>(a.x) + row * a.stride;
+    // whole 16-byte pieces from the piece that the row starts in
+    const int skew = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(X));
+    const int first = chunk * (kThreads * E) - skew + tid * VEC;  // index of the thread's first element
+    const int token = a.tokens ? a.tokens[row] : -1;
+    const bool known = token >= 0 && token < a.V;
+    float x[E];
+#pragma unroll
+    for (int l = 0; l < NL; ++l) {
+        const int i0 = first + l * (kThreads * VEC);
+        if (i0 >= 0 && i0 + VEC <= a.V) {
+            if constexpr (F16) {
+                const half8 v = __builtin_nontemporal_load(reinterpret_cast<const half8 *>(xr + i0));
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[l * VEC + i] = (float)v[i];
+            } else {
+                const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(xr + i0));
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[l * VEC + i] = v[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) x[l * VEC + i] = i0 + i >= 0 && i0 + i < a.V ? (float)xr[i0 + i] : -INFINITY;
+        }
+    }
+    const float xt = known ? (float)xr[token] : 0.0f;
+    // (a NaN orders as +inf: the row's results are NaN either way)
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = x[j] != x[j] ? INFINITY : x[j];
+    auto idx = [&](int j) {
+        const int i = first + j / VEC * (kThreads * VEC) + j % VEC;
+        return i < a.V ? i : -1;
+    };
+
+    // ---- this wave's sums
+    Sums w;
+    w.m = x[0];
+#pragma unroll
+    for (int j = 1; j < E; ++j) w.m = fmaxf(w.m, x[j]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) w.m = fmaxf(w.m, __shfl_xor(w.m, d));
+    w.s = w.t = 0.0f;
+    int equal = 0;
+    {
+        const float base = w.m == -INFINITY ? 0.0f : w.m;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool top = x[j] == w.m;
+            equal += __popcll(__ballot(top));
+            const float d = fmaxf((x[j] - base) * kLog2e, -300.0f), e = top ? 0.0f : __builtin_amdgcn_exp2f(d);
+            w.s += e;
+            w.t = fmaf(e, d, w.t);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) w.s += __shfl_xor(w.s, d), w.t += __shfl_xor(w.t, d);
+        w.s += (float)(equal - 1);
+    }
+    int ahead = 0;
+    if (known) {
+        const float xk = xt != xt ? INFINITY : xt;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int i = idx(j);
+            ahead += __popcll(__ballot(i >= 0 && (x[j] > xk || (x[j] == xk && i < token))));
+        }
+    }
+    if (lane == 0) s_sums[wave] = w, s_rank[wave] = ahead;
+    if (a.top > 0)
+        top_of_block(x, idx, a.top, sh, s_top);
+    else
+        __syncthreads();
+    Sums sum = s_sums[0];
+    ahead = s_rank[0];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) sum = join(sum, s_sums[k]), ahead += s_rank[k];
+
+    // ---- the row's chunks meet
+    if (a.chunks > 1) {
+        const int words = part_words(a.top);
+        const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(a.part + (size_t)row * a.chunks * words), (short)0, a.chunks * words * 4, kRsrcWord3);
+        const int at = chunk * words * 4;
+        if (tid == 0)
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u32x4{__float_as_uint(sum.m), __float_as_uint(sum.s), __float_as_uint(sum.t), (unsigned)ahead}, rp, at, 0, kCoherent);
+        if (tid < a.top)
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{(unsigned)s_top[tid], (unsigned)(s_top[tid] >> 32)}, rp, at + 16 + tid * 8, 0,
+                                                  kCoherent);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part is in memory
+        __syncthreads();
+        if (tid == 0) {
+            const unsigned done = __hip_atomic_fetch_add(&a.cnt[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            s_last = done == (unsigned)a.chunks - 1;
+            if (s_last) __hip_atomic_store(&a.cnt[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        }
+        __syncthreads();
+        if (!s_last) return;
+        Sums g{-INFINITY, 0.0f, 0.0f};
+        int r = 0;
+        for (int c = tid; c < a.chunks; c += kThreads) {
+            const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, c * words * 4, 0, kCoherent));
+            const unsigned v0 = v.x, v1 = v.y, v2 = v.z, v3 = v.w;
+            g = join(g, Sums{__uint_as_float(v0), __uint_as_float(v1), __uint_as_float(v2)});
+            r += (int)v3;
+        }
+        float kx[kMergeEach];
+        int ki[kMergeEach];
+        const int keys = a.chunks * a.top;
+#pragma unroll
+        for (int j = 0; j < kMergeEach; ++j) {
+            const int i = tid + j * kThreads;
+            kx[j] = -INFINITY, ki[j] = -1;
+            if (i < keys) {
+                const u32x2 v = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_raw_buffer_load_b64(rp, (i / a.top * words + 4 + i % a.top * 2) * 4, 0, kCoherent));
+                const unsigned lo = v.x, hi = v.y;
+                if (hi) kx[j] = value_of(hi), ki[j] = (int)~lo;
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            g = join(g, Sums{__shfl_xor(g.m, d), __shfl_xor(g.s, d), __shfl_xor(g.t, d)});
+            r += __shfl_xor(r, d);
+        }
+        __syncthreads();
+        if (lane == 0) s_sums[wave] = g, s_rank[wave] = r;
+        __syncthreads();
+        sum = s_sums[0], ahead = s_rank[0];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) sum = join(sum, s_sums[k]), ahead += s_rank[k];
+        if (a.top > 0) top_of_block(kx, [&](int j) { return ki[j]; }, a.top, sh, s_top);
+    }
+
+    // ---- the row's results
+    const bool finite = fabsf(sum.m) < INFINITY;  // (an infinity, a NaN, or nothing but -inf: no distribution)
+    const float base = finite ? sum.m : __builtin_nanf(""), logs = log1pf(sum.s);
+    if (tid == 0) {
+        if (a.logprob) a.logprob[row] = known ? (xt - base) - logs : __builtin_nanf("");
+        if (a.rank) a.rank[row] = known ? ahead : -1;
+        if (a.entropy) a.entropy[row] = finite ? logs - sum.t * kLn2 / (1.0f + sum.s) : __builtin_nanf("");
+    }
+    if (tid < a.top) {
+        const unsigned long long key = s_top[tid];
+        a.top_ids[(int64_t)row * a.top + tid] = (int32_t)~(unsigned)key;
+        if (a.top_logprobs) a.top_logprobs[(int64_t)row * a.top + tid] = (value_of((unsigned)(key >> 32)) - base) - logs;
+    }
+}
+
+template <bool F16, int E>
+int launch_rows(st_context *ctx, Args a, int M) {
+    const int vec = F16 ? 8 : 4;
+    // (a row that starts inside a piece reaches that much further)
+    a.chunks = (int)(((int64_t)a.V + vec - 1 + kThreads * E - 1) / (kThreads * E));
+    const size_t row = (size_t)a.chunks * part_words(a.top) * sizeof(float);
+    const int most = a.chunks == 1 ? 65535 : (int)std::min<size_t>(st::kSplitCounters, ctx->ws_bytes / row);
+    if (most < 1) return st::fail(ST_ERR_WORKSPACE, "st_token_logprobs: a row of %d logits needs %zu bytes of workspace", a.V, row);
+    a.part = ctx->ws;
+    a.cnt = ctx->split_counters;
+    const int size = F16 ? 2 : 4;
+    for (int m = 0; m < M; m += most) {
+        Args b = a;
+        const int n = std::min(most, M - m);
+        b.x = static_cast<const char *>(a.x) + (int64_t)m * a.stride * size;
+        if (a.tokens) b.tokens = a.tokens + m;
+        if (a.logprob) b.logprob = a.logprob + m;
+        if (a.entropy) b.entropy = a.entropy + m;
+        if (a.rank) b.rank = a.rank + m;
+        if (a.top_ids) b.top_ids = a.top_ids + (int64_t)m * a.top;
+        if (a.top_logprobs) b.top_logprobs = a.top_logprobs + (int64_t)m * a.top;
+        st::launch(ctx, logprobs_kernel<F16, E>, dim3((unsigned)a.chunks, (unsigned)n), dim3(kThreads), 0, b);
+        if (int rc = st::launch_check("logprobs_kernel")) return rc;
+    }
+    return ST_OK;
+}
+
+template <bool F16>
+int by_size(st_context *ctx, const Args &a, int M) {
+    // Few rows: small chunks, so that every CU has some (one row of 151936: 75
+    // workgroups); many: large ones, whose fixed cost is a quarter per logit.
+    const bool large = (int64_t)M * ((a.V + 8191) / 8192) >= 2 * ctx->num_cus || (int64_t)((a.V + 2054) / 2048) * a.top > kMaxMerged;
+    return large ? launch_rows<F16, 32>(ctx, a, M) : launch_rows<F16, 8>(ctx, a, M);
+}
+
+}  // namespace
+
+extern "C" int st_token_logprobs(st_context *ctx, const void *logits, int dtype, int64_t stride, const int32_t *tokens,
+                                 float *logprob, float *entropy, int32_t *rank, int32_t *top_ids, float *top_logprobs, int M,
+                                 int V, int top) {
+    const char *const fn = "st_token_logprobs";
+    if (!ctx || !logits) return st::fail(ST_ERR_INVALID, "%s: NULL argument", fn);
+    if (dtype != ST_F32 && dtype != ST_F16) return st::fail(ST_ERR_INVALID, "%s: dtype %d (f32 or f16)", fn, dtype);
+    if (!tokens && (logprob || rank)) return st::fail(ST_ERR_INVALID, "%s: logprob and rank need tokens", fn);
+    if (top < 0 || top > kMaxTop) return st::fail(ST_ERR_SHAPE, "%s: top=%d (at most %d)", fn, top, kMaxTop);
+    if (top > 0 && !top_ids) return st::fail(ST_ERR_INVALID, "%s: top=%d without top_ids", fn, top);
+    if (top == 0 && (top_ids || top_logprobs)) top_ids = nullptr, top_logprobs = nullptr;
+    if (M < 1 || V < 1 || V > (1 << 20) || top > V || stride < V)
+        return st::fail(ST_ERR_SHAPE, "%s: M=%d, V=%d (at most 2^20), stride %lld, top=%d", fn, M, V, (long long)stride, top);
+    if ((reinterpret_cast<uintptr_t>(logits) & (dtype == ST_F32 ? 3 : 1)) != 0)
+        return st::fail(ST_ERR_ALIGN, "%s: logits not aligned to their type", fn);
+    Args a{logits, stride, tokens, logprob, entropy, rank, top_ids, top_logprobs, V, top, 0, nullptr, nullptr};
+    return dtype == ST_F16 ? by_size<true>(ctx, a, M) : by_size<false>(ctx, a, M);
+}
