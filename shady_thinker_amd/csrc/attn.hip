@@ -478,7 +478,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's partial results are in memory
     __syncthreads();
     if (tid == 0) {
-        unsigned *const cnt = a.cnt + it.counter * a.c.heads + h;
+        unsigned *const cnt = a.cnt + st::spread_counter(it.counter * a.c.heads + h);
         const unsigned done = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         s_last = done == (unsigned)it.chunks - 1;
         if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
