@@ -35,110 +35,10 @@ namespace {
 using namespace st::attn;
 
 constexpr int kWaves = 4;
-constexpr int kMostRows = 1 << 24;      // row blocks of one call
+constexpr int kStep = 32;  // keys of a step of one wave
 constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
 constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
 constexpr float kShift = 14.0f;         // weights are held times 2^14: f16 keeps them normal down to 2^-28
-
-// One workgroup's share: row block rb of sequence b, chunk `chunk` of its
-// `chunks`, steps [s0, s1) of the sequence's keys; item ids of the chunks are
-// first + chunk * blocks.
-struct Item {
-    Seq s;
-    int b, rb, blocks, chunk, chunks, s0, s1, first, counter;
-};
-
-template <int PB>
-__device__ __forceinline__ int blocks_of(const Args &a, const Seq &s) {
-    return (s.q * a.group + PB - 1) / PB;
-}
-__device__ __forceinline__ int steps_of(const Args &a, const Seq &s) {
-    return (s.kv - first_key(a, s) + kStep - 1) / kStep;
-}
-
-// C: chunks of C steps so that all items fit the grid: sum over blocks of
-// ceil(steps / C) <= work / C + blocks <= G.
-__device__ __forceinline__ int chunk_steps(const Args &a, unsigned long long work, int blocks, int longest) {
-    if (!a.split) return INT_MAX;
-    const unsigned room = (unsigned)max(a.G - blocks, 1);
-    const unsigned long long up = work + room - 1;
-    unsigned long long c = up >> 32 ? up / room : (unsigned)up / room;
-    c = max(c, (unsigned long long)((longest + kMaxChunks - 1) / kMaxChunks));
-    c = max((c + kWaves - 1) / kWaves * kWaves, (unsigned long long)kWaves);  // (a step for every wave)
-    return c > INT_MAX ? INT_MAX : (int)c;
-}
-
-template <int PB>
-__device__ bool find_item(const Args &a, int w, Item &it) {
-    const int lane = threadIdx.x & 63;
-    if (a.B == 1) {
-        it.s = seq_of(a, 0);
-        it.b = 0;
-        it.blocks = blocks_of<PB>(a, it.s);
-        if (!it.blocks) return false;
-        const int steps = steps_of(a, it.s), C = chunk_steps(a, (unsigned long long)it.blocks * steps, it.blocks, steps);
-        it.chunks = max(1, (int)(((int64_t)steps + C - 1) / C));
-        if (w >= it.blocks * it.chunks) return false;
-        it.rb = w % it.blocks, it.chunk = w / it.blocks;
-        it.first = it.rb, it.counter = it.rb;
-        it.s0 = min((int64_t)it.chunk * C, (int64_t)steps), it.s1 = min((int64_t)(it.chunk + 1) * C, (int64_t)steps);
-        return true;
-    }
-    unsigned long long work = 0;
-    int blocks = 0, longest = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = b0 + lane;
-        if (b < a.B) {
-            const Seq s = seq_of(a, b);
-            const int n = blocks_of<PB>(a, s), steps = steps_of(a, s);
-            work += (unsigned long long)n * steps;
-            blocks = min(blocks + min(n, kMostRows), kMostRows);
-            longest = max(longest, n ? steps : 0);
-        }
-    }
-    work = wave_sum(work);
-    blocks = wave_sum(blocks);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) longest = max(longest, __shfl_xor(longest, d));
-    // (more row blocks than T rows have: q_start decreases somewhere. The
-    // counters and the grid are made for a.rows, so nothing is computed)
-    if (uniform(blocks) > a.rows) return false;
-    const int C = chunk_steps(a, work, uniform(blocks), uniform(longest));
-    int items = 0, rows = 0;  // before this turn's sequences
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = b0 + lane;
-        Seq s{0, 0, 0};
-        int n = 0, chunks = 1, steps = 0;
-        if (b < a.B) {
-            s = seq_of(a, b);
-            n = blocks_of<PB>(a, s), steps = steps_of(a, s);
-            chunks = max(1, (int)(((int64_t)steps + C - 1) / C));
-        }
-        int upto = n * chunks, rows_upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int i = __shfl_up(upto, d), r = __shfl_up(rows_upto, d);
-            if (lane >= d) upto += i, rows_upto += r;
-        }
-        const unsigned long long mine = __ballot(items + upto > w);
-        if (mine) {
-            const int l = __builtin_ctzll(mine);
-            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            it.b = b0 + l;
-            it.s = Seq{of(s.q0), of(s.q), of(s.kv)};
-            it.blocks = of(n), it.chunks = of(chunks);
-            const int begin = items + of(upto) - it.blocks * it.chunks, idx = w - begin;
-            it.rb = idx % it.blocks, it.chunk = idx / it.blocks;
-            it.first = begin + it.rb;
-            it.counter = rows + of(rows_upto) - it.blocks + it.rb;
-            const int64_t st = of(steps);
-            it.s0 = (int)min((int64_t)it.chunk * C, st), it.s1 = (int)min((int64_t)(it.chunk + 1) * C, st);
-            return true;
-        }
-        items += __builtin_amdgcn_readlane(upto, 63), rows += __builtin_amdgcn_readlane(rows_upto, 63);
-    }
-    return false;
-}
 
 template <int HD, bool I8, bool SPLIT>
 struct Frag {
@@ -177,7 +77,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     const int col = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.y;
     Item it;
-    if (!find_item<PB>(a, (int)blockIdx.x, it)) return;
+    if (!find_item<PB, kStep, kWaves>(a, (int)blockIdx.x, it)) return;
+    it = scalars(it);
 
     // ---- this lane's column: a (row, head) pair
     const int npair = it.s.q * a.group;
@@ -188,7 +89,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     const int pos = real ? p0 + tok : -1;
     const int low = a.window ? max(pos - a.window + 1, 0) : 0;  // keys low .. pos are visible
     // (uniform: the block's first and last rows' positions)
-    const int pmin = p0 + it.rb * PB / a.group, pmax = p0 + (min(it.rb * PB + PB, npair) - 1) / a.group;
+    const int pmin = p0 + scalar(it.rb * PB / a.group), pmax = p0 + scalar((min(it.rb * PB + PB, npair) - 1) / a.group);
     const int wmax = a.window ? pmax - a.window + 1 : 0;  // from here on a key is in every row's window
     const int wmin = a.window ? pmin - a.window + 1 : 0;  // before this it is in none's
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
@@ -242,7 +143,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     }
 
     // ---- the chunk's steps: this wave's are s0 + wave, + kWaves, ...
-    const int key0 = first_key(a, it.s);
+    const int key0 = first_key<kStep>(a, it.s);
     const int tile0 = key0 / 16, tiles = (it.s.kv + 15) / 16;  // tiles that hold a token
     const int tsh = a.c.tiles_shift();
     const int32_t *const table = a.table + (int64_t)it.b * a.table_stride;
@@ -444,8 +345,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
         const int g = it.rb * PB + p;
         row = it.s.q0 + g / a.group, hd = h * a.group + g % a.group;
     };
-    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, 0x7FFFFFFF, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, 0x7FFFFFFF, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, a.G * a.c.heads * PB * HD * 4, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, a.G * a.c.heads * PB * 8, kRsrcWord3);
     for (int i = tid; i < kQuads; i += 64 * kWaves) {
         const int p = i / (HD / 4), d = i % (HD / 4) * 4;
         if (p >= pairs_here) continue;
@@ -545,20 +446,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
 template <int HD, bool I8, bool SPLIT>
 int launch_attn(st_context *ctx, Args a) {
     constexpr int PB = SPLIT ? 8 : 16;
-    const int64_t rows = std::min<int64_t>(a.B, a.T) + (int64_t)a.T * a.group / PB + 1;  // row blocks at most
-    if (rows >= kMostRows) return st::fail(ST_ERR_SHAPE, "st_paged_attention: %d rows", a.T);
+    if (int rc = plan_cut(ctx, a, PB, HD, kStep, kWaves, 2 * ctx->num_cus / a.c.heads)) return rc;
     const int heads = a.c.heads;
-    const int64_t most_chunks = std::min<int64_t>(kMaxChunks, (a.capacity / kStep + 1 + kWaves - 1) / kWaves);
-    const size_t item = (size_t)heads * PB * (HD + 2) * sizeof(float);
-    int64_t extra = std::max<int64_t>(1, 2 * ctx->num_cus / heads);
-    extra = std::min(extra, rows * (most_chunks - 1));
-    extra = std::min(extra, (int64_t)(std::min<size_t>(ctx->ws_bytes, 0x7FFFFFFF) / item) - rows);
-    a.split = extra >= 1 && rows * heads <= st::kSplitCounters;
-    a.rows = (int)rows;
-    a.G = (int)(rows + (a.split ? extra : 0));
-    a.part = ctx->ws;
-    a.part_ml = ctx->ws + (size_t)a.G * heads * PB * HD;
-    a.cnt = ctx->split_counters;
     const size_t lds = (size_t)kWaves * PB * (HD + 4) * sizeof(float);
     auto kern = attn_kernel<HD, I8, SPLIT>;
     if (lds > 48 * 1024)
@@ -573,9 +462,37 @@ int by_type(st_context *ctx, const Args &a, bool i8, bool split) {
     return split ? launch_attn<HD, false, true>(ctx, a) : launch_attn<HD, false, false>(ctx, a);
 }
 
+// f16 rows of prompts go to the kernel with 128 pairs a workgroup.
+bool use_prompt(const st_context *ctx, const Args &a) {
+    return (int64_t)a.T * a.group >= 32 * (int64_t)a.B;
+}
+
 bool act_dtype(int d) { return d == ST_F32 || d == ST_F16; }
 
 }  // namespace
+
+namespace st {
+namespace attn {
+
+int plan_cut(st_context *ctx, Args &a, int pb, int hd, int step, int least, int64_t extra) {
+    const int64_t rows = std::min<int64_t>(a.B, a.T) + (int64_t)a.T * a.group / pb + 1;  // row blocks at most
+    if (rows >= kMostRows) return fail(ST_ERR_SHAPE, "st_paged_attention: %d rows", a.T);
+    const int heads = a.c.heads;
+    const int64_t most_chunks = std::min<int64_t>(kMaxChunks, (a.capacity / step + 1 + least - 1) / least);
+    const size_t item = (size_t)heads * pb * (hd + 2) * sizeof(float);
+    extra = std::min(extra, rows * (most_chunks - 1));
+    extra = std::min(extra, (int64_t)(std::min<size_t>(ctx->ws_bytes, 0x7FFFFFFF) / item) - rows);
+    a.split = extra >= 1 && rows * heads <= kSplitCounters;
+    a.rows = (int)rows;
+    a.G = (int)(rows + (a.split ? extra : 0));
+    a.part = ctx->ws;
+    a.part_ml = ctx->ws + (size_t)a.G * heads * pb * hd;
+    a.cnt = ctx->split_counters;
+    return ST_OK;
+}
+
+}  // namespace attn
+}  // namespace st
 
 extern "C" int st_paged_attention(st_context *ctx, const st_kv_cache *cache, const void *q, int q_dtype, const int32_t *table,
                                   int table_stride, const int32_t *kv_len, const int32_t *q_start, float scale, float cap,
@@ -605,8 +522,9 @@ extern "C" int st_paged_attention(st_context *ctx, const st_kv_cache *cache, con
     a.gate_stride = gate_stride, a.gate_head_stride = gate_head_stride;
     a.table_stride = table_stride, a.capacity = table_stride << a.c.page_shift;
     a.T = T, a.B = B, a.n_heads = n_heads, a.group = n_heads / a.c.heads;
-    a.window = window, a.scale = scale, a.cap = cap;
+    a.window = std::min(window, 1 << 30), a.scale = scale, a.cap = cap;
     a.q_f32 = q_dtype == ST_F32, a.gate_f32 = gate_dtype == ST_F32, a.out_f32 = out_dtype == ST_F32;
     const bool i8 = cache->dtype == ST_I8, split = a.q_f32 || a.out_f32;
+    if (!split && use_prompt(ctx, a)) return prompt_attention(ctx, a, i8, hd);
     return hd == 64 ? by_type<64>(ctx, a, i8, split) : hd == 128 ? by_type<128>(ctx, a, i8, split) : by_type<256>(ctx, a, i8, split);
 }

@@ -4,12 +4,13 @@
 
 #include "kvcache.hpp"
 
+#include <climits>
+
 namespace st {
 namespace attn {
 
 using namespace st::kv;
 
-constexpr int kStep = 32;            // keys of a step of one wave
 constexpr int kMaxChunks = 256;      // chunks of one sequence at most
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -34,6 +35,16 @@ struct Args {
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The same, certainly in a scalar register: the compiler drops the builtin for
+// a value that it knows to be uniform and then computes it in a vector one
+// where it came out of a division. Inside inline asm the wait states are the
+// writer's: one between a vector write and v_readfirstlane of it, five between
+// that write of a scalar and a vector load that reads it.
+__device__ __forceinline__ int scalar(int v) {
+    int r;
+    asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(r) : "v"(v));
+    return r;
+}
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // Sequence b's rows [q0, q0 + q) and tokens kv (with the rows'), within bounds
@@ -53,10 +64,11 @@ __device__ __forceinline__ Seq seq_of(const Args &a, int b) {
 }
 
 // First key that any of a sequence's rows sees, at a step's start.
+template <int STEP>
 __device__ __forceinline__ int first_key(const Args &a, const Seq &s) {
     if (!a.window) return 0;
-    const int64_t lo = (int64_t)s.kv - s.q + 1 - a.window;
-    return lo > 0 ? (int)lo & ~(kStep - 1) : 0;
+    const int lo = s.kv - s.q + 1 - a.window;  // (kv below 2^31, q at most 2^24, window at most 2^30)
+    return max(lo, 0) & ~(STEP - 1);
 }
 
 template <typename V>
@@ -64,6 +76,121 @@ __device__ __forceinline__ V wave_sum(V v) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
     return v;
+}
+
+// One workgroup's share: row block rb of sequence b, chunk `chunk` of its
+// `chunks`, steps [s0, s1) of the sequence's keys; item ids of the chunks are
+// first + chunk * blocks.
+struct Item {
+    Seq s;
+    int b, rb, blocks, chunk, chunks, s0, s1, first, counter;
+};
+
+constexpr int kMostRows = 1 << 24;   // row blocks of one call
+constexpr int kMostSteps = 1 << 27;  // steps of a sequence (of 16 keys at least)
+
+template <int PB>
+__device__ __forceinline__ int blocks_of(const Args &a, const Seq &s) {
+    return (s.q * a.group + PB - 1) / PB;
+}
+template <int STEP>
+__device__ __forceinline__ int steps_of(const Args &a, const Seq &s) {
+    return (s.kv - first_key<STEP>(a, s) + STEP - 1) / STEP;
+}
+
+// C: chunks of C steps so that all items fit the grid: sum over blocks of
+// ceil(steps / C) <= work / C + blocks <= G. A multiple of LEAST.
+template <int LEAST>
+__device__ __forceinline__ int chunk_steps(const Args &a, unsigned long long work, int blocks, int longest) {
+    if (!a.split) return kMostSteps;
+    const unsigned room = (unsigned)max(a.G - blocks, 1);
+    const unsigned long long up = work + room - 1;
+    unsigned long long c = up >> 32 ? up / room : (unsigned)up / room;
+    c = max(c, (unsigned long long)((longest + kMaxChunks - 1) / kMaxChunks));
+    c = max((c + LEAST - 1) / LEAST * LEAST, (unsigned long long)LEAST);
+    return c > kMostSteps ? kMostSteps : (int)c;
+}
+
+// Item w of the call (the same for every wave), or false: there is none.
+template <int PB, int STEP, int LEAST>
+__device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
+    const int lane = threadIdx.x & 63;
+    if (a.B == 1) {
+        it.s = seq_of(a, 0);
+        it.s = Seq{uniform(it.s.q0), uniform(it.s.q), uniform(it.s.kv)};
+        it.b = 0;
+        it.blocks = blocks_of<PB>(a, it.s);
+        if (!it.blocks) return false;
+        const int steps = steps_of<STEP>(a, it.s), C = chunk_steps<LEAST>(a, (unsigned long long)it.blocks * steps, it.blocks, steps);
+        it.chunks = max(1, (steps + C - 1) / C);
+        if (w >= it.blocks * it.chunks) return false;
+        it.rb = w % it.blocks, it.chunk = w / it.blocks;
+        it.first = it.rb, it.counter = it.rb;
+        it.s0 = min(it.chunk * C, steps), it.s1 = min(it.s0 + C, steps);
+        return true;
+    }
+    unsigned long long work = 0;
+    int blocks = 0, longest = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int b = b0 + lane;
+        if (b < a.B) {
+            const Seq s = seq_of(a, b);
+            const int n = blocks_of<PB>(a, s), steps = steps_of<STEP>(a, s);
+            work += (unsigned long long)n * steps;
+            blocks = min(blocks + min(n, kMostRows), kMostRows);
+            longest = max(longest, n ? steps : 0);
+        }
+    }
+    work = wave_sum(work);
+    blocks = wave_sum(blocks);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) longest = max(longest, __shfl_xor(longest, d));
+    // (more row blocks than T rows have: q_start decreases somewhere. The
+    // counters and the grid are made for a.rows, so nothing is computed)
+    if (uniform(blocks) > a.rows) return false;
+    const int C = chunk_steps<LEAST>(a, work, uniform(blocks), uniform(longest));
+    int items = 0, rows = 0;  // before this turn's sequences
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int b = b0 + lane;
+        Seq s{0, 0, 0};
+        int n = 0, chunks = 1, steps = 0;
+        if (b < a.B) {
+            s = seq_of(a, b);
+            n = blocks_of<PB>(a, s), steps = steps_of<STEP>(a, s);
+            chunks = max(1, (steps + C - 1) / C);
+        }
+        int upto = n * chunks, rows_upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int i = __shfl_up(upto, d), r = __shfl_up(rows_upto, d);
+            if (lane >= d) upto += i, rows_upto += r;
+        }
+        const unsigned long long mine = __ballot(items + upto > w);
+        if (mine) {
+            const int l = __builtin_ctzll(mine);
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            it.b = b0 + l;
+            it.s = Seq{of(s.q0), of(s.q), of(s.kv)};
+            it.blocks = of(n), it.chunks = of(chunks);
+            const int begin = items + of(upto) - it.blocks * it.chunks, idx = w - begin;
+            it.rb = idx % it.blocks, it.chunk = idx / it.blocks;
+            it.first = begin + it.rb;
+            it.counter = rows + of(rows_upto) - it.blocks + it.rb;
+            const int st = of(steps);
+            it.s0 = min(it.chunk * C, st), it.s1 = min(it.s0 + C, st);
+            return true;
+        }
+        items += __builtin_amdgcn_readlane(upto, 63), rows += __builtin_amdgcn_readlane(rows_upto, 63);
+    }
+    return false;
+}
+
+// An item's fields as scalars (once it is known that there is one): what is
+// derived from them (page loads, loop bounds) has to be, or the compiler takes
+// vector loads and waits for them among the pieces in flight.
+__device__ __forceinline__ Item scalars(const Item &it) {
+    return Item{Seq{scalar(it.s.q0), scalar(it.s.q), scalar(it.s.kv)}, scalar(it.b), scalar(it.rb), scalar(it.blocks),
+                scalar(it.chunk), scalar(it.chunks), scalar(it.s0), scalar(it.s1), scalar(it.first), scalar(it.counter)};
 }
 
 // Where the output's eight or four values go: times sigmoid(gate) where there
@@ -93,6 +220,13 @@ __device__ __forceinline__ void store_out(const Args &a, f32x4 o, int row, int h
             half4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
     }
 }
+
+// The cut of a call into row blocks of pb pairs and chunks of steps: a.G and
+// what goes with it; `extra` chunks more than row blocks at most.
+int plan_cut(st_context *ctx, Args &a, int pb, int hd, int step, int least, int64_t extra);
+
+// prompt.hip: f16 q and out, checked by the caller.
+int prompt_attention(st_context *ctx, const Args &a, bool i8, int hd);
 
 }  // namespace attn
 }  // namespace st

@@ -1,0 +1,459 @@
+// Attention of prompts over the paged cache (st_paged_attention, f16 q and
+// out, many rows of a sequence). No reference counterpart: it prefills token
+// by token (src/inference.rs:93-95).
+//
+// prompt_kernel: out^T = V^T P^T, P = softmax(K Q^T scale) as attn_kernel
+// (attn.hip), on v_mfma_f32_32x32x16_f16: a workgroup takes 128 (row, head)
+// pairs of one key head, 32 columns a wave, and goes over the keys once, KT at
+// a time.
+//  * K and V tiles are double-buffered in LDS, shared by the four waves: f16
+//    by the buffer-to-LDS DMA, in the cache's own order, whose 16-byte pieces
+//    are the fragments of both products (runs of 256 bytes: no bank
+//    conflicts); int8 through registers, converted once.
+//  * Scores come as columns, so each lane has one row's maximum, sum and
+//    rescaling factor, and the weights are the second product's operand in
+//    the registers where they are.
+//  * The accumulators are rescaled only when a maximum has grown by 2^8
+//    (weights up to 2^8 fit f16, sums are f32).
+//  * All workgroups of a key head run on one XCD where the head count allows,
+//    so a head's K and V are read from HBM once; the last rows, which see
+//    most keys, start first.
+//  * Few rows over a long cache: chunks of the keys, joined by the last one
+//    to count in, as attn_kernel's.
+#include "attn.hpp"
+
+namespace {
+
+using namespace st::attn;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 4, kPairs = 32 * kWaves;
+constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
+constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
+constexpr float kSlack = 8.0f;          // growth of a maximum that is let pass, in powers of two
+
+// (a helper of its own: written inside a kernel template the host pass drops
+// the kernel's launch stub)
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, _Float16 *lds, unsigned off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, off, 0, 0, 0);
+}
+
+__device__ __forceinline__ float other_half(float v) {  // lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <int HD>
+constexpr int kKeys = 64;  // keys of a tile (LDS for two of K and V: 64 KiB at 128 dims)
+
+template <int HD, bool I8, bool GEN>
+__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(Args a) {
+    constexpr int KT = kKeys<HD>, NKT = KT / 32, NS = HD / 16, ND = HD / 32;
+    constexpr int kTileE = 16 * HD;                       // elements of a cache tile
+    constexpr int kPer = KT * HD / 8 / (64 * kWaves);     // 16-byte pieces of K (and of V) a lane fetches per tile
+    __shared__ __align__(16) _Float16 k0s[KT * HD], v0s[KT * HD], k1s[KT * HD], v1s[KT * HD];
+    __shared__ __align__(16) float scales[I8 ? 2 : 1][2][I8 ? KT : 1];  // [stage][k, v]
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int col = lane & 31, hf = lane >> 5;
+    // (scalars: a division leaves its result in a vector register)
+    const int h = scalar((int)blockIdx.x % a.c.heads), item = scalar((int)blockIdx.x / a.c.heads);
+    Item it;
+    if (!find_item<kPairs, KT, 1>(a, item, it)) return;
+    it = scalars(it);
+
+    // ---- rows: the last block first
+    const int block = it.blocks - 1 - it.rb;
+    const int npair = it.s.q * a.group, p0 = it.s.kv - it.s.q;
+    const int wfirst = block * kPairs + 32 * wave;  // this wave's first pair
+    const int pair = wfirst + col;
+    const bool real = pair < npair;
+    const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
+    const int pos = real ? p0 + tok : -1;
+    const int low = a.window ? max(pos - a.window + 1, 0) : 0;  // keys low .. pos are visible
+    // (uniform) positions of the block's and of the wave's first and last rows
+    const int bmin = p0 + scalar(block * kPairs / a.group);
+    const int bmax = p0 + scalar((min(block * kPairs + kPairs, npair) - 1) / a.group);
+    const bool working = wfirst < npair;
+    const int wmin = p0 + scalar(wfirst / a.group), wmax = p0 + scalar((min(wfirst + 32, npair) - 1) / a.group);
+    const int blow = a.window ? max(bmin - a.window + 1, 0) : 0;    // no row of the block sees keys before this
+    const int wlow = a.window ? max(wmin - a.window + 1, 0) : 0;    // the same for the wave
+    const int whigh = a.window ? wmax - a.window + 1 : 0;           // from here on keys are in every window of the wave
+    const float slope = GEN && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+
+    half8 qf[NS];
+    {
+        const _Float16 *const q = static_cast<const _Float16 *>(a.q) + ((int64_t)(it.s.q0 + tok) * a.n_heads + head) * HD + 8 * hf;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const half8 *>(q + 16 * s);
+    }
+
+    // ---- this block's tiles of the chunk
+    const int key0 = first_key<KT>(a, it.s);
+    int t0 = it.s0, t1 = it.s1;
+    t1 = bmax < key0 ? t0 : min(t1, (bmax - key0) / KT + 1);
+    if (blow > key0) t0 = max(t0, (blow - key0) / KT);
+    t1 = max(t1, t0);
+
+    const int tile0 = key0 / 16, tiles = (it.s.kv + 15) / 16, tsh = a.c.tiles_shift();
+    const auto *const pages =
+        (const __attribute__((address_space(4))) int32_t *)(a.table + (int64_t)it.b * a.table_stride);
+    auto page_of = [&](int t) __attribute__((always_inline)) {
+        const int p = pages[max(min(t, tiles - 1), 0) >> tsh];
+        return t < tiles && (unsigned)p < (unsigned)a.c.num_pages ? p : -1;
+    };
+    // A wave fetches kPer pieces a lane, of one cache tile: its tile of the
+    // KT / 16, and from which piece on.
+    const int my_tile = wave * kPer * 64 * 8 / kTileE, my_piece = wave * kPer * 64 - my_tile * (kTileE / 8);
+    // Pages of the tile to fetch, a turn ahead; a bit of `missing` for each
+    // cache tile of the fetched one that is not read (it lands as zeros).
+    int page[KT / 16];
+    unsigned missing = 0;
+    auto look = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < KT / 16; ++j) page[j] = page_of(tile0 + t * (KT / 16) + j);
+    };
+    look(t0);
+    u32x2 kr[I8 ? kPer : 1], vr[I8 ? kPer : 1];
+    float sc = 0.0f;
+    auto fetch = [&](_Float16 *ks, _Float16 *vs, int t) __attribute__((always_inline)) {
+        int mine = page[0];
+        missing = 0;
+#pragma unroll
+        for (int j = 0; j < KT / 16; ++j) {
+            mine = my_tile == j ? page[j] : mine;
+            missing |= page[j] < 0 ? 1u << j : 0u;
+        }
+        const bool ok = mine >= 0 && t < t1;
+        const int ct = tile0 + t * (KT / 16) + my_tile;
+        const int64_t e = ok ? a.c.tile(mine, h, ct & ((1 << tsh) - 1)) * kTileE : 0;
+        constexpr int size = kTileE * (I8 ? 1 : 2);
+        using E = std::conditional_t<I8, signed char, _Float16>;
+        const __amdgpu_buffer_rsrc_t rk =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(static_cast<E *>(a.c.k) + e), (short)0, ok ? size : 0, kRsrcWord3);
+        const __amdgpu_buffer_rsrc_t rv =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(static_cast<E *>(a.c.v) + e), (short)0, ok ? size : 0, kRsrcWord3);
+        if constexpr (I8) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const unsigned off = (my_piece + 64 * i + lane) * 8;
+                kr[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, off, 0, 0));
+                vr[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0));
+            }
+            // lanes 0-15 the key scales of the wave's tile, 16-31 the value scales
+            const int64_t at = ok ? a.c.scale(mine, h, (ct * 16) & ((1 << a.c.page_shift) - 1)) : 0;
+            const float *const from = ((lane & 16) ? a.c.v_scale : a.c.k_scale) + at;
+            sc = from[lane & 15];
+            sc = ok ? sc : 0.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const unsigned off = (my_piece + 64 * i + lane) * 16;
+                dma16(rk, ks + (wave * kPer + i) * 64 * 8, off);
+                dma16(rv, vs + (wave * kPer + i) * 64 * 8, off);
+            }
+        }
+        look(t + 1);
+    };
+    auto put = [&](_Float16 *ks, _Float16 *vs, int stage) __attribute__((always_inline)) {  // int8: what fetch brought
+        if constexpr (I8) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                *reinterpret_cast<half8 *>(ks + ((wave * kPer + i) * 64 + lane) * 8) = i8_to_half8(kr[i]);
+                *reinterpret_cast<half8 *>(vs + ((wave * kPer + i) * 64 + lane) * 8) = i8_to_half8(vr[i]);
+            }
+            if (lane < 32 && my_piece == 0) scales[stage][lane >> 4][my_tile * 16 + (lane & 15)] = sc;
+        }
+    };
+
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // m in powers of two; l: this lane's half of the sum
+    int ve = -126;                  // int8: weights are held times their value scale over 2^ve
+    const float c1 = GEN ? 1.0f : a.scale * kLog2e;
+
+    auto compute = [&](const _Float16 *ks, const _Float16 *vs, int stage, int t, unsigned gone) __attribute__((always_inline)) {
+        const int kb = key0 + t * KT;
+        if (!working || kb > wmax || kb + KT <= wlow) return;  // (uniform) nothing here for this wave
+        f32x16 s[NKT];
+#pragma unroll
+        for (int n = 0; n < NKT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+            const _Float16 *const kp = ks + (2 * n + (col >> 4)) * kTileE + hf * 128 + (col & 15) * 8;
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(kp + 256 * j), qf[j], s[n], 0, 0, 0);
+        }
+        // element i of s[n] is key kb + 32 n + 8 (i / 4) + 4 hf + i % 4
+        auto key = [&](int n, int i) { return kb + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3); };
+        if constexpr (I8) {
+#pragma unroll
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 f = *reinterpret_cast<const f32x4 *>(&scales[stage][0][32 * n + 8 * g + 4 * hf]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][4 * g + i] *= f[i];
+                }
+        }
+        if constexpr (GEN) {
+            const float in = a.cap > 0.0f ? a.scale / a.cap * 2.0f * kLog2e : 0.0f, cap = a.cap * kLog2e;
+#pragma unroll
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[n][i];
+                    if (a.cap > 0.0f)  // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
+                        x = cap - 2.0f * cap * __builtin_amdgcn_rcpf(1.0f + exp2_(x * in));
+                    else
+                        x *= a.scale * kLog2e;
+                    if (a.slopes) x = fmaf(slope, (float)(key(n, i) - pos), x);
+                    s[n][i] = x;
+                }
+        }
+        // (uniform) a key that some row of the wave does not see
+        const bool masked = kb + KT - 1 > wmin || kb < whigh || gone;
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int k = key(n, i);
+                    s[n][i] = k >= low && k <= pos && !(gone >> (2 * n + (i >> 3)) & 1) ? s[n][i] : -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NKT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+        mx = fmaxf(mx, other_half(mx)) * c1;
+        float alpha = 1.0f;
+        if (__ballot(mx > m + kSlack)) {  // (m -inf: as soon as anything is visible)
+            const float mn = fmaxf(m, mx);
+            alpha = mn == -INFINITY ? 1.0f : exp2_(m - mn);
+            m = mn;
+            l *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NKT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[n][i] = exp2_(fmaf(s[n][i], c1, -base));
+                sum += s[n][i];
+            }
+        l += sum;
+        if constexpr (I8) {
+            const float mine = scales[stage][1][lane % KT];
+            float top = kb + lane % KT >= blow && kb + lane % KT <= bmax ? mine : 0.0f;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+            const int e = max(ve, (int)((__float_as_uint(top) >> 23) & 255) - 126);  // top / 2^e < 1
+            alpha = ldexpf(alpha, ve - e);
+            ve = e;
+            const float down = ldexpf(1.0f, -e);
+#pragma unroll
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 f = *reinterpret_cast<const f32x4 *>(&scales[stage][1][32 * n + 8 * g + 4 * hf]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = s[n][4 * g + i] * (f[i] * down);
+                        s[n][4 * g + i] = masked && s[n][4 * g + i] == 0.0f ? 0.0f : w;
+                    }
+                }
+        }
+        if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= alpha;
+        }
+#pragma unroll
+        for (int n = 0; n < NKT; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                half8 p;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = (_Float16)s[n][8 * u + j];
+                const _Float16 *const vp = vs + (2 * n + u) * kTileE + hf * (HD * 8) + col * 8;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(vp + 256 * d), p, o[d], 0, 0, 0);
+            }
+    };
+    // f16: zeros in the place of values that no row of the block sees (they
+    // may be anything, and 0 times anything has to be 0).
+    auto clean = [&](_Float16 *vs, int t) __attribute__((always_inline)) {
+        const int kb = key0 + t * KT;
+        if (I8 || (kb + KT - 1 <= bmax && kb >= blow)) return;  // (uniform)
+        for (int i = tid; i < KT * HD / 8; i += 64 * kWaves) {
+            const int tile = i / (kTileE / 8), half = i % (kTileE / 8) / HD;
+            half8 v = *reinterpret_cast<half8 *>(vs + i * 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int k = kb + 16 * tile + v_token(half, j);
+                v[j] = k >= blow && k <= bmax ? v[j] : (_Float16)0.0f;
+            }
+            *reinterpret_cast<half8 *>(vs + i * 8) = v;
+        }
+        __syncthreads();
+    };
+
+    auto turn = [&](_Float16 *ks, _Float16 *vs, _Float16 *kn, _Float16 *vn, int stage, int t) __attribute__((always_inline)) {
+        const unsigned gone = missing;
+        if constexpr (I8) {
+            fetch(kn, vn, t + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(ks, vs, stage, t, gone);
+            put(kn, vn, stage ^ 1);
+            __syncthreads();
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // this tile is in LDS, the other free
+            fetch(kn, vn, t + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            clean(vs, t);
+            compute(ks, vs, stage, t, gone);
+        }
+    };
+    fetch(k0s, v0s, t0);
+    if constexpr (I8) {
+        put(k0s, v0s, 0);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1;) {
+        turn(k0s, v0s, k1s, v1s, 0, t);
+        if (++t >= t1) break;
+        turn(k1s, v1s, k0s, v0s, 1, t);
+        ++t;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a fetch past the end)
+
+    l += other_half(l);
+    if constexpr (I8) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], ve);
+    }
+    const int row = it.s.q0 + tok;
+    if (it.chunks == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees nothing is zero)
+        if (real) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 v = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+                    store_out(a, v, row, head, 32 * d + 8 * g + 4 * hf, HD);
+                }
+        }
+        return;
+    }
+
+    // ---- chunks: as attn_kernel's; a lane joins what it would have written
+    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, a.G * a.c.heads * kPairs * HD * 4, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, a.G * a.c.heads * kPairs * 8, kRsrcWord3);
+    const int mine = 32 * wave + col;
+    auto at = [&](int i) { return (unsigned)((i * a.c.heads + h) * kPairs + mine); };
+    if (real) {
+        const unsigned r = at(item);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rp, (r * HD + 32 * d + 8 * g + 4 * hf) * 4, 0, kCoherent);
+            }
+        if (hf == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, rm, r * 8, 0, kCoherent);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's partial results are in memory
+    __syncthreads();
+    if (tid == 0) {
+        unsigned *const cnt = a.cnt + st::spread_counter(it.counter * a.c.heads + h);
+        const unsigned done = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        s_last = done == (unsigned)it.chunks - 1;
+        if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+    __syncthreads();
+    if (!s_last || !real) return;
+    auto ml_of = [&](int c, float &mc, float &lc) {
+        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, at(it.first + c * it.blocks) * 8, 0, kCoherent));
+        const unsigned w0 = w.x, w1 = w.y;
+        mc = __uint_as_float(w0), lc = __uint_as_float(w1);
+    };
+    float top = -INFINITY, total = 0.0f;
+    for (int c = 0; c < it.chunks; ++c) {
+        float mc, lc;
+        ml_of(c, mc, lc);
+        const float mn = fmaxf(top, mc);
+        if (mn > -INFINITY) total = total * exp2_(top - mn) + (mc == -INFINITY ? 0.0f : lc * exp2_(mc - mn));
+        top = mn;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    for (int c = 0; c < it.chunks; ++c) {
+        float mc, lc;
+        ml_of(c, mc, lc);
+        const float w = mc == -INFINITY ? 0.0f : exp2_(mc - top) * inv;
+        const unsigned r = at(it.first + c * it.blocks);
+        u32x4 v[ND][4];
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                v[d][g] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (r * HD + 32 * d + 8 * g + 4 * hf) * 4, 0, kCoherent));
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 f = __builtin_bit_cast(f32x4, v[d][g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][4 * g + i] = fmaf(w, f[i], o[d][4 * g + i]);
+            }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            store_out(a, f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]}, row, head, 32 * d + 8 * g + 4 * hf, HD);
+}
+
+template <int HD, bool I8, bool GEN>
+int launch_prompt(st_context *ctx, Args a) {
+    const int heads = a.c.heads;
+    // chunks only where the row blocks alone leave CUs without work
+    const int64_t blocks = ((int64_t)a.T * a.group + kPairs - 1) / kPairs * heads, slots = 2 * ctx->num_cus;
+    if (int rc = plan_cut(ctx, a, kPairs, HD, kKeys<HD>, 1, (slots - blocks) / heads)) return rc;
+    st::launch(ctx, prompt_kernel<HD, I8, GEN>, dim3((unsigned)(a.G * heads)), dim3(64 * kWaves), 0, a);
+    return st::launch_check("prompt_kernel");
+}
+
+template <int HD>
+int by_type(st_context *ctx, const Args &a, bool i8) {
+    const bool gen = a.cap > 0.0f || a.slopes;
+    if (i8) return gen ? launch_prompt<HD, true, true>(ctx, a) : launch_prompt<HD, true, false>(ctx, a);
+    return gen ? launch_prompt<HD, false, true>(ctx, a) : launch_prompt<HD, false, false>(ctx, a);
+}
+
+}  // namespace
+
+namespace st {
+namespace attn {
+
+int prompt_attention(st_context *ctx, const Args &a, bool i8, int hd) {
+    return hd == 64 ? by_type<64>(ctx, a, i8) : hd == 128 ? by_type<128>(ctx, a, i8) : by_type<256>(ctx, a, i8);
+}
+
+}  // namespace attn
+}  // namespace st
