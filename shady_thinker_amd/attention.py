@@ -20,7 +20,6 @@ Errors raise ValueError / TypeError (arguments) or ShadyHipError (a call).
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -40,18 +39,40 @@ def _act(t, name: str) -> int:
     return d
 
 
-def _rows_of(t, name: str, width: int) -> int:
-    """Elements from one row of `t` [T, width] to the next: a row's elements
-    side by side (a part of a wider row will do)."""
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, strides {t.stride()} (need [T, {width}], rows of adjacent elements)")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+# As in model.py, what is right in the common case is found by few cheap
+# tensor queries (a small call's kernel takes 4 us); a failing check goes on to
+# a function that says what is wrong.
+def _bad_rows(t, name: str, rows: int, width: int, dtype):
+    raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, strides {t.stride()} (need {dtype} [{rows}, {width}], rows of adjacent "
+                     "elements)")
+
+
+def _rows(t, name: str, rows: int, width: int, dtype) -> int:
+    """Elements from one row of `t` [rows, width] to the next; a row's
+    elements are side by side (a part of a wider row will do)."""
+    if t.dtype is not dtype or t.shape != (rows, width):
+        _bad_rows(t, name, rows, width, dtype)
+    if rows == 1 and t.is_contiguous():
+        return width
+    s = t.stride()
+    if s[1] != 1:
+        _bad_rows(t, name, rows, width, dtype)
+    return s[0]
 
 
 def _index(t, name: str, n: int) -> int:
     """Address of a contiguous int32 tensor of at least n."""
     if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
         _need(t, name, (_I32,), n)
+    return t.data_ptr()
+
+
+def _f32(t, name: str, n: int) -> int | None:
+    """Address of a contiguous float32 tensor of at least n (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not _F32 or t.numel() < n or not t.is_contiguous():
+        _need(t, name, (_F32,), n)
     return t.data_ptr()
 
 
@@ -101,6 +122,7 @@ class KvCache:
             k_scale = v_scale = None
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.dtype, self.num_pages, self.page_size, self.n_kv_heads, self.head_dim = k.dtype, pages, page_size, heads, d8 * 8
+        self.kv_width = heads * d8 * 8  # a token's keys, or values
         self._struct = KvCacheStruct(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), ST_I8 if k.dtype is _I8 else ST_F16, pages, page_size,
                                      heads, d8 * 8)
         self.handle = ctypes.addressof(self._struct)
@@ -129,46 +151,41 @@ def qk_norm_rope_store(gpu, cache: KvCache, q, k, v, q_out, slots, positions=Non
     parts of one q|k|v row. q_out [T, heads * head_dim] float32 or float16.
     q and q_out None: keys and values only. one_plus: weights hold w - 1;
     pairs: dims (2j, 2j + 1) rotate together, not (j, j + rot / 2)."""
-    hd, kw = cache.head_dim, cache.n_kv_heads * cache.head_dim
+    hd, kw = cache.head_dim, cache.kv_width
+    dtype = k.dtype
     dt = _act(k, "k")
     T = k.shape[0]
-    ks, vs = _rows_of(k, "k", kw), _rows_of(v, "v", kw)
-    if v.dtype is not k.dtype or v.shape[0] != T:
-        raise ValueError(f"v: {v.dtype} {tuple(v.shape)} beside k: {k.dtype} {tuple(k.shape)}")
-    heads, qs, qh, qd = 0, 0, 0, 0
+    ks, vs = _rows(k, "k", T, kw, dtype), _rows(v, "v", T, kw, dtype)
+    heads = qs = qh = qd = rot = n_pos = 0
+    qp = op = at = cp = sp = None
     if q is not None:
         if q_out is None:
             raise ValueError("q without q_out")
         qh = 2 * hd if gated else hd
-        if q.dtype is not k.dtype or q.dim() != 2 or q.shape[0] != T or q.shape[1] % qh or q.shape[1] == 0:
-            raise ValueError(f"q: {q.dtype} {tuple(q.shape)} (need {k.dtype} [{T}, heads * {qh}])")
-        heads = q.shape[1] // qh
-        qs = _rows_of(q, "q", heads * qh)
+        heads = q.shape[-1] // qh
+        qs = _rows(q, "q", T, max(heads, 1) * qh, dtype)
         qd = _act(q_out, "q_out")
         if q_out.numel() < T * heads * hd or not q_out.is_contiguous():
             _need(q_out, "q_out", (_F32, _F16), T * heads * hd)
+        qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    rot = n_pos = 0
-    at = None
     if cos is not None:
         if sin is None or positions is None:
             raise ValueError("cos needs sin and positions")
-        if cos.dim() != 2 or sin.shape != cos.shape:
-            raise ValueError(f"cos {tuple(cos.shape)}, sin {tuple(sin.shape)} (need [n_pos, rot / 2] both)")
-        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
-        if cos.dtype is not _F32 or sin.dtype is not _F32 or not cos.is_contiguous() or not sin.is_contiguous():
-            _need(cos, "cos", (_F32,), 0)
-            _need(sin, "sin", (_F32,), 0)
+        if cos.dim() != 2:
+            raise ValueError(f"cos {tuple(cos.shape)} (need [n_pos, rot / 2])")
+        n_pos, rot = cos.shape
+        cp, sp = _f32(cos, "cos", 1), _f32(sin, "sin", n_pos * rot)
+        rot *= 2
         at = _index(positions, "positions", T)
     elif sin is not None:
         raise ValueError("sin needs cos")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None and (w.dtype is not _F32 or w.numel() < hd or not w.is_contiguous()):
-            _need(w, name, (_F32,), hd)
+    qw, kwt = _f32(q_weight, "q_weight", hd), _f32(k_weight, "k_weight", hd)
+    slots_at = _index(slots, "slots", T)
     gpu.sync_stream()
-    call("st_qk_norm_rope_store", gpu.handle, cache.handle, ptr(q), k.data_ptr(), v.data_ptr(), dt, qs, ks, vs, qh, ptr(q_weight),
-         ptr(k_weight), eps, ptr(cos), ptr(sin), rot, n_pos, at, _index(slots, "slots", T), ptr(q_out), qd, T, heads,
+    call("st_qk_norm_rope_store", gpu.handle, cache.handle, qp, k.data_ptr(), v.data_ptr(), dt, qs, ks, vs, qh, qw, kwt, eps, cp, sp, rot,
+         n_pos, at, slots_at, op, qd, T, heads,
          (ST_FLAG_NORM_PLUS_ONE if one_plus else 0) | (ST_FLAG_ROPE_PAIRS if pairs else 0))
 
 
@@ -176,13 +193,15 @@ def kv_read(gpu, cache: KvCache, slots, k_out, v_out) -> None:
     """k_out, v_out [T, n_kv_heads, head_dim] (float32 or float16): the cached
     tokens of `slots` [T], dequantised; zeros for a slot outside the cache."""
     T = slots.numel()
-    n = T * cache.n_kv_heads * cache.head_dim
+    n = T * cache.kv_width
+    dtype = k_out.dtype
     dt = _act(k_out, "k_out")
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t.dtype is not k_out.dtype or t.numel() < n or not t.is_contiguous():
-            _need(t, name, (k_out.dtype,), n)
+    if v_out.dtype is not dtype or k_out.numel() < n or v_out.numel() < n or not k_out.is_contiguous() or not v_out.is_contiguous():
+        _need(k_out, "k_out", (dtype,), n)
+        _need(v_out, "v_out", (dtype,), n)
+    slots_at = _index(slots, "slots", T)
     gpu.sync_stream()
-    call("st_kv_read", gpu.handle, cache.handle, _index(slots, "slots", T), k_out.data_ptr(), v_out.data_ptr(), dt, T)
+    call("st_kv_read", gpu.handle, cache.handle, slots_at, k_out.data_ptr(), v_out.data_ptr(), dt, T)
 
 
 def paged_attention(gpu, cache: KvCache, q, out, table, kv_len, q_start=None, scale: float | None = None, cap: float = 0.0,
@@ -200,32 +219,30 @@ def paged_attention(gpu, cache: KvCache, q, out, table, kv_len, q_start=None, sc
     qkv rows' gated q, [T, heads * 2 * head_dim], each head's query followed
     by its gate), rows of adjacent elements."""
     hd = cache.head_dim
-    if table.dim() != 2:
-        raise ValueError(f"table: shape {tuple(table.shape)} (need [B, pages])")
+    if table.dim() != 2 or q.dim() != 2:
+        raise ValueError(f"table {tuple(table.shape)}, q {tuple(q.shape)} (need [B, pages], [T, heads * {hd}])")
     B, pages = table.shape
-    if q.dim() != 2 or q.shape[1] % hd or not q.is_contiguous():
-        raise ValueError(f"q: shape {tuple(q.shape)} (need contiguous [T, heads * {hd}])")
     T, width = q.shape
     heads = width // hd
+    if heads * hd != width or not q.is_contiguous():
+        raise ValueError(f"q: shape {tuple(q.shape)} (need contiguous [T, heads * {hd}])")
     qd, od = _act(q, "q"), _act(out, "out")
     if out.numel() < T * width or not out.is_contiguous():
         _need(out, "out", (_F32, _F16), T * width)
-    if slopes is not None and (slopes.dtype is not _F32 or slopes.numel() < heads or not slopes.is_contiguous()):
-        _need(slopes, "slopes", (_F32,), heads)
     gp, gd, gs, gh = None, 0, 0, 0
     if gate is not None:
         gd = _act(gate, "gate")
         gh = 2 * hd if gated else hd
-        gs = _rows_of(gate, "gate", heads * gh)
-        if gate.shape[0] != T:
-            raise ValueError(f"gate: {gate.shape[0]} rows beside {T}")
+        gs = _rows(gate, "gate", T, heads * gh, gate.dtype)
         gp = gate.data_ptr()
-        if gated:  # (from the first head's gate; the last head ends the row)
+        if gated:  # (from the first head's gate; the last head's ends the row)
             gp += hd * gate.element_size()
+    table_at, len_at = _index(table, "table", B * pages), _index(kv_len, "kv_len", B)
+    start_at = None if q_start is None else _index(q_start, "q_start", B + 1)
+    slopes_at = _f32(slopes, "slopes", heads)
     gpu.sync_stream()
-    call("st_paged_attention", gpu.handle, cache.handle, q.data_ptr(), qd, _index(table, "table", B * pages), pages,
-         _index(kv_len, "kv_len", B), None if q_start is None else _index(q_start, "q_start", B + 1),
-         1.0 / math.sqrt(hd) if scale is None else scale, cap, window, ptr(slopes), gp, gd, gs, gh, out.data_ptr(), od, T, B, heads)
+    call("st_paged_attention", gpu.handle, cache.handle, q.data_ptr(), qd, table_at, pages, len_at, start_at,
+         hd ** -0.5 if scale is None else scale, cap, window, slopes_at, gp, gd, gs, gh, out.data_ptr(), od, T, B, heads)
 
 
 def token_logprobs(gpu, logits, tokens=None, logprob=None, entropy=None, rank=None, top_ids=None, top_logprobs=None) -> None:
@@ -237,26 +254,23 @@ def token_logprobs(gpu, logits, tokens=None, logprob=None, entropy=None, rank=No
         raise ValueError(f"logits: shape {tuple(logits.shape)} (need [M, V])")
     M, V = logits.shape
     dt = _act(logits, "logits")
-    stride = _rows_of(logits, "logits", V)
+    stride = _rows(logits, "logits", M, V, logits.dtype)
     if tokens is None and (logprob is not None or rank is not None):
         raise ValueError("logprob and rank need tokens")
-    for t, name, d in ((logprob, "logprob", _F32), (entropy, "entropy", _F32), (rank, "rank", _I32)):
-        if t is not None and (t.dtype is not d or t.numel() < M or not t.is_contiguous()):
-            _need(t, name, (d,), M)
-    top = 0
+    tokens_at = None if tokens is None else _index(tokens, "tokens", M)
+    lp, ent = _f32(logprob, "logprob", M), _f32(entropy, "entropy", M)
+    rank_at = None if rank is None else _index(rank, "rank", M)
+    top, ids, tops = 0, None, None
     if top_ids is not None:
         if top_ids.dim() != 2 or top_ids.shape[0] != M:
             raise ValueError(f"top_ids: shape {tuple(top_ids.shape)} (need [{M}, n])")
         top = top_ids.shape[1]
-        _index(top_ids, "top_ids", 0)
-        if top_logprobs is not None and (top_logprobs.dtype is not _F32 or top_logprobs.numel() < M * top
-                                         or not top_logprobs.is_contiguous()):
-            _need(top_logprobs, "top_logprobs", (_F32,), M * top)
+        if top:
+            ids, tops = _index(top_ids, "top_ids", M * top), _f32(top_logprobs, "top_logprobs", M * top)
     elif top_logprobs is not None:
         raise ValueError("top_logprobs needs top_ids")
     gpu.sync_stream()
-    call("st_token_logprobs", gpu.handle, logits.data_ptr(), dt, stride, None if tokens is None else _index(tokens, "tokens", M),
-         ptr(logprob), ptr(entropy), ptr(rank), ptr(top_ids) if top else None, ptr(top_logprobs) if top else None, M, V, top)
+    call("st_token_logprobs", gpu.handle, logits.data_ptr(), dt, stride, tokens_at, lp, ent, rank_at, ids, tops, M, V, top)
 
 
 class PagedAttention:

@@ -34,57 +34,89 @@ namespace {
 
 using namespace st::attn;
 
-constexpr int kWaves = 4;
-constexpr int kStep = 32;  // keys of a step of one wave
 constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
 constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
 constexpr float kShift = 14.0f;         // weights are held times 2^14: f16 keeps them normal down to 2^-28
 
-template <int HD, bool I8, bool SPLIT>
+// Keys of a step of one wave: 32 (two tiles) of f16, 64 of int8 (the same
+// bytes; what a step costs beside its products then counts half).
+template <bool I8>
+constexpr int kStep = I8 ? 64 : 32;
+// Steps of a chunk (a multiple of the first), steps that stay in one.
+template <bool I8>
+constexpr int kLeast = I8 ? 4 : 8;
+template <bool I8>
+constexpr int kWhole = I8 ? 16 : 32;
+
+template <int HD, bool I8>
 struct Frag {
-    static constexpr int NS = HD / 32, ND = HD / 16;
-    using P = std::conditional_t<I8, u32x2, half8>;  // a piece: eight elements
-    P k[2][NS], v[ND];
-    f32x4 ks[I8 ? 2 : 1], vs[I8 ? 2 : 1];  // the lane's eight keys' scales
+    static constexpr int SUB = kStep<I8> / 32, NS = HD / 32, ND = HD / 16;
+    // 16 bytes a load: a piece of f16; of int8 the pieces of two tokens (k),
+    // of two dims (v)
+    u32x4 k[I8 ? SUB : 2 * SUB][NS], v[SUB][I8 ? ND / 2 : ND];
+    float ks, vs;  // int8: the scales of key `lane` of the step's 64
+    unsigned ok;                                       // (uniform) a bit for each tile that is there
 };
 
-__device__ __forceinline__ half8 as_half8(half8 v) { return v; }
-__device__ __forceinline__ half8 as_half8(u32x2 v) { return i8_to_half8(v); }
+// Piece `half` of the pair in w (int8), or w (f16).
+template <bool I8>
+__device__ __forceinline__ half8 piece(u32x4 w, int half) {
+    if constexpr (!I8) return __builtin_bit_cast(half8, w);
+    const unsigned a = half ? w.z : w.x, b = half ? w.w : w.y;
+    return i8_to_half8(u32x2{a, b});
+}
 
-__device__ __forceinline__ float max_q4(float v) {  // over the four lanes of a column
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+template <bool NTL>
+__device__ __forceinline__ u32x4 fetch16(const void *p) {
+    const u32x4 *const q = static_cast<const u32x4 *>(p);
+    return NTL ? __builtin_nontemporal_load(q) : *q;
 }
-__device__ __forceinline__ float half_turn(float v) {  // the lane eight columns on
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, true));
+
+// Over the four lanes of a column (col, col + 16, + 32, + 48).
+template <typename Op>
+__device__ __forceinline__ float over_q4(float v, Op op) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
+__device__ __forceinline__ float max_q4(float v) {
+    return over_q4(v, [](float x, float y) { return fmaxf(x, y); });
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float half_turn(float v) { return dpp<0x128>(v); }  // the lane eight columns on
 
 // Two steps' pieces in registers (256 dims: one, two do not fit).
-template <int HD, bool I8>
+template <int HD>
 constexpr bool kTwo = HD <= 128;
 
-template <int HD, bool I8, bool SPLIT>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
+// GEN: capped scores or slopes. NTL: non-temporal loads of the cache.
+template <int HD, bool I8, bool SPLIT, bool GEN, bool NTL, int NW>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     constexpr int PB = SPLIT ? 8 : 16;  // pairs of a block
-    constexpr int NS = HD / 32, ND = HD / 16, kRow = HD + 4;
-    using F = Frag<HD, I8, SPLIT>;
+    constexpr int ST = kStep<I8>, SUB = ST / 32, NS = HD / 32, ND = HD / 16, kRow = HD + 4, NT = 64 * NW;
+    using F = Frag<HD, I8>;
     using E = std::conditional_t<I8, signed char, _Float16>;
-    extern __shared__ __align__(16) float so[];  // [kWaves][PB][kRow]
-    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    extern __shared__ __align__(16) float so[];  // [NW][PB][kRow]
+    __shared__ float sm[NW][16], sl[NW][16];
     __shared__ float sw[kMaxChunks * PB];
+    __shared__ __align__(16) float scales[I8 ? NW : 1][2][I8 ? ST : 1];  // int8: each wave's step's, by key
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int col = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.y;
     Item it;
-    if (!find_item<PB, kStep, kWaves>(a, (int)blockIdx.x, it)) return;
+    if (!find_item<PB, ST, kLeast<I8>, kWhole<I8>>(a, (int)blockIdx.x, it)) return;
     it = scalars(it);
 
     // ---- this lane's column: a (row, head) pair
     const int npair = it.s.q * a.group;
     const int pair = it.rb * PB + (SPLIT ? col & 7 : col);
     const bool real = pair < npair;
-    const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair % a.group : 0);
+    const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
     const int p0 = it.s.kv - it.s.q;  // position of the sequence's first row
     const int pos = real ? p0 + tok : -1;
     const int low = a.window ? max(pos - a.window + 1, 0) : 0;  // keys low .. pos are visible
@@ -92,101 +124,98 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     const int pmin = p0 + scalar(it.rb * PB / a.group), pmax = p0 + scalar((min(it.rb * PB + PB, npair) - 1) / a.group);
     const int wmax = a.window ? pmax - a.window + 1 : 0;  // from here on a key is in every row's window
     const int wmin = a.window ? pmin - a.window + 1 : 0;  // before this it is in none's
-    const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    const float slope = GEN && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
 
+    // ---- the queries: loads on their way while the pages are looked up
     half8 qf[NS];
     float qs = a.scale;  // scores are matrix sums times qs
+    float x32[SPLIT ? NS : 1][8];
     {
-        float x[NS][8];
         const int64_t at = ((int64_t)(it.s.q0 + tok) * a.n_heads + head) * HD + q4 * 8;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            if (a.q_f32) {
-                const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + at + 32 * s);
-                const f32x4 u = p[0], w = p[1];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[s][i] = u[i], x[s][4 + i] = w[i];
-            } else {
-                const half8 u = *reinterpret_cast<const half8 *>(static_cast<const _Float16 *>(a.q) + at + 32 * s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[s][i] = (float)u[i];
-            }
-        }
-        if constexpr (SPLIT) {
-            float m = 0.0f;
+        if (SPLIT && a.q_f32) {
+            const float *const q = static_cast<const float *>(a.q) + at;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[s][i]));
-            m = max_q4(m);
-            int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-            e = max(e, -126);
+                for (int i = 0; i < 8; i += 4) {
+                    const f32x4 u = *reinterpret_cast<const f32x4 *>(q + 32 * s + i);
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = ldexpf(x[s][i], -e);
-                    const _Float16 hi = (_Float16)v;
-                    qf[s][i] = col < 8 ? hi : (_Float16)(v - (float)hi);
+                    for (int j = 0; j < 4; ++j) x32[SPLIT ? s : 0][i + j] = u[j];
                 }
-            qs = ldexpf(qs, e);
         } else {
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+            for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const half8 *>(static_cast<const _Float16 *>(a.q) + at + 32 * s);
+            if constexpr (SPLIT) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)x[s][i];
-        }
-        if (!real) {
+                for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) qf[s] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                    for (int i = 0; i < 8; ++i) x32[s][i] = (float)qf[s][i];
+            }
         }
     }
 
-    // ---- the chunk's steps: this wave's are s0 + wave, + kWaves, ...
-    const int key0 = first_key<kStep>(a, it.s);
+    // ---- the chunk's steps: this wave's are s0 + wave, + NW, ...
+    const int key0 = first_key<ST>(a, it.s);
     const int tile0 = key0 / 16, tiles = (it.s.kv + 15) / 16;  // tiles that hold a token
     const int tsh = a.c.tiles_shift();
-    const int32_t *const table = a.table + (int64_t)it.b * a.table_stride;
-    // A tile's page (-1: none to read), through the scalar cache: its waits
-    // are not those of the pieces in flight.
-    const auto *const pages = (const __attribute__((address_space(4))) int32_t *)table;
-    auto page_of = [&](int t) __attribute__((always_inline)) {
-        const int p = pages[max(min(t, tiles - 1), 0) >> tsh];
+    // Pages come through the scalar cache a step ahead, as they are in the
+    // table and from a place that is in it; whether there is such a tile and
+    // page is asked when the step is loaded (asked at once, every step waited
+    // for its table entry: 3 us a step of a batch that no cache holds).
+    const auto *const pages =
+        (const __attribute__((address_space(4))) int32_t *)(a.table + (int64_t)it.b * a.table_stride);
+    int next[2 * SUB];  // of the step to load
+    auto look = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2 * SUB; ++j) next[j] = pages[max(min(tile0 + 2 * SUB * step + j, tiles - 1), 0) >> tsh];
+    };
+    auto page_of = [&](int t, int p) __attribute__((always_inline)) {  // (-1: none to read)
         return t < tiles && (unsigned)p < (unsigned)a.c.num_pages ? p : -1;
     };
-    int next0 = page_of(tile0 + 2 * (it.s0 + wave)), next1 = page_of(tile0 + 2 * (it.s0 + wave) + 1);  // of the step to load
-    // (this lane's pieces: K row r = lane % 16 is place r % 8 (+ 8) of tile
-    // r / 8, V piece half q4 % 2 of tile q4 / 2)
-    const int k_off = q4 * 128 + (col & 7) * 8, v_off = ((q4 & 1) * HD + col) * 8;
-    auto load = [&](F &f, int step, bool &ok0, bool &ok1) __attribute__((always_inline)) {
+    look(it.s0 + wave);
+    // This lane's pieces. Scores: row r = lane % 16 of product `half` is a
+    // place of tile r / 8 of two, so that rows 4 q4 .. 4 q4 + 3 of both
+    // products, the lane's scores, are the places of V piece q4 % 2 of tile
+    // q4 / 2. f16: place r % 8 + 8 half (score i of product `half` goes to
+    // place 4 half + i of the piece; runs of 128 bytes a load). int8: place
+    // 2 i' + half, i' = r % 8 with its upper two bits swapped (to place
+    // 2 i + half), so that one 16-byte load has both products' rows; f16 in
+    // that order reads every line twice, by half (32 sequences of 1000: 21 ->
+    // 32 us). Values: row r is dim 16 d + r, of int8 32 d + 2 r + half.
+    const int in_tile = I8 ? ((col & 1) | (col >> 1 & 2) | (col << 1 & 4)) * 16 : (col & 7) * 8;
+    const int k_off = q4 * 128 + in_tile, v_off = ((q4 & 1) * HD + (I8 ? 2 * col : col)) * 8;
+    auto load = [&](F &f, int step) __attribute__((always_inline)) {
         const bool in = step < it.s1;
-        const int t = tile0 + 2 * step;
-        const int p0 = next0, p1 = next1;
-        next0 = page_of(t + 2 * kWaves), next1 = page_of(t + 2 * kWaves + 1);
-        ok0 = in && p0 >= 0, ok1 = in && p1 >= 0;
-        // a tile that is not read: every lane at the cache's first piece
-        const int64_t e0 = ok0 ? a.c.tile(p0, h, t & ((1 << tsh) - 1)) * (16 * HD) : 0;
-        const int64_t e1 = ok1 ? a.c.tile(p1, h, (t + 1) & ((1 << tsh) - 1)) * (16 * HD) : 0;
-        const bool kt = col >= 8, vt = q4 >= 2;
-        const E *kp = static_cast<const E *>(a.c.k) + (kt ? e1 : e0) + ((kt ? ok1 : ok0) ? k_off : 0);
-        const E *vp = static_cast<const E *>(a.c.v) + (vt ? e1 : e0) + ((vt ? ok1 : ok0) ? v_off : 0);
+        f.ok = 0;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int u = 0; u < SUB; ++u) {
+            const int t = tile0 + 2 * (SUB * step + u);
+            const int p0 = page_of(t, next[2 * u]), p1 = page_of(t + 1, next[2 * u + 1]);
+            const bool ok0 = in && p0 >= 0, ok1 = in && p1 >= 0;
+            f.ok |= (ok0 ? 1u : 0u) << (2 * u) | (ok1 ? 1u : 0u) << (2 * u + 1);
+            // a tile that is not read: every lane at the cache's first piece
+            const int64_t e0 = ok0 ? a.c.tile(p0, h, t & ((1 << tsh) - 1)) * (16 * HD) : 0;
+            const int64_t e1 = ok1 ? a.c.tile(p1, h, (t + 1) & ((1 << tsh) - 1)) * (16 * HD) : 0;
+            const bool kt = col >= 8, vt = q4 >= 2;
+            const E *kp = static_cast<const E *>(a.c.k) + (kt ? e1 : e0) + ((kt ? ok1 : ok0) ? k_off : 0);
+            const E *vp = static_cast<const E *>(a.c.v) + (vt ? e1 : e0) + ((vt ? ok1 : ok0) ? v_off : 0);
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-                f.k[half][s] = *reinterpret_cast<const typename F::P *>(kp + 512 * s + 64 * half);
+            for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) f.v[d] = *reinterpret_cast<const typename F::P *>(vp + 128 * d);
-        if constexpr (I8) {
-            const int64_t s0 = ok0 ? a.c.scale(p0, h, (t * 16) & ((1 << a.c.page_shift) - 1)) : 0;
-            const int64_t s1 = ok1 ? a.c.scale(p1, h, (t * 16 + 16) & ((1 << a.c.page_shift) - 1)) : 0;
-            const int64_t at = (vt ? s1 : s0) + (q4 & 1) * 4;
+                for (int half = 0; half < (I8 ? 1 : 2); ++half)
+                    f.k[I8 ? u : 2 * u + half][s] = fetch16<NTL>(kp + 512 * s + 64 * half);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                f.ks[half] = *reinterpret_cast<const f32x4 *>(a.c.k_scale + at + 8 * half);
-                f.vs[half] = *reinterpret_cast<const f32x4 *>(a.c.v_scale + at + 8 * half);
-            }
+            for (int d = 0; d < (I8 ? ND / 2 : ND); ++d) f.v[u][d] = fetch16<NTL>(vp + (I8 ? 256 : 128) * d);
         }
+        if constexpr (I8) {
+            int p = next[0];
+            p = q4 == 1 ? next[1] : p, p = q4 == 2 ? next[2] : p, p = q4 == 3 ? next[3] : p;
+            const int t = tile0 + 4 * step + q4;
+            const bool there = in && page_of(t, p) >= 0;
+            const int64_t at = there ? a.c.scale(p, h, ((t * 16) & ((1 << a.c.page_shift) - 1)) + col) : 0;
+            f.ks = a.c.k_scale[at], f.vs = a.c.v_scale[at];
+        }
+        look(step + NW);
     };
 
     f32x4 o[ND];
@@ -195,129 +224,192 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     float m = -INFINITY, l = 0.0f;
     int ve = -126;  // int8: weights are held times their value scale over 2^ve
 
-    auto compute = [&](F &f, int step, bool ok0, bool ok1) __attribute__((always_inline)) {
-        const int kb = key0 + 32 * step;
-        f32x4 s4[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            s4[half] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                s4[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(f.k[half][s]), qf[s], s4[half], 0, 0, 0);
-        }
-        // this lane's keys: key(j) for weight j of the second product
+    auto compute = [&](F &f, int step) __attribute__((always_inline)) {
+        const int kb = key0 + ST * step;
+        // this lane's keys: key(j) for weight j % 8 of product j / 8
         const int kl = kb + 16 * (q4 >> 1) + 4 * (q4 & 1);
-        auto key = [&](int j) { return kl + (j & 3) + 8 * (j >> 2); };
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v = s4[j >> 2][j & 3];
-            if constexpr (SPLIT) v += half_turn(v);
-            if constexpr (I8) v *= f.ks[j >> 2][j & 3];
-            x[j] = v * qs;
+        auto key = [&](int j) { return kl + (j & 3) + 8 * (j >> 2 & 1) + 32 * (j >> 3); };
+        auto there = [&](int j) { return (f.ok >> (2 * (j >> 3) + (q4 >> 1)) & 1) != 0; };
+        float x[8 * SUB];
+        float alpha = 1.0f;
+        if constexpr (I8) {
+            // Scales go by LDS to the lanes that have their keys; those of
+            // values over 2^ve (kept as large as any so far needs it; scales
+            // that no row of the block sees may be anything).
+            const int k = kb + lane;
+            const bool any = (f.ok >> q4 & 1) && k <= pmax && k >= wmin;
+            const float vs = any ? f.vs : 0.0f;
+            float top = vs;
+            top = fmaxf(top, dpp<0x121>(top)), top = fmaxf(top, dpp<0x122>(top));
+            top = fmaxf(top, dpp<0x124>(top)), top = fmaxf(top, dpp<0x128>(top));
+            top = max_q4(top);
+            const int e = max(ve, uniform((int)((__float_as_uint(top) >> 23) & 255)) - 126);  // top / 2^e < 1
+            alpha = ldexpf(1.0f, ve - e);
+            ve = e;
+            scales[wave][0][lane] = f.ks, scales[wave][1][lane] = ldexpf(vs, -ve);
         }
-        if (a.cap > 0.0f) {
+        auto scale_of = [&](int which, int t) {  // of x[4 t] .. x[4 t + 3]
+            return *reinterpret_cast<const f32x4 *>(&scales[wave][which][32 * (t >> 1) + 16 * (q4 >> 1) + 4 * (q4 & 1) + 8 * (t & 1)]);
+        };
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = a.cap * tanhf(x[j] / a.cap);
-        }
+        for (int u = 0; u < SUB; ++u) {
+            f32x4 s4[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= kLog2e;
-        if (a.slopes) {
+            for (int half = 0; half < 2; ++half) {
+                s4[half] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = fmaf(slope, (float)(key(j) - pos), x[j]);
-        }
-        const bool full = ok0 && ok1 && kb + 31 <= pmin && kb >= wmax;  // (uniform) every key for every row
-        unsigned seen = 0xFF;
-        if (!full) {
-            const bool ok = q4 >= 2 ? ok1 : ok0;
-            seen = 0;
+                for (int s = 0; s < NS; ++s)
+                    s4[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece<I8>(f.k[I8 ? u : 2 * u + half][s], half), qf[s], s4[half], 0, 0, 0);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int kj = key(j);
-                if (ok && kj >= low && kj <= pos) seen |= 1u << j;
-                x[j] = seen >> j & 1 ? x[j] : -INFINITY;
+                float v = I8 ? s4[j & 1][j >> 1] : s4[j >> 2][j & 3];
+                if constexpr (SPLIT) v += half_turn(v);
+                x[8 * u + j] = v * qs;
             }
-            // values no row of the block sees may be anything
-            const bool none0 = !ok;
-            if constexpr (!I8) {
+        }
+        if constexpr (I8) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int kj = key(j);
-                    const bool any = !none0 && kj <= pmax && kj >= wmin;
+            for (int t = 0; t < 2 * SUB; ++t) {
+                const f32x4 ks = scale_of(0, t);
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) f.v[d][j] = any ? f.v[d][j] : (_Float16)0.0f;
+                for (int i = 0; i < 4; ++i) x[4 * t + i] *= ks[i];
+            }
+        }
+        if constexpr (GEN) {
+            if (a.cap > 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 8 * SUB; ++j) x[j] = a.cap * kLog2e * tanhf(x[j] / a.cap);
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int j = 0; j < 8 * SUB; ++j) x[j] = fmaf(slope, (float)(key(j) - pos), x[j]);
+            }
+        }
+        // (uniform) whether every key is there for every row
+        const bool full = f.ok == (1u << (2 * SUB)) - 1 && kb + ST - 1 <= pmin && kb >= wmax;
+        unsigned seen = (1u << (8 * SUB)) - 1;
+        if (!full) {
+            seen = 0;
+#pragma unroll
+            for (int j = 0; j < 8 * SUB; ++j) {
+                const int kj = key(j);
+                const bool see = there(j) && kj >= low && kj <= pos;
+                seen |= see ? 1u << j : 0u;
+                x[j] = see ? x[j] : -INFINITY;
+                // values no row of the block sees may be anything
+                const bool any = there(j) && kj <= pmax && kj >= wmin;
+                if constexpr (!I8) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        half8 w = __builtin_bit_cast(half8, f.v[j >> 3][d]);
+                        w[j & 7] = any ? w[j & 7] : (_Float16)0.0f;
+                        f.v[j >> 3][d] = __builtin_bit_cast(u32x4, w);
+                    }
                 }
             }
         }
         float mx = x[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
+        for (int j = 1; j < 8 * SUB; ++j) mx = fmaxf(mx, x[j]);
         const float mn = fmaxf(m, max_q4(mx));
         const float base = mn == -INFINITY ? 0.0f : mn;
-        float alpha = exp2_(m - base);  // (0 before the first visible key)
+        const float grown = exp2_(m - base);  // (0 before the first visible key)
+        alpha *= grown;
         m = mn;
-        float p[8], sum = 0.0f;
+        float p[8 * SUB], sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = exp2_(x[j] - base + kShift);
+        for (int j = 0; j < 8 * SUB; ++j) {
+            p[j] = exp2_(x[j] - (base - kShift));
             sum += p[j];
         }
-        l = fmaf(l, alpha, sum);
+        l = fmaf(l, grown, sum);
         if constexpr (I8) {
-            float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, seen >> j & 1 ? f.vs[j >> 2][j & 3] : 0.0f);
+            for (int t = 0; t < 2 * SUB; ++t) {
+                const f32x4 vs = scale_of(1, t);
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-            const int e = max(ve, (int)((__float_as_uint(top) >> 23) & 255) - 126);  // top / 2^e < 1
-            alpha = ldexpf(alpha, ve - e);
-            ve = e;
+                for (int i = 0; i < 4; ++i) p[4 * t + i] *= vs[i];
+            }
+            if (!full) {  // (a scale that another row sees may be a NaN)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = seen >> j & 1 ? p[j] * ldexpf(f.vs[j >> 2][j & 3], -ve) : 0.0f;
+                for (int j = 0; j < 8 * SUB; ++j) p[j] = seen >> j & 1 ? p[j] : 0.0f;
+            }
         }
         if (__ballot(alpha != 1.0f)) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
         }
-        half8 pf;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const _Float16 hi = (_Float16)p[j];
-            pf[j] = hi;
-            if constexpr (SPLIT) pf[j] = col < 8 ? hi : (_Float16)(p[j] - (float)hi);
+        for (int u = 0; u < SUB; ++u) {
+            half8 pf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const _Float16 hi = (_Float16)p[8 * u + j];
+                pf[j] = hi;
+                if constexpr (SPLIT) pf[j] = col < 8 ? hi : (_Float16)(p[8 * u + j] - (float)hi);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(piece<I8>(f.v[u][I8 ? d / 2 : d], d & 1), pf, o[d], 0, 0, 0);
         }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(f.v[d]), pf, o[d], 0, 0, 0);
     };
 
-    if constexpr (kTwo<HD, I8>) {
-        int step = it.s0 + wave;
-        F fa, fb;
-        bool a0, a1, b0, b1;
-        load(fa, step, a0, a1);
-        while (step < it.s1) {
-            load(fb, step + kWaves, b0, b1);
-            __builtin_amdgcn_sched_barrier(0);
-            compute(fa, step, a0, a1);
-            step += kWaves;
-            if (step >= it.s1) break;
-            load(fa, step + kWaves, a0, a1);
-            __builtin_amdgcn_sched_barrier(0);
-            compute(fb, step, b0, b1);
-            step += kWaves;
+    auto split_q = [&]() __attribute__((always_inline)) {
+        if constexpr (SPLIT) {
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x32[s][i]));
+            top = max_q4(top);
+            const int e = max((int)((__float_as_uint(top) >> 23) & 255) - 127, -126);
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = ldexpf(x32[s][i], -e);
+                    const _Float16 hi = (_Float16)v;
+                    qf[s][i] = col < 8 ? hi : (_Float16)(v - (float)hi);
+                }
+            qs = ldexpf(qs, e);
         }
+        if (!real) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) qf[s] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+        if (!GEN || !(a.cap > 0.0f)) qs *= kLog2e;  // (scores in powers of two)
+    };
+
+    if constexpr (kTwo<HD>) {
+        // Two steps a turn, one exit: with a break between them the compiler
+        // saw a way from there back to the top with the second buffer's loads
+        // still in flight, and waited for every load before issuing more.
+        int step = it.s0 + wave;
+        const int mine = step < it.s1 ? (it.s1 - step + NW - 1) / NW : 0;
+        F fa, fb;
+        load(fa, step);
+        split_q();
+        for (int i = 0; i < mine / 2; ++i, step += 2 * NW) {
+            load(fb, step + NW);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(fa, step);
+            load(fa, step + 2 * NW);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(fb, step + NW);
+        }
+        if (mine & 1) compute(fa, step);
     } else {
         F f;
-        bool ok0, ok1;
-        for (int step = it.s0 + wave; step < it.s1; step += kWaves) {
-            load(f, step, ok0, ok1);
-            compute(f, step, ok0, ok1);
+        split_q();
+        for (int step = it.s0 + wave; step < it.s1; step += NW) {
+            load(f, step);
+            compute(f, step);
         }
     }
 
-    // ---- the four waves meet in LDS
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    // ---- the waves meet in LDS
+    l = over_q4(l, [](float x, float y) { return x + y; });
     if constexpr (I8) {
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -332,40 +424,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     }
     if (col < PB) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-            *reinterpret_cast<f32x4 *>(&so[(wave * PB + col) * kRow + d * 16 + q4 * 4]) = o[d];
+        for (int d = 0; d < ND; ++d) {
+            if constexpr (I8) {  // (dims 32 d + 8 q4 .. + 7 in o[2 d] and o[2 d + 1], by turns)
+                if (d & 1) continue;
+                float *const to = &so[(wave * PB + col) * kRow + d * 16 + q4 * 8];
+                *reinterpret_cast<f32x4 *>(to) = f32x4{o[d][0], o[d + 1][0], o[d][1], o[d + 1][1]};
+                *reinterpret_cast<f32x4 *>(to + 4) = f32x4{o[d][2], o[d + 1][2], o[d][3], o[d + 1][3]};
+            } else {
+                *reinterpret_cast<f32x4 *>(&so[(wave * PB + col) * kRow + d * 16 + q4 * 4]) = o[d];
+            }
+        }
         if (q4 == 0) sm[wave][col] = m, sl[wave][col] = l;
     }
     __syncthreads();
-    constexpr int kQuads = PB * HD / 4;
     const int pairs_here = min(PB, npair - it.rb * PB);
+    const int quads = pairs_here * (HD / 4);
     const int row_id = (int)blockIdx.x * a.c.heads + h;
     auto weight = [](float mw, float top) { return mw == -INFINITY ? 0.0f : exp2_(mw - top); };
-    auto row_of = [&](int p, int &row, int &hd) {
-        const int g = it.rb * PB + p;
-        row = it.s.q0 + g / a.group, hd = h * a.group + g % a.group;
+    auto put = [&](f32x4 v, int p, int d) {
+        const int g = it.rb * PB + p, t = g / a.group;
+        store_out(a, v, it.s.q0 + t, h * a.group + g - t * a.group, d, HD);
     };
-    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, a.G * a.c.heads * PB * HD * 4, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, a.G * a.c.heads * PB * 8, kRsrcWord3);
-    for (int i = tid; i < kQuads; i += 64 * kWaves) {
+    const __amdgpu_buffer_rsrc_t rp =
+        __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, a.G * a.c.heads * PB * HD * 4, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t rm =
+        __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, a.G * a.c.heads * PB * 8, kRsrcWord3);
+    for (int i = tid; i < quads; i += NT) {
         const int p = i / (HD / 4), d = i % (HD / 4) * 4;
-        if (p >= pairs_here) continue;
         float top = sm[0][p];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][p]);
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w][p]);
         f32x4 v = {0, 0, 0, 0};
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = weight(sm[w][p], top);
             sum = fmaf(f, sl[w][p], sum);
             v += f * *reinterpret_cast<const f32x4 *>(&so[(w * PB + p) * kRow + d]);
         }
         if (it.chunks == 1) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees nothing is zero)
-            int row, hd;
-            row_of(p, row, hd);
-            store_out(a, v * inv, row, hd, d, HD);
+            put(v * (sum == 0.0f ? 0.0f : 1.0f / sum), p, d);  // (a row that sees nothing is zero)
         } else {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rp, ((row_id * PB + p) * HD + d) * 4, 0, kCoherent);
             if (d == 0)
@@ -375,7 +473,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     }
     if (it.chunks == 1) return;
 
-    // ---- the chunks meet: the last one to count in joins them in order
+    // ---- the chunks meet: the last one to count in joins them
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's partial results are in memory
     __syncthreads();
     if (tid == 0) {
@@ -387,18 +485,34 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
     __syncthreads();
     if (!s_last) return;
     auto row_at = [&](int c) { return (it.first + c * it.blocks) * a.c.heads + h; };
-    constexpr int TP = 64 * kWaves / PB;  // threads of a pair (of one wave)
-    {
-        const int p = tid / TP, i = tid % TP;
-        constexpr int kEach = (kMaxChunks + TP - 1) / TP;
+    // Thread (part, quad) takes every parts-th chunk of its quad, so that all
+    // chunks' loads are in flight at once; the parts meet in LDS, in order.
+    const int parts = max(1, min(NT / quads, (int)(sizeof(float) * NW * PB * kRow / (16 * quads))));
+    const int part = tid / quads, i = tid % quads, p = i / (HD / 4), d = i % (HD / 4) * 4;
+    constexpr int kFlight = 16;
+    u32x4 w8[kFlight];
+    auto fetch = [&](int quad, int c0, int by) __attribute__((always_inline)) {
+        const int pq = quad / (HD / 4), dq = quad % (HD / 4) * 4;
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+            const int c = c0 + j * by;
+            w8[j] = __builtin_amdgcn_raw_buffer_load_b128(rp, c < it.chunks ? ((row_at(c) * PB + pq) * HD + dq) * 4 : 0x80000000u, 0, kCoherent);
+        }
+    };
+    if (part < parts) fetch(i, part, parts);
+    constexpr int TP = 64 / PB * NW;  // threads of a pair (side by side in one wave, or in whole waves' halves)
+    constexpr int TW = TP > 64 ? 64 : TP;
+    if (tid < PB * TW) {
+        const int pp = tid / TW, ii = tid % TW;
+        constexpr int kEach = (kMaxChunks + TW - 1) / TW;
         float mv[kEach], lv[kEach];
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int c = i + j * TP;
+            const int c = ii + j * TW;
             mv[j] = -INFINITY, lv[j] = 0.0f;
-            if (c < it.chunks && p < pairs_here) {
-                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, (row_at(c) * PB + p) * 8, 0, kCoherent));
+            if (c < it.chunks && pp < pairs_here) {
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, (row_at(c) * PB + pp) * 8, 0, kCoherent));
                 const unsigned w0 = w.x, w1 = w.y;
                 mv[j] = __uint_as_float(w0), lv[j] = __uint_as_float(w1);
             }
@@ -406,7 +520,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) top = fmaxf(top, mv[j]);
 #pragma unroll
-        for (int d = 1; d < TP; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        for (int x = 1; x < TW; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
@@ -414,52 +528,82 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(Args a) {
             sum = fmaf(mv[j], lv[j], sum);
         }
 #pragma unroll
-        for (int d = 1; d < TP; d *= 2) sum += __shfl_xor(sum, d);
+        for (int x = 1; x < TW; x *= 2) sum += __shfl_xor(sum, x);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int c = i + j * TP;
-            if (c < it.chunks) sw[c * PB + p] = mv[j] * inv;
+            const int c = ii + j * TW;
+            if (c < it.chunks) sw[c * PB + pp] = mv[j] * inv;
         }
     }
     __syncthreads();
-    for (int i = tid; i < kQuads; i += 64 * kWaves) {
-        const int p = i / (HD / 4), d = i % (HD / 4) * 4;
-        if (p >= pairs_here) continue;
-        f32x4 v = {0, 0, 0, 0};
-        for (int c0 = 0; c0 < it.chunks; c0 += 8) {
-            u32x4 w[8];
+    auto add = [&](f32x4 &v, int pq, int c0, int by) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = __builtin_amdgcn_raw_buffer_load_b128(rp, c0 + j < it.chunks ? ((row_at(c0 + j) * PB + p) * HD + d) * 4 : 0x80000000u, 0,
-                                                             kCoherent);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + j < it.chunks) v += sw[(c0 + j) * PB + p] * __builtin_bit_cast(f32x4, w[j]);
+        for (int j = 0; j < kFlight; ++j) {
+            const int c = c0 + j * by;
+            if (c < it.chunks) v += sw[c * PB + pq] * __builtin_bit_cast(f32x4, w8[j]);
         }
-        int row, hd;
-        row_of(p, row, hd);
-        store_out(a, v, row, hd, d, HD);
+    };
+    if (parts > 1) {
+        f32x4 v = {0, 0, 0, 0};
+        if (part < parts) {
+            add(v, p, part, parts);
+            for (int c0 = part + kFlight * parts; c0 < it.chunks; c0 += kFlight * parts) {
+                fetch(i, c0, parts);
+                add(v, p, c0, parts);
+            }
+            *reinterpret_cast<f32x4 *>(&so[(part * quads + i) * 4]) = v;
+        }
+        __syncthreads();
+        if (part == 0) {
+            for (int k = 1; k < parts; ++k) v += *reinterpret_cast<const f32x4 *>(&so[(k * quads + i) * 4]);
+            put(v, p, d);
+        }
+        return;
+    }
+    for (int q = tid; q < quads; q += NT) {
+        const int pq = q / (HD / 4), dq = q % (HD / 4) * 4;
+        f32x4 v = {0, 0, 0, 0};
+        for (int c0 = 0; c0 < it.chunks; c0 += kFlight) {
+            if (q != tid || c0 > 0) fetch(q, c0, 1);
+            add(v, pq, c0, 1);
+        }
+        put(v, pq, dq);
     }
 }
 
-template <int HD, bool I8, bool SPLIT>
+template <int HD, bool I8, bool SPLIT, bool GEN, bool NTL>
 int launch_attn(st_context *ctx, Args a) {
-    constexpr int PB = SPLIT ? 8 : 16;
-    if (int rc = plan_cut(ctx, a, PB, HD, kStep, kWaves, 2 * ctx->num_cus / a.c.heads)) return rc;
-    const int heads = a.c.heads;
-    const size_t lds = (size_t)kWaves * PB * (HD + 4) * sizeof(float);
-    auto kern = attn_kernel<HD, I8, SPLIT>;
-    if (lds > 48 * 1024)
+    constexpr int PB = SPLIT ? 8 : 16, NW = 4;
+    const int64_t slots = 2 * ctx->num_cus;
+    if (int rc = plan_cut(ctx, a, PB, HD, kStep<I8>, kLeast<I8>, slots / a.c.heads)) return rc;
+    const size_t lds = (size_t)NW * PB * (HD + 4) * sizeof(float);
+    auto kern = attn_kernel<HD, I8, SPLIT, GEN, NTL, NW>;
+    if (lds > 32 * 1024)
         ST_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    st::launch(ctx, kern, dim3((unsigned)a.G, (unsigned)heads), dim3(64 * kWaves), lds, a);
+    st::launch(ctx, kern, dim3((unsigned)a.G, (unsigned)a.c.heads), dim3(64 * NW), lds, a);
     return st::launch_check("attn_kernel");
+}
+
+template <int HD, bool I8, bool SPLIT, bool GEN>
+int by_size(st_context *ctx, const Args &a) {
+    // A cache that no more than one row block reads, and that is larger than
+    // what a cache level keeps between calls
+    const int64_t bytes = (int64_t)a.B * a.capacity * a.c.heads * HD * (I8 ? 2 : 4);
+    const bool once = a.T == a.B && a.group <= (SPLIT ? 8 : 16) && bytes >= (int64_t)96 << 20;
+    return once ? launch_attn<HD, I8, SPLIT, GEN, true>(ctx, a) : launch_attn<HD, I8, SPLIT, GEN, false>(ctx, a);
+}
+
+template <int HD, bool I8>
+int by_scores(st_context *ctx, const Args &a, bool split) {
+    const bool gen = a.cap > 0.0f || a.slopes;
+    if (split) return gen ? by_size<HD, I8, true, true>(ctx, a) : by_size<HD, I8, true, false>(ctx, a);
+    return gen ? by_size<HD, I8, false, true>(ctx, a) : by_size<HD, I8, false, false>(ctx, a);
 }
 
 template <int HD>
 int by_type(st_context *ctx, const Args &a, bool i8, bool split) {
-    if (i8) return split ? launch_attn<HD, true, true>(ctx, a) : launch_attn<HD, true, false>(ctx, a);
-    return split ? launch_attn<HD, false, true>(ctx, a) : launch_attn<HD, false, false>(ctx, a);
+    return i8 ? by_scores<HD, true>(ctx, a, split) : by_scores<HD, false>(ctx, a, split);
 }
 
 // f16 rows of prompts go to the kernel with 128 pairs a workgroup.

@@ -111,8 +111,15 @@ __device__ __forceinline__ int chunk_steps(const Args &a, unsigned long long wor
     return c > kMostSteps ? kMostSteps : (int)c;
 }
 
+// A sequence of up to WHOLE steps stays in one chunk: joining chunks costs
+// more than that many steps.
+template <int WHOLE>
+__device__ __forceinline__ int chunks_of(int steps, int C) {
+    return steps <= max(C, WHOLE) ? 1 : (steps + C - 1) / C;
+}
+
 // Item w of the call (the same for every wave), or false: there is none.
-template <int PB, int STEP, int LEAST>
+template <int PB, int STEP, int LEAST, int WHOLE>
 __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
     const int lane = threadIdx.x & 63;
     if (a.B == 1) {
@@ -122,11 +129,11 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
         it.blocks = blocks_of<PB>(a, it.s);
         if (!it.blocks) return false;
         const int steps = steps_of<STEP>(a, it.s), C = chunk_steps<LEAST>(a, (unsigned long long)it.blocks * steps, it.blocks, steps);
-        it.chunks = max(1, (steps + C - 1) / C);
+        it.chunks = chunks_of<WHOLE>(steps, C);
         if (w >= it.blocks * it.chunks) return false;
         it.rb = w % it.blocks, it.chunk = w / it.blocks;
         it.first = it.rb, it.counter = it.rb;
-        it.s0 = min(it.chunk * C, steps), it.s1 = min(it.s0 + C, steps);
+        it.s0 = min(it.chunk * C, steps), it.s1 = it.chunks == 1 ? steps : min(it.s0 + C, steps);
         return true;
     }
     unsigned long long work = 0;
@@ -157,7 +164,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
         if (b < a.B) {
             s = seq_of(a, b);
             n = blocks_of<PB>(a, s), steps = steps_of<STEP>(a, s);
-            chunks = max(1, (steps + C - 1) / C);
+            chunks = chunks_of<WHOLE>(steps, C);
         }
         int upto = n * chunks, rows_upto = n;
 #pragma unroll
@@ -177,7 +184,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
             it.first = begin + it.rb;
             it.counter = rows + of(rows_upto) - it.blocks + it.rb;
             const int st = of(steps);
-            it.s0 = min(it.chunk * C, st), it.s1 = min(it.s0 + C, st);
+            it.s0 = min(it.chunk * C, st), it.s1 = it.chunks == 1 ? st : min(it.s0 + C, st);
             return true;
         }
         items += __builtin_amdgcn_readlane(upto, 63), rows += __builtin_amdgcn_readlane(rows_upto, 63);

@@ -232,12 +232,13 @@ struct ReadArgs {
     int T, shift;
 };
 
-template <int HD, bool OF32, bool I8>
+// U heads a workgroup, their loads in flight together.
+template <int HD, bool OF32, bool I8, int U>
 __global__ __launch_bounds__(2 * HD) void read_kernel(ReadArgs a) {
     constexpr int P = HD / 8;
     using E = std::conditional_t<I8, signed char, _Float16>;
     using E8 = std::conditional_t<I8, u32x2, half8>;
-    const int tid = threadIdx.x, piece = tid % P, tok = tid / P, head = blockIdx.y;
+    const int tid = threadIdx.x, piece = tid % P, tok = tid / P, head0 = blockIdx.y * U, heads = a.c.heads;
     const bool is_v = blockIdx.z != 0;
     const int t0 = (int)blockIdx.x * kTile - (a.shift ? a.slots[0] & (kTile - 1) : 0);
     const int t = t0 + tok;
@@ -245,79 +246,117 @@ __global__ __launch_bounds__(2 * HD) void read_kernel(ReadArgs a) {
     const int slot = live ? a.slots[t] : -1;
     const int page = slot >> a.c.page_shift, place = slot & ((1 << a.c.page_shift) - 1);
     const bool held = slot >= 0 && page < a.c.num_pages;
-    const int64_t tile = held ? a.c.tile(page, head, place >> 4) : 0;
+    const int64_t tile = held ? a.c.tile(page, head0, place >> 4) * (kTile * HD) : 0;
+    const int64_t next = held ? (int64_t)(kTile * HD) << a.c.tiles_shift() : 0;
     const int in_tile = place & (kTile - 1);
-    float scale = 1.0f;
-    if constexpr (I8) {
-        if (held) scale = (is_v ? a.c.v_scale : a.c.k_scale)[a.c.scale(page, head, place)];
+    auto of = [&](int u) { return head0 + u < heads ? u : 0; };  // (past the last head: the first again, not written)
+    float scale[U];
+    E8 e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        scale[u] = 1.0f;
+        e[u] = E8{};
+        if constexpr (I8) {
+            if (held) scale[u] = (is_v ? a.c.v_scale : a.c.k_scale)[a.c.scale(page, head0 + of(u), place)];
+        }
     }
-    E8 e = {};
     if (!is_v) {
-        if (held) e = *reinterpret_cast<const E8 *>(static_cast<const E *>(a.c.k) + tile * (kTile * HD) + piece * 128 + in_tile * 8);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (held) e[u] = *reinterpret_cast<const E8 *>(static_cast<const E *>(a.c.k) + tile + of(u) * next + piece * 128 + in_tile * 8);
     } else {
-        const E *const v = static_cast<const E *>(a.c.v) + tile * (kTile * HD);
+        const E *const v = static_cast<const E *>(a.c.v) + tile;
         if (whole_tile(a.c, a.slots, t0, tok, a.T, slot, held) >= 0) {
             constexpr int kRow = kTurnRow<HD, E>;
-            __shared__ __align__(16) E turn[kTile * kRow];
+            __shared__ __align__(16) E turn[U][kTile * kRow];
             const int half = tid / HD, d = tid % HD;
-            const E8 o = *reinterpret_cast<const E8 *>(v + (half * HD + d) * 8);
-            E in[8];
-            __builtin_memcpy(in, &o, sizeof o);
+            E8 o[U];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) turn[v_token(half, j) * kRow + d] = in[j];
+            for (int u = 0; u < U; ++u) o[u] = *reinterpret_cast<const E8 *>(v + of(u) * next + (half * HD + d) * 8);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                E in[8];
+                __builtin_memcpy(in, &o[u], sizeof o[u]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) turn[u][v_token(half, j) * kRow + d] = in[j];
+            }
             __syncthreads();
-            e = *reinterpret_cast<const E8 *>(&turn[tok * kRow + piece * 8]);
-        } else if (held) {
-            const E *const from = v + (v_half(in_tile) * HD + piece * 8) * 8 + v_place(in_tile);
-            E in[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) in[i] = from[i * 8];
-            __builtin_memcpy(&e, in, sizeof e);
+            for (int u = 0; u < U; ++u) e[u] = *reinterpret_cast<const E8 *>(&turn[u][tok * kRow + piece * 8]);
+        } else if (held) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const E *const from = v + of(u) * next + (v_half(in_tile) * HD + piece * 8) * 8 + v_place(in_tile);
+                E in[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) in[i] = from[i * 8];
+                __builtin_memcpy(&e[u], in, sizeof e[u]);
+            }
         }
     }
     if (!live) return;
-    float x[8];
-    if constexpr (I8) {
-        const half8 h = i8_to_half8(e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = held ? (float)h[i] * scale : 0.0f;
-    } else {
+    for (int u = 0; u < U; ++u) {
+        if (head0 + u >= heads) return;
+        float x[8];
+        if constexpr (I8) {
+            const half8 h = i8_to_half8(e[u]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
+            for (int i = 0; i < 8; ++i) x[i] = held ? (float)h[i] * scale[u] : 0.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)e[u][i];
+        }
+        store8<OF32>(is_v ? a.v_out : a.k_out, ((int64_t)t * heads + head0 + u) * HD + piece * 8, x);
     }
-    store8<OF32>(is_v ? a.v_out : a.k_out, ((int64_t)t * a.c.heads + head) * HD + piece * 8, x);
-}
-
-template <int HD, bool XF32, bool QF32>
-void launch_store(st_context *ctx, const StoreArgs &a, bool i8, dim3 grid) {
-    if (i8)
-        st::launch(ctx, store_kernel<HD, XF32, QF32, true>, grid, dim3(2 * HD), 0, a);
-    else
-        st::launch(ctx, store_kernel<HD, XF32, QF32, false>, grid, dim3(2 * HD), 0, a);
-}
-
-template <int HD>
-void launch_store(st_context *ctx, const StoreArgs &a, bool xf32, bool qf32, bool i8, dim3 grid) {
-    if (xf32)
-        qf32 ? launch_store<HD, true, true>(ctx, a, i8, grid) : launch_store<HD, true, false>(ctx, a, i8, grid);
-    else
-        qf32 ? launch_store<HD, false, true>(ctx, a, i8, grid) : launch_store<HD, false, false>(ctx, a, i8, grid);
-}
-
-template <int HD>
-void launch_read(st_context *ctx, const ReadArgs &a, bool f32, bool i8, dim3 grid) {
-    if (i8)
-        f32 ? st::launch(ctx, read_kernel<HD, true, true>, grid, dim3(2 * HD), 0, a)
-            : st::launch(ctx, read_kernel<HD, false, true>, grid, dim3(2 * HD), 0, a);
-    else
-        f32 ? st::launch(ctx, read_kernel<HD, true, false>, grid, dim3(2 * HD), 0, a)
-            : st::launch(ctx, read_kernel<HD, false, false>, grid, dim3(2 * HD), 0, a);
 }
 
 // Groups of 16 tokens; from a group's length of tokens on they start with the
 // first token's tile (a prompt that goes on within a page then fills tiles).
 bool shifted(int T) { return T >= kTile; }
 unsigned groups(int T) { return (unsigned)((T + kTile - 1) / kTile + (shifted(T) ? 1 : 0)); }
+
+template <int HD, bool XF32, bool QF32, bool I8>
+void launch_store(st_context *ctx, const StoreArgs &a) {
+    // (one head a workgroup at every length: 2047 tokens 13.6 us with one,
+    // 13.8 with two, 15.4 with four)
+    const dim3 grid(groups(a.T), (unsigned)(a.n_heads + 2 * a.c.heads));
+    st::launch(ctx, store_kernel<HD, XF32, QF32, I8>, grid, dim3(2 * HD), 0, a);
+}
+
+template <int HD, bool OF32, bool I8>
+void launch_read(st_context *ctx, const ReadArgs &a) {
+    // Four heads a workgroup where that still leaves every CU some workgroups
+    // (16384 int8 tokens of 8 heads: 28.5 us with one, 23.1 with four).
+    constexpr int kHeads = 4;
+    const int few = (a.c.heads + kHeads - 1) / kHeads;
+    const bool several = (int64_t)groups(a.T) * 2 * few >= 4 * (int64_t)ctx->num_cus;
+    const dim3 grid(groups(a.T), (unsigned)(several ? few : a.c.heads), 2);
+    if (!several)
+        st::launch(ctx, read_kernel<HD, OF32, I8, 1>, grid, dim3(2 * HD), 0, a);
+    else
+        st::launch(ctx, read_kernel<HD, OF32, I8, kHeads>, grid, dim3(2 * HD), 0, a);
+}
+
+template <int HD>
+void store_by_type(st_context *ctx, const StoreArgs &a, bool xf32, bool qf32, bool i8) {
+    if (xf32 && qf32)
+        i8 ? launch_store<HD, true, true, true>(ctx, a) : launch_store<HD, true, true, false>(ctx, a);
+    else if (xf32)
+        i8 ? launch_store<HD, true, false, true>(ctx, a) : launch_store<HD, true, false, false>(ctx, a);
+    else if (qf32)
+        i8 ? launch_store<HD, false, true, true>(ctx, a) : launch_store<HD, false, true, false>(ctx, a);
+    else
+        i8 ? launch_store<HD, false, false, true>(ctx, a) : launch_store<HD, false, false, false>(ctx, a);
+}
+
+template <int HD>
+void read_by_type(st_context *ctx, const ReadArgs &a, bool f32, bool i8) {
+    if (f32)
+        i8 ? launch_read<HD, true, true>(ctx, a) : launch_read<HD, true, false>(ctx, a);
+    else
+        i8 ? launch_read<HD, false, true>(ctx, a) : launch_read<HD, false, false>(ctx, a);
+}
 
 bool act_dtype(int d) { return d == ST_F32 || d == ST_F16; }
 bool whole16(int64_t elements, int dtype) { return elements % (dtype == ST_F32 ? 4 : 8) == 0; }
@@ -362,14 +401,13 @@ extern "C" int st_qk_norm_rope_store(st_context *ctx, const st_kv_cache *cache, 
     a.rot = rot, a.n_pos = n_pos, a.pairs = (flags & ST_FLAG_ROPE_PAIRS) != 0;
     a.positions = positions, a.slots = slots, a.q_out = q_out;
     a.T = T, a.shift = shifted(T);
-    const dim3 grid(groups(T), (unsigned)(a.n_heads + 2 * a.c.heads));
     const bool xf32 = x_dtype == ST_F32, qf32 = q_dtype == ST_F32, i8 = cache->dtype == ST_I8;
     if (hd == 64)
-        launch_store<64>(ctx, a, xf32, qf32, i8, grid);
+        store_by_type<64>(ctx, a, xf32, qf32, i8);
     else if (hd == 128)
-        launch_store<128>(ctx, a, xf32, qf32, i8, grid);
+        store_by_type<128>(ctx, a, xf32, qf32, i8);
     else
-        launch_store<256>(ctx, a, xf32, qf32, i8, grid);
+        store_by_type<256>(ctx, a, xf32, qf32, i8);
     return st::launch_check("store_kernel");
 }
 
@@ -383,13 +421,12 @@ extern "C" int st_kv_read(st_context *ctx, const st_kv_cache *cache, const int32
     if (T < 1) return st::fail(ST_ERR_SHAPE, "%s: T=%d", fn, T);
     if (!st::aligned16(k_out) || !st::aligned16(v_out)) return st::fail(ST_ERR_ALIGN, "%s: outputs must be 16-byte aligned", fn);
     a.slots = slots, a.k_out = k_out, a.v_out = v_out, a.T = T, a.shift = shifted(T);
-    const dim3 grid(groups(T), (unsigned)a.c.heads, 2);
     const bool f32 = out_dtype == ST_F32, i8 = cache->dtype == ST_I8;
     if (cache->head_dim == 64)
-        launch_read<64>(ctx, a, f32, i8, grid);
+        read_by_type<64>(ctx, a, f32, i8);
     else if (cache->head_dim == 128)
-        launch_read<128>(ctx, a, f32, i8, grid);
+        read_by_type<128>(ctx, a, f32, i8);
     else
-        launch_read<256>(ctx, a, f32, i8, grid);
+        read_by_type<256>(ctx, a, f32, i8);
     return st::launch_check("read_kernel");
 }

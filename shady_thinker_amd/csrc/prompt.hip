@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
     // (scalars: a division leaves its result in a vector register)
     const int h = scalar((int)blockIdx.x % a.c.heads), item = scalar((int)blockIdx.x / a.c.heads);
     Item it;
-    if (!find_item<kPairs, KT, 1>(a, item, it)) return;
+    if (!find_item<kPairs, KT, 1, 4>(a, item, it)) return;
     it = scalars(it);
 
     // ---- rows: the last block first
@@ -99,31 +99,32 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
     const int tile0 = key0 / 16, tiles = (it.s.kv + 15) / 16, tsh = a.c.tiles_shift();
     const auto *const pages =
         (const __attribute__((address_space(4))) int32_t *)(a.table + (int64_t)it.b * a.table_stride);
-    auto page_of = [&](int t) __attribute__((always_inline)) {
-        const int p = pages[max(min(t, tiles - 1), 0) >> tsh];
+    auto page_of = [&](int t, int p) __attribute__((always_inline)) {  // (-1: none to read)
         return t < tiles && (unsigned)p < (unsigned)a.c.num_pages ? p : -1;
     };
     // A wave fetches kPer pieces a lane, of one cache tile: its tile of the
     // KT / 16, and from which piece on.
     const int my_tile = wave * kPer * 64 * 8 / kTileE, my_piece = wave * kPer * 64 - my_tile * (kTileE / 8);
-    // Pages of the tile to fetch, a turn ahead; a bit of `missing` for each
+    // Pages of the tile to fetch, a turn ahead and as they are in the table
+    // (as attn_kernel's); a bit of `missing` for each
     // cache tile of the fetched one that is not read (it lands as zeros).
     int page[KT / 16];
     unsigned missing = 0;
     auto look = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < KT / 16; ++j) page[j] = page_of(tile0 + t * (KT / 16) + j);
+        for (int j = 0; j < KT / 16; ++j) page[j] = pages[max(min(tile0 + t * (KT / 16) + j, tiles - 1), 0) >> tsh];
     };
     look(t0);
     u32x2 kr[I8 ? kPer : 1], vr[I8 ? kPer : 1];
     float sc = 0.0f;
     auto fetch = [&](_Float16 *ks, _Float16 *vs, int t) __attribute__((always_inline)) {
-        int mine = page[0];
+        int mine = -1;
         missing = 0;
 #pragma unroll
         for (int j = 0; j < KT / 16; ++j) {
-            mine = my_tile == j ? page[j] : mine;
-            missing |= page[j] < 0 ? 1u << j : 0u;
+            const int p = page_of(tile0 + t * (KT / 16) + j, page[j]);
+            mine = my_tile == j ? p : mine;
+            missing |= p < 0 ? 1u << j : 0u;
         }
         const bool ok = mine >= 0 && t < t1;
         const int ct = tile0 + t * (KT / 16) + my_tile;
