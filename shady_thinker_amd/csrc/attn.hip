@@ -116,12 +116,12 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     const int npair = it.s.q * a.group;
     const int pair = it.rb * PB + (SPLIT ? col & 7 : col);
     const bool real = pair < npair;
-    const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
+    const int tok = real ? row_of_pair(a, pair) : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
     const int p0 = it.s.kv - it.s.q;  // position of the sequence's first row
     const int pos = real ? p0 + tok : -1;
     const int low = a.window ? max(pos - a.window + 1, 0) : 0;  // keys low .. pos are visible
     // (uniform: the block's first and last rows' positions)
-    const int pmin = p0 + scalar(it.rb * PB / a.group), pmax = p0 + scalar((min(it.rb * PB + PB, npair) - 1) / a.group);
+    const int pmin = p0 + scalar(row_of_pair(a, it.rb * PB)), pmax = p0 + scalar(row_of_pair(a, min(it.rb * PB + PB, npair) - 1));
     const int wmax = a.window ? pmax - a.window + 1 : 0;  // from here on a key is in every row's window
     const int wmin = a.window ? pmin - a.window + 1 : 0;  // before this it is in none's
     const float slope = GEN && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
@@ -389,6 +389,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
         const int mine = step < it.s1 ? (it.s1 - step + NW - 1) / NW : 0;
         F fa, fb;
         load(fa, step);
+        __builtin_amdgcn_sched_barrier(0);  // (or the queries are waited for first)
         split_q();
         for (int i = 0; i < mine / 2; ++i, step += 2 * NW) {
             load(fb, step + NW);
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     const int row_id = (int)blockIdx.x * a.c.heads + h;
     auto weight = [](float mw, float top) { return mw == -INFINITY ? 0.0f : exp2_(mw - top); };
     auto put = [&](f32x4 v, int p, int d) {
-        const int g = it.rb * PB + p, t = g / a.group;
+        const int g = it.rb * PB + p, t = row_of_pair(a, g);
         store_out(a, v, it.s.q0 + t, h * a.group + g - t * a.group, d, HD);
     };
     const __amdgpu_buffer_rsrc_t rp =
@@ -606,9 +607,14 @@ int by_type(st_context *ctx, const Args &a, bool i8, bool split) {
     return i8 ? by_scores<HD, true>(ctx, a, split) : by_scores<HD, false>(ctx, a, split);
 }
 
-// f16 rows of prompts go to the kernel with 128 pairs a workgroup.
+// f16 rows of prompts go to the kernel with 128 pairs a workgroup, where the
+// call can be large enough to fill such workgroups and pay for its second
+// launch (the host knows what the tables hold at most, not the lengths). Both
+// ways, 32/8 heads of 128, in us, this kernel first: 16 rows over 8192 tokens
+// 30.6 and 19.6, over 2048 16.5 and 14, over 600 8.9 and 13; 64 rows over 600
+// 11.4 and 15; 512 over 512 24 and 24, 4096 over 4096 674 and 167.
 bool use_prompt(const st_context *ctx, const Args &a) {
-    return (int64_t)a.T * a.group >= 32 * (int64_t)a.B;
+    return (int64_t)a.T * a.group >= 32 * (int64_t)a.B && (int64_t)a.T * a.group * a.capacity >= 1 << 19;
 }
 
 bool act_dtype(int d) { return d == ST_F32 || d == ST_F16; }
@@ -666,6 +672,7 @@ extern "C" int st_paged_attention(st_context *ctx, const st_kv_cache *cache, con
     a.gate_stride = gate_stride, a.gate_head_stride = gate_head_stride;
     a.table_stride = table_stride, a.capacity = table_stride << a.c.page_shift;
     a.T = T, a.B = B, a.n_heads = n_heads, a.group = n_heads / a.c.heads;
+    a.group_shift = (a.group & (a.group - 1)) == 0 ? __builtin_ctz(a.group) : -1;
     a.window = std::min(window, 1 << 30), a.scale = scale, a.cap = cap;
     a.q_f32 = q_dtype == ST_F32, a.gate_f32 = gate_dtype == ST_F32, a.out_f32 = out_dtype == ST_F32;
     const bool i8 = cache->dtype == ST_I8, split = a.q_f32 || a.out_f32;

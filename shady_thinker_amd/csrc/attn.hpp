@@ -24,6 +24,7 @@ struct Args {
     int gate_head_stride;
     int table_stride, capacity;  // pages of a table row, tokens they hold
     int T, B, n_heads, group;    // group: query heads of a key head
+    int group_shift;             // its logarithm, -1: not a power of two
     int window;                  // 0: none
     float scale, cap;            // cap 0: none
     bool q_f32, gate_f32, out_f32;
@@ -44,6 +45,10 @@ __device__ __forceinline__ int scalar(int v) {
     int r;
     asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(r) : "v"(v));
     return r;
+}
+// A pair's row.
+__device__ __forceinline__ int row_of_pair(const Args &a, int pair) {
+    return a.group_shift >= 0 ? pair >> a.group_shift : pair / a.group;
 }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -91,7 +96,7 @@ constexpr int kMostSteps = 1 << 27;  // steps of a sequence (of 16 keys at least
 
 template <int PB>
 __device__ __forceinline__ int blocks_of(const Args &a, const Seq &s) {
-    return (s.q * a.group + PB - 1) / PB;
+    return (int)((unsigned)(s.q * a.group + PB - 1) / PB);
 }
 template <int STEP>
 __device__ __forceinline__ int steps_of(const Args &a, const Seq &s) {
@@ -100,9 +105,9 @@ __device__ __forceinline__ int steps_of(const Args &a, const Seq &s) {
 
 // C: chunks of C steps so that all items fit the grid: sum over blocks of
 // ceil(steps / C) <= work / C + blocks <= G. A multiple of LEAST.
-template <int LEAST>
+template <int LEAST, int WHOLE>
 __device__ __forceinline__ int chunk_steps(const Args &a, unsigned long long work, int blocks, int longest) {
-    if (!a.split) return kMostSteps;
+    if (!a.split || longest <= WHOLE) return kMostSteps;
     const unsigned room = (unsigned)max(a.G - blocks, 1);
     const unsigned long long up = work + room - 1;
     unsigned long long c = up >> 32 ? up / room : (unsigned)up / room;
@@ -128,10 +133,10 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
         it.b = 0;
         it.blocks = blocks_of<PB>(a, it.s);
         if (!it.blocks) return false;
-        const int steps = steps_of<STEP>(a, it.s), C = chunk_steps<LEAST>(a, (unsigned long long)it.blocks * steps, it.blocks, steps);
+        const int steps = steps_of<STEP>(a, it.s), C = chunk_steps<LEAST, WHOLE>(a, (unsigned long long)it.blocks * steps, it.blocks, steps);
         it.chunks = chunks_of<WHOLE>(steps, C);
         if (w >= it.blocks * it.chunks) return false;
-        it.rb = w % it.blocks, it.chunk = w / it.blocks;
+        it.chunk = it.blocks == 1 ? w : w / it.blocks, it.rb = w - it.chunk * it.blocks;
         it.first = it.rb, it.counter = it.rb;
         it.s0 = min(it.chunk * C, steps), it.s1 = it.chunks == 1 ? steps : min(it.s0 + C, steps);
         return true;
@@ -155,7 +160,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
     // (more row blocks than T rows have: q_start decreases somewhere. The
     // counters and the grid are made for a.rows, so nothing is computed)
     if (uniform(blocks) > a.rows) return false;
-    const int C = chunk_steps<LEAST>(a, work, uniform(blocks), uniform(longest));
+    const int C = chunk_steps<LEAST, WHOLE>(a, work, uniform(blocks), uniform(longest));
     int items = 0, rows = 0;  // before this turn's sequences
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int b = b0 + lane;
@@ -180,7 +185,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
             it.s = Seq{of(s.q0), of(s.q), of(s.kv)};
             it.blocks = of(n), it.chunks = of(chunks);
             const int begin = items + of(upto) - it.blocks * it.chunks, idx = w - begin;
-            it.rb = idx % it.blocks, it.chunk = idx / it.blocks;
+            it.chunk = it.blocks == 1 ? idx : idx / it.blocks, it.rb = idx - it.chunk * it.blocks;
             it.first = begin + it.rb;
             it.counter = rows + of(rows_upto) - it.blocks + it.rb;
             const int st = of(steps);

@@ -18,8 +18,8 @@
 //  * All workgroups of a key head run on one XCD where the head count allows,
 //    so a head's K and V are read from HBM once; the last rows, which see
 //    most keys, start first.
-//  * Few rows over a long cache: chunks of the keys, joined by the last one
-//    to count in, as attn_kernel's.
+//  * Few rows over a long cache: chunks of the keys, joined by a second
+//    launch.
 #include "attn.hpp"
 
 namespace {
@@ -27,10 +27,16 @@ namespace {
 using namespace st::attn;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kPairs = 32 * kWaves;
 constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
-constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
+constexpr int kJoin = 4;                // parts of a join's workgroup
+// Tiles of a chunk at least; of a sequence that stays in one chunk. (16 and 32
+// rows over 8192 tokens: 19.6 and 21.1 us with 4 tiles at least, 22.5 and 24.4
+// with 2, 22.4 and 24.6 with 1; 128 rows: 40.1, 37.3, 37.4; 64 rows over 2048:
+// 17.6 with 8 tiles in one chunk, 21.4 with 4.)
+constexpr int kLeast = 4, kWhole = 8;
 constexpr float kSlack = 8.0f;          // growth of a maximum that is let pass, in powers of two
 
 // (a helper of its own: written inside a kernel template the host pass drops
@@ -54,13 +60,12 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
     constexpr int kPer = KT * HD / 8 / (64 * kWaves);     // 16-byte pieces of K (and of V) a lane fetches per tile
     __shared__ __align__(16) _Float16 k0s[KT * HD], v0s[KT * HD], k1s[KT * HD], v1s[KT * HD];
     __shared__ __align__(16) float scales[I8 ? 2 : 1][2][I8 ? KT : 1];  // [stage][k, v]
-    __shared__ unsigned s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int col = lane & 31, hf = lane >> 5;
     // (scalars: a division leaves its result in a vector register)
     const int h = scalar((int)blockIdx.x % a.c.heads), item = scalar((int)blockIdx.x / a.c.heads);
     Item it;
-    if (!find_item<kPairs, KT, 1, 4>(a, item, it)) return;
+    if (!find_item<kPairs, KT, kLeast, kWhole>(a, item, it)) return;
     it = scalars(it);
 
     // ---- rows: the last block first
@@ -358,86 +363,111 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
         return;
     }
 
-    // ---- chunks: as attn_kernel's; a lane joins what it would have written
-    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void *)a.part, (short)0, a.G * a.c.heads * kPairs * HD * 4, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rm = __builtin_amdgcn_make_buffer_rsrc((void *)a.part_ml, (short)0, a.G * a.c.heads * kPairs * 8, kRsrcWord3);
+    // ---- a chunk: its sums to memory, four dims of the block's pairs at a time
+    if (!real) return;
     const int mine = 32 * wave + col;
-    auto at = [&](int i) { return (unsigned)((i * a.c.heads + h) * kPairs + mine); };
-    if (real) {
-        const unsigned r = at(item);
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 v = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rp, (r * HD + 32 * d + 8 * g + 4 * hf) * 4, 0, kCoherent);
-            }
-        if (hf == 0)
-            __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, rm, r * 8, 0, kCoherent);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's partial results are in memory
-    __syncthreads();
-    if (tid == 0) {
-        unsigned *const cnt = a.cnt + st::spread_counter(it.counter * a.c.heads + h);
-        const unsigned done = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        s_last = done == (unsigned)it.chunks - 1;
-        if (s_last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    }
-    __syncthreads();
-    if (!s_last || !real) return;
-    auto ml_of = [&](int c, float &mc, float &lc) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, at(it.first + c * it.blocks) * 8, 0, kCoherent));
-        const unsigned w0 = w.x, w1 = w.y;
-        mc = __uint_as_float(w0), lc = __uint_as_float(w1);
-    };
-    float top = -INFINITY, total = 0.0f;
-    for (int c = 0; c < it.chunks; ++c) {
-        float mc, lc;
-        ml_of(c, mc, lc);
-        const float mn = fmaxf(top, mc);
-        if (mn > -INFINITY) total = total * exp2_(top - mn) + (mc == -INFINITY ? 0.0f : lc * exp2_(mc - mn));
-        top = mn;
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    for (int c = 0; c < it.chunks; ++c) {
-        float mc, lc;
-        ml_of(c, mc, lc);
-        const float w = mc == -INFINITY ? 0.0f : exp2_(mc - top) * inv;
-        const unsigned r = at(it.first + c * it.blocks);
-        u32x4 v[ND][4];
+    const int64_t at = (int64_t)item * a.c.heads + h;
+    if (t1 > t0) {
+        f32x4 *const part = reinterpret_cast<f32x4 *>(a.part) + at * (HD / 4) * kPairs + mine;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                v[d][g] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, (r * HD + 32 * d + 8 * g + 4 * hf) * 4, 0, kCoherent));
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 f = __builtin_bit_cast(f32x4, v[d][g]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[d][4 * g + i] = fmaf(w, f[i], o[d][4 * g + i]);
-            }
+                part[(8 * d + 2 * g + hf) * kPairs] = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
     }
+    if (hf == 0) reinterpret_cast<f32x2 *>(a.part_ml)[at * kPairs + mine] = f32x2{m, l};
+}
+
+// The chunks of prompt_kernel joined, a launch of its own: the sums of a chunk
+// are 64 KiB at 128 dims, which one workgroup (the last to count in) took
+// 3 us a chunk to read; here the workgroups of a block's chunks share its dims.
+// 77 rows over 8192 tokens, 32/8 heads of 128: 35 us with both launches, 82
+// with the join in the first.
+template <int HD>
+__global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
+    constexpr int N = 8;  // chunks asked for at once
+    __shared__ __align__(16) f32x4 sums[kJoin - 1][kPairs];
+    __shared__ __align__(8) f32x2 tops[kJoin - 1][kPairs];
+    const int tid = threadIdx.x, mine = tid % kPairs, part = uniform(tid / kPairs);
+    const int h = scalar((int)blockIdx.x % a.c.heads), item = scalar((int)blockIdx.x / a.c.heads);
+    Item it;
+    if (!find_item<kPairs, kKeys<HD>, kLeast, kWhole>(a, item, it) || it.chunks == 1) return;
+    it = scalars(it);
+    const int pair = (it.blocks - 1 - it.rb) * kPairs + mine;
+    const bool real = pair < it.s.q * a.group;
+    const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
+    const int share = scalar((HD / 4 + it.chunks - 1) / it.chunks);  // groups of four dims
+    const int end = min((it.chunk + 1) * share, HD / 4);
+    // many chunks: cut among the parts, else the dims are
+    const bool cut = it.chunks > 2 * N;
+    const int each = cut ? (it.chunks + kJoin - 1) / kJoin : it.chunks;
+    const int first = cut ? part * each : 0, last = min(first + each, it.chunks);
+    const int64_t at = (int64_t)it.first * a.c.heads + h, next = (int64_t)it.blocks * a.c.heads;
+    const f32x2 *const ml = reinterpret_cast<const f32x2 *>(a.part_ml) + at * kPairs + mine;
+    // (the workgroup's turns are the same for all its waves)
+    for (int d0 = it.chunk * share; d0 < end; d0 += cut ? 1 : kJoin) {
+        const int d = cut ? d0 : min(d0 + part, end - 1);
+        const f32x4 *const from = reinterpret_cast<const f32x4 *>(a.part) + (at * (HD / 4) + d) * kPairs + mine;
+        float top = -INFINITY, total = 0.0f;
+        f32x4 sum = {};
+        auto add = [&](const f32x2 *x, const f32x4 *v, int n) __attribute__((always_inline)) {
+            float high = top;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+            for (int i = 0; i < N; ++i) high = fmaxf(high, i < n ? x[i][0] : -INFINITY);
+            if (high == -INFINITY) return;  // (a chunk that the row does not see holds no sums)
+            const float was = exp2_(top - high);
+            top = high, total *= was;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            store_out(a, f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]}, row, head, 32 * d + 8 * g + 4 * hf, HD);
+            for (int k = 0; k < 4; ++k) sum[k] *= was;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool use = i < n && x[i][0] > -INFINITY;
+                const float w = use ? exp2_(x[i][0] - high) : 0.0f;
+                total = use ? fmaf(w, x[i][1], total) : total;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum[k] = use ? fmaf(w, v[i][k], sum[k]) : sum[k];
+            }
+        };
+        for (int c0 = first; c0 < last; c0 += N) {
+            f32x2 x[N];
+            f32x4 v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = min(c0 + i, last - 1);
+                x[i] = ml[c * next * kPairs];
+                v[i] = from[c * next * (HD / 4) * kPairs];
+            }
+            add(x, v, last - c0);
+        }
+        if (cut) {
+            if (part) sums[part - 1][mine] = sum, tops[part - 1][mine] = f32x2{top, total};
+            __syncthreads();
+            f32x2 x[N];
+            f32x4 v[N];
+#pragma unroll
+            for (int i = 0; i < kJoin - 1; ++i) x[i] = tops[i][mine], v[i] = sums[i][mine];
+            __syncthreads();
+            if (part) continue;
+            add(x, v, kJoin - 1);
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (real && (cut || d0 + part < end))
+            store_out(a, f32x4{sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv}, it.s.q0 + tok, head, 4 * d, HD);
+    }
 }
 
 template <int HD, bool I8, bool GEN>
 int launch_prompt(st_context *ctx, Args a) {
     const int heads = a.c.heads;
-    // chunks only where the row blocks alone leave CUs without work
-    const int64_t blocks = ((int64_t)a.T * a.group + kPairs - 1) / kPairs * heads, slots = 2 * ctx->num_cus;
-    if (int rc = plan_cut(ctx, a, kPairs, HD, kKeys<HD>, 1, (slots - blocks) / heads)) return rc;
+    // chunks only where the row blocks alone leave CUs without work (at 256 dims
+    // a CU holds one workgroup: 77 rows over 8192 tokens, 16 heads of 256, 71 us
+    // with as many chunks as fit at once, 80 with twice that)
+    const int64_t blocks = ((int64_t)a.T * a.group + kPairs - 1) / kPairs * heads, slots = (HD == 256 ? 1 : 2) * ctx->num_cus;
+    if (int rc = plan_cut(ctx, a, kPairs, HD, kKeys<HD>, kLeast, (slots - blocks) / heads)) return rc;
     st::launch(ctx, prompt_kernel<HD, I8, GEN>, dim3((unsigned)(a.G * heads)), dim3(64 * kWaves), 0, a);
-    return st::launch_check("prompt_kernel");
+    if (int rc = st::launch_check("prompt_kernel"); rc || !a.split) return rc;
+    st::launch(ctx, prompt_join_kernel<HD>, dim3((unsigned)(a.G * heads)), dim3(kJoin * kPairs), 0, a);
+    return st::launch_check("prompt_join_kernel");
 }
 
 template <int HD>
