@@ -93,10 +93,16 @@ __device__ __forceinline__ float half_turn(float v) { return dpp<0x128>(v); }  /
 template <int HD>
 constexpr bool kTwo = HD <= 128;
 
-// GEN: capped scores or slopes. NTL: non-temporal loads of the cache.
-template <int HD, bool I8, bool SPLIT, bool GEN, bool NTL, int NW>
+// What a call's rows are like.
+constexpr int kRows = 0;    // sequences of several rows, perhaps
+constexpr int kOne = 1;     // one row each: a block's pairs see the same keys
+constexpr int kOneNt = 2;   // the same, and the cache by non-temporal loads
+
+// GEN: capped scores or slopes.
+template <int HD, bool I8, bool SPLIT, bool GEN, int MODE, int NW>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     constexpr int PB = SPLIT ? 8 : 16;  // pairs of a block
+    constexpr bool NTL = MODE == kOneNt, ONE = MODE != kRows;
     constexpr int ST = kStep<I8>, SUB = ST / 32, NS = HD / 32, ND = HD / 16, kRow = HD + 4, NT = 64 * NW;
     using F = Frag<HD, I8>;
     using E = std::conditional_t<I8, signed char, _Float16>;
@@ -223,6 +229,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     int ve = -126;  // int8: weights are held times their value scale over 2^ve
+    unsigned odd = 0;  // values that were not finite and not seen by every row
 
     auto compute = [&](F &f, int step) __attribute__((always_inline)) {
         const int kb = key0 + ST * step;
@@ -239,7 +246,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
             const int k = kb + lane;
             const bool any = (f.ok >> q4 & 1) && k <= pmax && k >= wmin;
             const float vs = any ? f.vs : 0.0f;
-            float top = vs;
+            // (one that is not finite makes its rows NaN by itself; in `top` it
+            // would drown the rows that do not see it)
+            float top = vs < INFINITY ? vs : 0.0f;
             top = fmaxf(top, dpp<0x121>(top)), top = fmaxf(top, dpp<0x122>(top));
             top = fmaxf(top, dpp<0x124>(top)), top = fmaxf(top, dpp<0x128>(top));
             top = max_q4(top);
@@ -306,6 +315,20 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
                         w[j & 7] = any ? w[j & 7] : (_Float16)0.0f;
                         f.v[j >> 3][d] = __builtin_bit_cast(u32x4, w);
                     }
+                }
+            }
+            if constexpr (!I8 && !ONE) {
+                // 0 times a value that is not finite is a NaN, also for rows
+                // that do not see it: zero too, until the loop is done
+                if (pmin != pmax) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const unsigned w = f.v[0][d][i], t = not_finite(w);
+                            odd |= t;
+                            f.v[0][d][i] = finite(w, t);
+                        }
                 }
             }
         }
@@ -406,6 +429,39 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
         for (int step = it.s0 + wave; step < it.s1; step += NW) {
             load(f, step);
             compute(f, step);
+        }
+    }
+
+    if constexpr (!I8 && !ONE) {
+        // Such values again, for the rows that see them: their sums are
+        // infinite of the value's sign, or NaN, whatever the weight.
+        if (__ballot(odd != 0)) {
+            look(it.s0 + wave);
+            for (int step = it.s0 + wave; step < it.s1; step += NW) {
+                F f;
+                load(f, step);
+                half8 see;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int k = key0 + ST * step + 16 * (q4 >> 1) + 4 * (q4 & 1) + (j & 3) + 8 * (j >> 2);
+                    see[j] = (f.ok >> (q4 >> 1) & 1) && k >= low && k <= pos ? (_Float16)1.0f : (_Float16)0.0f;
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    half8 v = __builtin_bit_cast(half8, f.v[0][d]), up, down;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool bad = !(fabsf((float)v[j]) < INFINITY);
+                        up[j] = bad && !(v[j] < (_Float16)0.0f) ? (_Float16)1.0f : (_Float16)0.0f;  // +inf, NaN
+                        down[j] = bad && !(v[j] > (_Float16)0.0f) ? (_Float16)1.0f : (_Float16)0.0f;
+                    }
+                    const f32x4 none = {0, 0, 0, 0};
+                    const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_f16(up, see, none, 0, 0, 0);
+                    const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(down, see, none, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][i] += (n[i] > 0.0f ? INFINITY : 0.0f) + (m[i] > 0.0f ? -INFINITY : 0.0f);
+                }
+            }
         }
     }
 
@@ -573,13 +629,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     }
 }
 
-template <int HD, bool I8, bool SPLIT, bool GEN, bool NTL>
+template <int HD, bool I8, bool SPLIT, bool GEN, int MODE>
 int launch_attn(st_context *ctx, Args a) {
     constexpr int PB = SPLIT ? 8 : 16, NW = 4;
     const int64_t slots = 2 * ctx->num_cus;
     if (int rc = plan_cut(ctx, a, PB, HD, kStep<I8>, kLeast<I8>, slots / a.c.heads)) return rc;
     const size_t lds = (size_t)NW * PB * (HD + 4) * sizeof(float);
-    auto kern = attn_kernel<HD, I8, SPLIT, GEN, NTL, NW>;
+    auto kern = attn_kernel<HD, I8, SPLIT, GEN, MODE, NW>;
     if (lds > 32 * 1024)
         ST_HIP(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     st::launch(ctx, kern, dim3((unsigned)a.G, (unsigned)a.c.heads), dim3(64 * NW), lds, a);
@@ -591,8 +647,9 @@ int by_size(st_context *ctx, const Args &a) {
     // A cache that no more than one row block reads, and that is larger than
     // what a cache level keeps between calls
     const int64_t bytes = (int64_t)a.B * a.capacity * a.c.heads * HD * (I8 ? 2 : 4);
-    const bool once = a.T == a.B && a.group <= (SPLIT ? 8 : 16) && bytes >= (int64_t)96 << 20;
-    return once ? launch_attn<HD, I8, SPLIT, GEN, true>(ctx, a) : launch_attn<HD, I8, SPLIT, GEN, false>(ctx, a);
+    const bool once = !a.q_start && a.group <= (SPLIT ? 8 : 16) && bytes >= (int64_t)96 << 20;
+    if (once) return launch_attn<HD, I8, SPLIT, GEN, kOneNt>(ctx, a);
+    return a.q_start ? launch_attn<HD, I8, SPLIT, GEN, kRows>(ctx, a) : launch_attn<HD, I8, SPLIT, GEN, kOne>(ctx, a);
 }
 
 template <int HD, bool I8>

@@ -33,6 +33,8 @@ struct Args {
     int G, split, rows;  // rows: row blocks at most
     float *part, *part_ml;
     unsigned *cnt;
+    // prompts: *odd becomes call where a block left out values (odd_values)
+    unsigned *odd, call;
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -203,6 +205,14 @@ __device__ __forceinline__ bool find_item(const Args &a, int w, Item &it) {
 __device__ __forceinline__ Item scalars(const Item &it) {
     return Item{Seq{scalar(it.s.q0), scalar(it.s.q), scalar(it.s.kv)}, scalar(it.b), scalar(it.rb), scalar(it.blocks),
                 scalar(it.chunk), scalar(it.chunks), scalar(it.s0), scalar(it.s1), scalar(it.first), scalar(it.counter)};
+}
+
+// Sign bits set where a half of w is an infinity or a NaN; w with zeros there.
+__device__ __forceinline__ unsigned not_finite(unsigned w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ unsigned finite(unsigned w, unsigned odd) { return w & ~((odd - (odd >> 15)) | odd); }
+__device__ __forceinline__ unsigned not_finite(half8 v) {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    return not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
 }
 
 // Where the output's eight or four values go: times sigmoid(gate) where there

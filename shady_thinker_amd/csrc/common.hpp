@@ -26,6 +26,9 @@ struct st_context {
     // split-K counters of the decode kernels (kSplitCounters words, zero
     // between calls: the last slice of each tile group clears its own)
     unsigned *split_counters = nullptr;
+    // in the line after them: the prompt attention's call that has to look at
+    // its values again; the number of such calls
+    unsigned calls = 0;
     // the no-allocation entry point's scratch on this context's GPU (the
     // device address of runtime.hip's static array)
     void *scratch = nullptr;

@@ -45,6 +45,9 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, _Float16 *lds, u
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, off, 0, 0, 0);
 }
 
+// A barrier for LDS alone (__syncthreads also waits for the tile on its way).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ float other_half(float v) {  // lane ^ 32
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
@@ -83,6 +86,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
     const bool working = wfirst < npair;
     const int wmin = p0 + scalar(wfirst / a.group), wmax = p0 + scalar((min(wfirst + 32, npair) - 1) / a.group);
     const int blow = a.window ? max(bmin - a.window + 1, 0) : 0;    // no row of the block sees keys before this
+    const int bhigh = a.window ? bmax - a.window + 1 : 0;           // from here on keys are in every window of the block
     const int wlow = a.window ? max(wmin - a.window + 1, 0) : 0;    // the same for the wave
     const int whigh = a.window ? wmax - a.window + 1 : 0;           // from here on keys are in every window of the wave
     const float slope = GEN && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
@@ -258,7 +262,9 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
         l += sum;
         if constexpr (I8) {
             const float mine = scales[stage][1][lane % KT];
-            float top = kb + lane % KT >= blow && kb + lane % KT <= bmax ? mine : 0.0f;
+            // (one that is not finite makes its rows NaN by itself; in `top` it
+            // would drown the rows that do not see it)
+            float top = kb + lane % KT >= blow && kb + lane % KT <= bmax && mine < INFINITY ? mine : 0.0f;
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
             const int e = max(ve, (int)((__float_as_uint(top) >> 23) & 255) - 126);  // top / 2^e < 1
@@ -294,22 +300,40 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(vp + 256 * d), p, o[d], 0, 0, 0);
             }
     };
-    // f16: zeros in the place of values that no row of the block sees (they
-    // may be anything, and 0 times anything has to be 0).
+    // f16 values, where some row of the block does not see the tile's every
+    // key: 0 times a value that is not finite is a NaN. Those that no row sees
+    // may be anything and become zeros; others become zeros too, and the second
+    // launch puts them where they are seen. (Without this 4096 rows take 165 us,
+    // not 171; 1000 rows over 32000 tokens 720, not 820, though only the last
+    // tiles of a block come here.)
     auto clean = [&](_Float16 *vs, int t) __attribute__((always_inline)) {
         const int kb = key0 + t * KT;
-        if (I8 || (kb + KT - 1 <= bmax && kb >= blow)) return;  // (uniform)
+        if (I8 || (kb + KT - 1 <= bmin && kb >= bhigh)) return;  // (uniform)
+        const bool edge = kb + KT - 1 > bmax || kb < blow;
         for (int i = tid; i < KT * HD / 8; i += 64 * kWaves) {
             const int tile = i / (kTileE / 8), half = i % (kTileE / 8) / HD;
-            half8 v = *reinterpret_cast<half8 *>(vs + i * 8);
+            u32x4 *const at = reinterpret_cast<u32x4 *>(vs + i * 8);
+            u32x4 w = *at;
+            if (edge) {
+                half8 v = __builtin_bit_cast(half8, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = kb + 16 * tile + v_token(half, j);
-                v[j] = k >= blow && k <= bmax ? v[j] : (_Float16)0.0f;
+                for (int j = 0; j < 8; ++j) {
+                    const int k = kb + 16 * tile + v_token(half, j);
+                    v[j] = k >= blow && k <= bmax ? v[j] : (_Float16)0.0f;
+                }
+                w = __builtin_bit_cast(u32x4, v);
             }
-            *reinterpret_cast<half8 *>(vs + i * 8) = v;
+            unsigned any = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned x = w[j], n = not_finite(x);
+                any |= n;
+                w[j] = finite(x, n);
+            }
+            if (edge || any) *at = w;
+            if (__builtin_expect(any != 0, 0)) *a.odd = a.call;
         }
-        __syncthreads();
+        lds_barrier();
     };
 
     auto turn = [&](_Float16 *ks, _Float16 *vs, _Float16 *kn, _Float16 *vn, int stage, int t) __attribute__((always_inline)) {
@@ -348,41 +372,71 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], ve);
     }
-    const int row = it.s.q0 + tok;
-    if (it.chunks == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees nothing is zero)
-        if (real) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 v = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
-                    store_out(a, v, row, head, 32 * d + 8 * g + 4 * hf, HD);
-                }
-        }
-        return;
-    }
-
-    // ---- a chunk: its sums to memory, four dims of the block's pairs at a time
-    if (!real) return;
-    const int mine = 32 * wave + col;
+    // ---- the rows, or a chunk's sums to memory, four dims of the block's pairs
+    // at a time
+    const int row = it.s.q0 + tok, mine = 32 * wave + col;
     const int64_t at = (int64_t)item * a.c.heads + h;
-    if (t1 > t0) {
-        f32x4 *const part = reinterpret_cast<f32x4 *>(a.part) + at * (HD / 4) * kPairs + mine;
+    f32x4 *const part = reinterpret_cast<f32x4 *>(a.part) + at * (HD / 4) * kPairs + mine;
+    if (real && it.chunks == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees nothing is zero)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                part[(8 * d + 2 * g + hf) * kPairs] = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = {o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+                store_out(a, v, row, head, 32 * d + 8 * g + 4 * hf, HD);
+            }
+    } else if (real) {
+        if (t1 > t0) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    part[(8 * d + 2 * g + hf) * kPairs] = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        }
+        if (hf == 0) reinterpret_cast<f32x2 *>(a.part_ml)[at * kPairs + mine] = f32x2{m, l};
     }
-    if (hf == 0) reinterpret_cast<f32x2 *>(a.part_ml)[at * kPairs + mine] = f32x2{m, l};
 }
 
-// The chunks of prompt_kernel joined, a launch of its own: the sums of a chunk
-// are 64 KiB at 128 dims, which one workgroup (the last to count in) took
-// 3 us a chunk to read; here the workgroups of a block's chunks share its dims.
-// 77 rows over 8192 tokens, 32/8 heads of 128: 35 us with both launches, 82
-// with the join in the first.
+// Sum of the f16 values of dims 4 d .. 4 d + 3 that are not finite, that keys
+// low .. pos have, over the tiles where prompt_kernel left such values out
+// (those that some row of the block, at positions bmin .. bmax, does not see).
+template <int HD>
+__device__ f32x4 odd_values(const Args &a, const Item &it, int h, int d, int bmin, int bmax, int low, int pos) {
+    constexpr int KT = kKeys<HD>;
+    const int key0 = first_key<KT>(a, it.s), steps = steps_of<KT>(a, it.s), tsh = a.c.tiles_shift();
+    const int blow = a.window ? max(bmin - a.window + 1, 0) : 0, bhigh = a.window ? bmax - a.window + 1 : 0;
+    f32x4 sum = {};
+    for (int t = 0; t < steps; ++t) {
+        const int kb = key0 + t * KT;
+        if (kb > bmax || kb + KT <= blow || (kb + KT - 1 <= bmin && kb >= bhigh)) continue;
+        for (int k = kb; k < kb + KT; k += 4) {  // places of one half of a piece
+            if (k > pos || k + 3 < low) continue;
+            const int p = a.table[(int64_t)it.b * a.table_stride + (k >> 4 >> tsh)];
+            if ((unsigned)p >= (unsigned)a.c.num_pages) continue;
+            const int64_t tile = a.c.tile(p, h, (k >> 4) & ((1 << tsh) - 1));
+            const _Float16 *const v = static_cast<const _Float16 *>(a.c.v) + tile * (16 * HD) + v_half(k & 15) * (HD * 8) + v_place(k & 15);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half4 x = *reinterpret_cast<const half4 *>(v + (4 * d + i) * 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float y = (float)x[j];
+                    sum[i] += k + j >= low && k + j <= pos && !(fabsf(y) < INFINITY) ? y : 0.0f;
+                }
+            }
+        }
+    }
+    return sum;
+}
+
+// After prompt_kernel: its chunks joined. A launch of its own: the sums of a
+// chunk are 64 KiB at 128 dims, which one workgroup (the last to count in) took
+// 3 us a chunk to read; here the workgroups of a block's chunks share its dims
+// (77 rows over 8192 tokens, 32/8 heads of 128: 35 us with both launches, 82
+// with the join in the first). And the values that prompt_kernel left out, if
+// it met any: a sum with one is infinite of its sign, or NaN, whatever the
+// weight.
 template <int HD>
 __global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
     constexpr int N = 8;  // chunks asked for at once
@@ -391,11 +445,32 @@ __global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
     const int tid = threadIdx.x, mine = tid % kPairs, part = uniform(tid / kPairs);
     const int h = scalar((int)blockIdx.x % a.c.heads), item = scalar((int)blockIdx.x / a.c.heads);
     Item it;
-    if (!find_item<kPairs, kKeys<HD>, kLeast, kWhole>(a, item, it) || it.chunks == 1) return;
+    const bool odd = uniform(*a.odd) == a.call;  // (a stale one costs time, no more)
+    if (!a.split && !odd) return;
+    if (!find_item<kPairs, kKeys<HD>, kLeast, kWhole>(a, item, it)) return;
     it = scalars(it);
-    const int pair = (it.blocks - 1 - it.rb) * kPairs + mine;
+    if (it.chunks == 1 && !odd) return;
+    const int block = it.blocks - 1 - it.rb, pair = block * kPairs + mine;
     const bool real = pair < it.s.q * a.group;
     const int tok = real ? pair / a.group : 0, head = h * a.group + (real ? pair - tok * a.group : 0);
+    const int p0 = it.s.kv - it.s.q, npair = it.s.q * a.group, pos = real ? p0 + tok : -1;
+    auto odd_sum = [&](int d) {
+        return odd_values<HD>(a, it, h, d, p0 + block * kPairs / a.group, p0 + (min(block * kPairs + kPairs, npair) - 1) / a.group,
+                              a.window ? max(pos - a.window + 1, 0) : 0, pos);
+    };
+    if (it.chunks == 1) {
+        for (int d = part; d < HD / 4; d += kJoin) {
+            const f32x4 sum = odd_sum(d);
+            if (!real || (sum[0] == 0.0f && sum[1] == 0.0f && sum[2] == 0.0f && sum[3] == 0.0f)) continue;
+            const int row = it.s.q0 + tok;
+            const f32x4 v = gated(a, sum, row, head, 4 * d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (sum[i] != 0.0f)
+                    static_cast<_Float16 *>(a.out)[((int64_t)row * a.n_heads + head) * HD + 4 * d + i] = (_Float16)v[i];
+        }
+        return;
+    }
     const int share = scalar((HD / 4 + it.chunks - 1) / it.chunks);  // groups of four dims
     const int end = min((it.chunk + 1) * share, HD / 4);
     // many chunks: cut among the parts, else the dims are
@@ -451,6 +526,11 @@ __global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
             add(x, v, kJoin - 1);
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (odd) {
+            const f32x4 more = odd_sum(d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += more[i];
+        }
         if (real && (cut || d0 + part < end))
             store_out(a, f32x4{sum[0] * inv, sum[1] * inv, sum[2] * inv, sum[3] * inv}, it.s.q0 + tok, head, 4 * d, HD);
     }
@@ -464,8 +544,9 @@ int launch_prompt(st_context *ctx, Args a) {
     // with as many chunks as fit at once, 80 with twice that)
     const int64_t blocks = ((int64_t)a.T * a.group + kPairs - 1) / kPairs * heads, slots = (HD == 256 ? 1 : 2) * ctx->num_cus;
     if (int rc = plan_cut(ctx, a, kPairs, HD, kKeys<HD>, kLeast, (slots - blocks) / heads)) return rc;
+    a.odd = ctx->split_counters + st::kSplitCounters, a.call = ++ctx->calls;
     st::launch(ctx, prompt_kernel<HD, I8, GEN>, dim3((unsigned)(a.G * heads)), dim3(64 * kWaves), 0, a);
-    if (int rc = st::launch_check("prompt_kernel"); rc || !a.split) return rc;
+    if (int rc = st::launch_check("prompt_kernel"); rc || (I8 && !a.split)) return rc;
     st::launch(ctx, prompt_join_kernel<HD>, dim3((unsigned)(a.G * heads)), dim3(kJoin * kPairs), 0, a);
     return st::launch_check("prompt_join_kernel");
 }

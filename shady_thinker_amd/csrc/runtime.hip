@@ -101,8 +101,8 @@ int st_context_create(int device, st_context **out) {
         return st::hip_fail(e, "st_context_create: workspace");
     }
     ctx->ws_bytes = kDefaultWorkspace;
-    e = hipMalloc(&ctx->split_counters, st::kSplitCounters * sizeof(unsigned));
-    if (e == hipSuccess) e = hipMemset(ctx->split_counters, 0, st::kSplitCounters * sizeof(unsigned));
+    e = hipMalloc(&ctx->split_counters, (st::kSplitCounters + 32) * sizeof(unsigned));
+    if (e == hipSuccess) e = hipMemset(ctx->split_counters, 0, (st::kSplitCounters + 32) * sizeof(unsigned));
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         if (ctx->split_counters) (void)hipFree(ctx->split_counters);

@@ -16,6 +16,7 @@ import pytest
 import torch
 
 import shady_thinker_amd as sta
+from shady_thinker_amd._lib import launches
 from attn_util import attention, indices, norm_rope, rel, shapes
 
 pytestmark = pytest.mark.gpu
@@ -177,15 +178,17 @@ def test_read(gpu, hd, nkv, T, page, cd, od, where):
 class Batch:
     """A cache with random tokens of sequences of given (rows, kv_len), pages
     in random order, everything no row may see set to NaN (f16) or to NaN
-    scales (int8)."""
+    scales (int8). wide: the table's rows hold that many tokens at least
+    (many rows of f16 queries go to the prompt kernel where what the table
+    holds could make a large call)."""
 
-    def __init__(self, gpu, lens, nh, nkv, hd, page, cd, qd, seed=0, gaps=0, q_size=1.5):
+    def __init__(self, gpu, lens, nh, nkv, hd, page, cd, qd, seed=0, gaps=0, q_size=1.5, wide=0):
         g = rng(seed + hd + page)
         self.gpu, self.nh, self.nkv, self.hd = gpu, nh, nkv, hd
         need = [-(-kv // page) for _, kv in lens]
         B, pages = len(lens), sum(need) + 3
         order = torch.randperm(pages, generator=g)
-        self.table = torch.full((B, max(max(need), 1) + 1), -1)
+        self.table = torch.full((B, max(max(need) + 1, 2, wide // page)), -1)
         at = 0
         for b, n in enumerate(need):
             self.table[b, :n] = order[at:at + n]
@@ -276,6 +279,62 @@ def test_attention(gpu, lens, nh, nkv, hd, page, cd, qd):
     for r0, rows, kv in b.spans:
         if kv == 0:
             assert (got[r0:r0 + rows] == 0).all()
+
+
+def as_prompt(b):
+    """Runs the batch; it took the kernel of prompts."""
+    launches()
+    got = b.run()
+    assert launches() == ["prompt_kernel", "prompt_join_kernel"]
+    return got
+
+
+@pytest.mark.parametrize("lens,nh,nkv,hd,page,cd", [
+    ([(16, 16)], 2, 1, 128, 16, F16),
+    ([(64, 200)], 4, 2, 128, 16, F16),
+    ([(100, 100)], 8, 2, 64, 32, I8),
+    ([(257, 600)], 2, 2, 128, 16, F16),
+    ([(77, 2222)], 6, 2, 128, 64, I8),
+    ([(77, 4097)], 8, 2, 128, 64, F16),
+    ([(33, 3000)], 8, 1, 256, 16, F16),
+    ([(40, 1531)], 4, 1, 64, 16, F16),
+    ([(130, 131), (3, 3), (0, 70), (70, 1000)], 6, 2, 128, 64, F16),
+    ([(90, 91), (129, 1300)], 4, 1, 256, 32, I8),
+])
+def test_attention_prompts(gpu, lens, nh, nkv, hd, page, cd):
+    b = Batch(gpu, lens, nh, nkv, hd, page, cd, F16, wide=1 << 15, gaps=1)
+    b.check(as_prompt(b), b.want())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("window", [0, 30])
+@pytest.mark.parametrize("rows,hd,cd,qd,wide", [
+    (6, 128, F16, F32, 0), (6, 256, F16, F16, 0), (6, 64, I8, F32, 0), (20, 128, F16, F16, 0),
+    (100, 128, F16, F16, 1 << 15), (70, 64, F16, F16, 1 << 15), (70, 256, F16, F16, 1 << 15), (100, 128, I8, F16, 1 << 15)])
+def test_attention_values_not_finite(gpu, value, window, rows, hd, cd, qd, wide):
+    """A value, key or scale that is not finite is in the rows that see its
+    token (a value: in its dim), and nowhere else."""
+    kv, nkv, nh, page = rows + 50, 2, 6, 16
+    for what in ("value", "key"):
+        b = Batch(gpu, [(rows, kv)], nh, nkv, hd, page, cd, qd, wide=wide)
+        p, d = kv - rows + rows // 2, 21
+        slot = (b.table[0, p // page] * page + p % page).reshape(1)
+        ki, vi, si = indices(slot, nkv, page, hd)
+        if cd is F16:
+            t, at = (b.cache.v, vi[0, 1, d]) if what == "value" else (b.cache.k, ki[0, 1, d])
+        else:
+            t, at = (b.cache.v_scale if what == "value" else b.cache.k_scale), si[0, 1]
+        t.view(-1)[at] = value
+        got, want = b.run(window=window), b.want(window=window)
+        at_row = torch.arange(rows) + kv - rows
+        see = (at_row >= p) & ((at_row < p + window) if window else True)
+        assert see.any() and not see.all()
+        bad = torch.zeros_like(want, dtype=torch.bool)
+        bad[see, nh // 2:, d if cd is F16 and what == "value" else slice(None)] = True
+        if what == "value" or math.isnan(value):  # (an infinite key: its score may be the lowest, too)
+            assert not got[bad].isfinite().any()
+        assert got[~bad].isfinite().all()
+        assert rel(got[~bad], want[~bad]) < (1e-5 if qd is F32 else 1e-3)
 
 
 @pytest.mark.parametrize("opts", [dict(cap=5.0), dict(window=1), dict(window=40), dict(window=333, cap=20.0), dict(slopes=True),
@@ -395,8 +454,6 @@ def test_attention_stream_and_repeat(gpu):
 
 
 def test_attention_uses_the_kernel(gpu):
-    from shady_thinker_amd._lib import launches
-
     b = Batch(gpu, [(1, 100)], 4, 2, 128, 16, F16, F32)
     launches()
     b.run()
