@@ -32,7 +32,9 @@
  *    holds the prefill GEMM's pre-processed A and split-K partials, the
  *    split-K partials of multi-token (M > 1) decode calls on linears with few
  *    16-column tiles, and the split f32 x of multi-token GPTQ calls with
- *    act-order; one-token decode calls use none. Calls on one context
+ *    act-order; one-token decode calls of linears use none. Attention and
+ *    log probabilities keep the partial results of their chunks there (and
+ *    cut less where it is small). Calls on one context
  *    are ordered by its stream, so they never overlap on it.
  */
 #ifndef SHADY_HIP_H

@@ -11,17 +11,22 @@
 //    rows); f32 calls take two columns for a pair, its f16 high and low part
 //    (22 bits of q, scaled by a power of two, and of each softmax weight), so
 //    that nothing but the cache itself is held in 16 bits.
-//  * A wave takes 32 keys (two tiles) at a time. The scores' lanes are the
-//    columns and each lane's eight keys are those whose values one piece of
-//    the cache's value tiles holds: the weights go from the first product to
-//    the second in the registers where they are, and K and V go from HBM to
-//    registers in 16-byte (8-byte) pieces, with no LDS.
+//  * A wave takes 32 keys (two tiles) of f16 or 64 of int8 at a time. The
+//    scores' lanes are the columns and each lane's keys are those whose values
+//    one piece of the cache's value tiles holds: the weights go from the first
+//    product to the second in the registers where they are, and K and V go
+//    from HBM to registers in 16-byte pieces, with no LDS.
 //  * Bound by HBM (4 matrix cycles per KiB of the cache are 4% of its time),
 //    that is by how many loads are in flight: the next step's are issued
-//    before this step's are used.
+//    before this step's are used. 32/8 heads of 128, f16 cache: 31 sequences
+//    of 800 to 8191 tokens 106 us (5.4 TB/s); one of 32000 28 us (4.6 TB/s);
+//    int8, one of 65000 38.5 us (3.6 TB/s, of which 3.5 us join the chunks).
+//  * A short call is its chain of latencies: 32 keys in 6.2 us, of which 0.6
+//    are the item, 1.5 until the loads are out, 0.6 until they are used, 0.3
+//    the waves' meeting, 0.5 the store (the rest is the launch).
 //  * The cut: every sequence's keys go in chunks of C steps to workgroups of
-//    four waves, C the smallest with which all fit the grid, found by each
-//    workgroup from the lengths on the device (so that a captured graph stays
+//    four waves, C the smallest with which all fit the grid (two workgroups a
+//    CU), found by each workgroup from the lengths on the device (so that a captured graph stays
 //    right, and batches of mixed lengths even, as they grow). The last chunk
 //    of a (row block, key head) to count in joins them in order: the counter
 //    protocol of the split-K kernels (see qmv_kernel.hpp on its visibility).
@@ -42,7 +47,10 @@ constexpr float kShift = 14.0f;         // weights are held times 2^14: f16 keep
 // bytes; what a step costs beside its products then counts half).
 template <bool I8>
 constexpr int kStep = I8 ? 64 : 32;
-// Steps of a chunk (a multiple of the first), steps that stay in one.
+// Steps of a chunk (a multiple of the first), steps that stay in one. A join
+// costs 3 to 3.5 us: one sequence of 1000 tokens takes 10.1 us in one chunk
+// and 9.2 with 16 steps for 32, but 16 sequences of 4000 tokens of 256 dims
+// the same within 3% either way, and a batch's short sequences then join, too.
 template <bool I8>
 constexpr int kLeast = I8 ? 4 : 8;
 template <bool I8>
@@ -166,8 +174,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
     const int tsh = a.c.tiles_shift();
     // Pages come through the scalar cache a step ahead, as they are in the
     // table and from a place that is in it; whether there is such a tile and
-    // page is asked when the step is loaded (asked at once, every step waited
-    // for its table entry: 3 us a step of a batch that no cache holds).
+    // page is asked when the step is loaded (asked at once, every step waits for
+    // its table entry: 1 us more at one sequence of 1000 tokens).
     const auto *const pages =
         (const __attribute__((address_space(4))) int32_t *)(a.table + (int64_t)it.b * a.table_stride);
     int next[2 * SUB];  // of the step to load
@@ -645,7 +653,9 @@ int launch_attn(st_context *ctx, Args a) {
 template <int HD, bool I8, bool SPLIT, bool GEN>
 int by_size(st_context *ctx, const Args &a) {
     // A cache that no more than one row block reads, and that is larger than
-    // what a cache level keeps between calls
+    // what a cache level keeps between calls: non-temporal loads (31 sequences
+    // of 8191 tokens at most 114 -> 104 us; in small caches, which the next call
+    // finds in L2 again, they cost 1.2 us of 6.2)
     const int64_t bytes = (int64_t)a.B * a.capacity * a.c.heads * HD * (I8 ? 2 : 4);
     const bool once = !a.q_start && a.group <= (SPLIT ? 8 : 16) && bytes >= (int64_t)96 << 20;
     if (once) return launch_attn<HD, I8, SPLIT, GEN, kOneNt>(ctx, a);

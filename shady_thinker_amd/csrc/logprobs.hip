@@ -11,9 +11,13 @@
 // registers; each wave has (m, S, T) of its own and they meet in LDS. The top
 // tokens: the k-th of the threads' largest logits is a lower bound of the
 // chunk's k-th largest, so only logits from there on (k and a few more) are
-// candidates; these are ranked among each other by value, then index. The last chunk of a row to count in joins the
-// chunks (the counter protocol of the split-K kernels, see qmv_kernel.hpp),
-// its top tokens found in the same way among the chunks'.
+// candidates; these are ranked among each other by value, then index. The
+// last chunk of a row to count in joins the chunks (the counter protocol of the
+// split-K kernels, see qmv_kernel.hpp), its top tokens found in the same way
+// among the chunks'.
+// 512 rows of 151936 f32, top 5: 74 us (4.2 TB/s; 57 without top tokens, 5.5
+// TB/s); one row, top 20: 12.3 us (top 1 8.7, none 5.9: a selection's three
+// barriers and ranking are 3 us, in the chunks and again in the join).
 #include "common.hpp"
 
 #include <algorithm>
