@@ -47,14 +47,16 @@ constexpr float kShift = 14.0f;         // weights are held times 2^14: f16 keep
 // bytes; what a step costs beside its products then counts half).
 template <bool I8>
 constexpr int kStep = I8 ? 64 : 32;
-// Steps of a chunk (a multiple of the first), steps that stay in one. A join
-// costs 3 to 3.5 us: one sequence of 1000 tokens takes 10.1 us in one chunk
-// and 9.2 with 16 steps for 32, but 16 sequences of 4000 tokens of 256 dims
-// the same within 3% either way, and a batch's short sequences then join, too.
+// Steps of a chunk (a multiple of the first), steps that stay in one (a join
+// costs 3 to 3.5 us). 16 steps of f16 in one chunk against 32: a sequence of
+// 1000 tokens 9.1 and 10.1 us, 16 sequences of up to 4000 of 256 dims 39 and
+// 43, batches of 128 dims the same or 3% less; with 8, one of 333 tokens takes
+// 8.5, not 6.3. At least 4 steps against 8: 1000 tokens 8.0 and 9.2, but 4
+// sequences of up to 2000 13.1 and 11.2.
 template <bool I8>
 constexpr int kLeast = I8 ? 4 : 8;
 template <bool I8>
-constexpr int kWhole = I8 ? 16 : 32;
+constexpr int kWhole = I8 ? 8 : 16;
 
 template <int HD, bool I8>
 struct Frag {
