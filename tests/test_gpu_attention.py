@@ -337,6 +337,23 @@ def test_attention_values_not_finite(gpu, value, window, rows, hd, cd, qd, wide)
         assert rel(got[~bad], want[~bad]) < (1e-5 if qd is F32 else 1e-3)
 
 
+def test_attention_values_not_finite_long_prompt(gpu):
+    """The same in a call whose row blocks fill the GPU, so without chunks: bit
+    for bit the call without, but for what sees the value."""
+    rows, nkv, nh, hd, page = 4200, 4, 16, 64, 64
+    b = Batch(gpu, [(rows, rows)], nh, nkv, hd, page, F16, F16)
+    want = as_prompt(b)
+    places = [(5, 0, 3), (2100, 2, 63), (4199, 3, 17)]  # token, key head, dim
+    bad = torch.zeros_like(want, dtype=torch.bool)
+    for p, h, d in places:
+        slot = (b.table[0, p // page] * page + p % page).reshape(1)
+        b.cache.v.view(-1)[indices(slot, nkv, page, hd)[1][0, h, d]] = -math.inf
+        bad[p:, h * nh // nkv:(h + 1) * nh // nkv, d] = True
+    got = as_prompt(b)
+    assert not got[bad].isfinite().any()
+    assert torch.equal(got[~bad], want[~bad])
+
+
 @pytest.mark.parametrize("opts", [dict(cap=5.0), dict(window=1), dict(window=40), dict(window=333, cap=20.0), dict(slopes=True),
                                   dict(slopes=True, window=64, cap=8.0), dict(gate=True), dict(scale=0.05, gate=True)])
 @pytest.mark.parametrize("lens,nh,nkv,hd,page,cd,qd", [
