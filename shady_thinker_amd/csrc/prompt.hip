@@ -394,7 +394,9 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
                 for (int g = 0; g < 4; ++g)
                     part[(8 * d + 2 * g + hf) * kPairs] = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
         }
-        if (hf == 0) reinterpret_cast<f32x2 *>(a.part_ml)[at * kPairs + mine] = f32x2{m, l};
+        // (a row whose scores here are all NaN has no maximum: -inf would say
+        // that it sees nothing of the chunk, and the join would pass it over)
+        if (hf == 0) reinterpret_cast<f32x2 *>(a.part_ml)[at * kPairs + mine] = f32x2{l != l ? 0.0f : m, l};
     }
 }
 
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
             float high = top;
 #pragma unroll
             for (int i = 0; i < N; ++i) high = fmaxf(high, i < n ? x[i][0] : -INFINITY);
-            if (high == -INFINITY) return;  // (a chunk that the row does not see holds no sums)
+            if (high == -INFINITY) return;  // (chunks that the row does not see hold no sums)
             const float was = exp2_(top - high);
             top = high, total *= was;
 #pragma unroll
