@@ -29,6 +29,7 @@ from .model import _need
 
 _F32, _F16, _I32, _I8 = torch.float32, torch.float16, torch.int32, torch.int8
 _DT = {_F32: ST_F32, _F16: ST_F16}
+_MAX_I32 = 2**31 - 1
 TILE = 16  # tokens of a cache tile
 
 
@@ -133,10 +134,15 @@ class KvCache:
 
     def slots(self, table, positions):
         """Slots (int32) of `positions` [B] or [B, n] in the sequences whose
-        pages are the rows of `table` [B, pages]; torch ops, capturable."""
+        pages are the rows of `table` [B, pages]; torch ops, capturable.
+        Positions that the table has no page for, and places of a page outside
+        the cache, get a slot outside the cache, which is not written."""
         p = positions.long()
-        page = torch.gather(table, 1, (p // self.page_size).view(table.shape[0], -1)).view(p.shape)
-        return (page * self.page_size + p % self.page_size).to(_I32)
+        i = p // self.page_size
+        held = i.clamp(0, table.shape[1] - 1)
+        page = torch.gather(table, 1, held.view(table.shape[0], -1)).view(p.shape)
+        slot = torch.add(p, page - i, alpha=self.page_size)  # (64 bits: no product comes round)
+        return torch.where(i == held, slot, -1).clamp_(-1, _MAX_I32).to(_I32)
 
 
 def qk_norm_rope_store(gpu, cache: KvCache, q, k, v, q_out, slots, positions=None, cos=None, sin=None, q_weight=None, k_weight=None,
@@ -301,10 +307,12 @@ class PagedAttention:
 
     def advance(self) -> None:
         """Every sequence gets its next place (torch ops on device tensors, so
-        a captured step can begin with it): positions = kv_len, then kv_len + 1."""
+        a captured step can begin with it): positions = kv_len, then kv_len + 1.
+        A sequence that fills its table stays as long as that: its new tokens
+        are not stored, and its row attends to those that are."""
         self.positions.copy_(self.kv_len)
         self.slots.copy_(self.cache.slots(self.table, self.positions))
-        self.kv_len += 1
+        self.kv_len.add_(1).clamp_(max=self.table.shape[1] * self.cache.page_size)
 
     def _split(self, qkv):
         w, kw = self.widths

@@ -10,8 +10,9 @@ import math
 import pytest
 import torch
 
+import shady_thinker_amd as sta
 from attn_util import attention, indices, rel
-from test_gpu_attention import F16, F32, I8, Batch, as_prompt
+from test_gpu_attention import F16, F32, I8, Batch, as_prompt, rng
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,67 @@ def test_nan_key_alone_in_a_chunk(gpu, hd, cd, window):
     assert got[see].isnan().all()
     assert got[~see].isfinite().all()
     assert rel(got[~see], want[~see]) < 1e-3
+
+
+# -------------------------------------------------- the end of a page table
+@pytest.mark.parametrize("cd", [F16, I8])
+def test_steps_past_the_table(gpu, cd):
+    """Captured steps of a batch of which one sequence after the other fills
+    its table: it attends to what is stored, and every other sequence's tokens
+    stay where they are, bit for bit."""
+    nh, nkv, hd, page, B = 4, 2, 64, 16, 3
+    dev = gpu.device
+    width = (nh + 2 * nkv) * hd
+    c = sta.KvCache(gpu, 8, page, nkv, hd, cd)
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        if t is not None:
+            t.zero_()
+    table = torch.tensor([[3, 6], [5, 0], [2, 7]], dtype=torch.int32, device=dev)
+    p = sta.PagedAttention(gpu, [c], nh, table)
+    start = torch.tensor([30, 4, 31], dtype=torch.int32)
+
+    class Rows:
+        qkv = torch.zeros(B, width, device=dev)
+        attn = torch.zeros(B, nh * hd, device=dev)
+
+    def step():
+        p.advance()
+        p.attention(0, Rows)
+
+    stream = torch.cuda.Stream(device=dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        step()  # warm-up
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    torch.cuda.current_stream(dev).wait_stream(stream)
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        if t is not None:
+            t.zero_()
+    p.kv_len.copy_(start)
+    g = rng(6)
+    every = torch.arange(page * 8, dtype=torch.int32, device=dev)
+
+    def contents():
+        ko, vo = (torch.empty(page * 8, nkv, hd, device=dev) for _ in range(2))
+        sta.kv_read(gpu, c, every, ko, vo)
+        return ko.cpu().double(), vo.cpu().double()
+
+    places = [(table[b].cpu()[torch.arange(32) // page] * page + torch.arange(32) % page).long() for b in range(B)]
+    lens, were = start.tolist(), contents()
+    for i in range(6):
+        x = torch.randn(B, width, generator=g)
+        Rows.qkv.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        now = contents()
+        touched = [int(places[b][n]) for b, n in enumerate(lens) if n < 32]
+        rest = torch.ones(page * 8, dtype=torch.bool)
+        rest[touched] = False
+        assert all(torch.equal(a[rest], z[rest]) for a, z in zip(were, now))
+        lens, were = [min(n + 1, 32) for n in lens], now
+        assert p.kv_len.tolist() == lens
+        want = attention(x[:, :nh * hd].view(B, nh, hd), lambda b: now[0][places[b][:lens[b]]], lambda b: now[1][places[b][:lens[b]]],
+                         [(b, 1, lens[b]) for b in range(B)], 1 / math.sqrt(hd))
+        assert rel(Rows.attn.view(B, nh, hd), want) < 1e-5
