@@ -92,7 +92,6 @@ def decode(gpu, stack, embedding, prompts, tokens, cache_dtype=torch.float16, gr
     h = Hooks(gpu, embedding, table.to(gpu.device, torch.int32), cache_dtype)
     b = stack.buffers(gpu, B)
     run = stack.capture(gpu, b, h) if graph else None
-    h.kv_len.zero_()  # (the capture's warm-up stored a token)
     ids, lps = [], []
     for i in range(n + tokens - 1):
         h.tokens.copy_(prompts[:, i] if i < n else h.top[:, 0])

@@ -19,6 +19,7 @@ Errors raise ValueError / TypeError (arguments) or ShadyHipError (a call).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -283,7 +284,8 @@ class PagedAttention:
     """The self-attention of a model's layers over paged caches: a
     DecoderStack's `attention` hook for one token of each of B sequences
     (captured in the stack's graph, with `advance` before it), and `prefill`
-    for prompts beside DecoderLinears.prefill.
+    for prompts beside DecoderLinears.prefill. Capturing is not a step: the
+    lengths and the caches stay as they are (`warm_up`).
 
     caches: one KvCache per layer (None for layers of another kind). table
     [B, pages] int32, each sequence's pages, the caller's to fill before they
@@ -301,7 +303,9 @@ class PagedAttention:
         self.gated, self.options, self.cache = gated, attention, c
         B = table.shape[0]
         mk = lambda: torch.zeros(B, dtype=_I32, device=gpu.device)
-        self.kv_len, self.positions, self.slots = mk(), mk(), mk()
+        self.kv_len, self.positions = mk(), mk()
+        self.slots, self._nowhere = mk().fill_(-1), mk().fill_(-1)
+        self._stores = True
         self.q = torch.empty(B, n_heads * c.head_dim, device=gpu.device)
         self.widths = (n_heads * c.head_dim * (2 if gated else 1), c.n_kv_heads * c.head_dim)
 
@@ -313,6 +317,18 @@ class PagedAttention:
         self.positions.copy_(self.kv_len)
         self.slots.copy_(self.cache.slots(self.table, self.positions))
         self.kv_len.add_(1).clamp_(max=self.table.shape[1] * self.cache.page_size)
+
+    @contextlib.contextmanager
+    def warm_up(self):
+        """DecoderStack hook, around the eager step before a capture: it stores
+        no token (its place may not be the sequence's yet), and the lengths
+        are afterwards what they were."""
+        kept, self._stores = self.kv_len.clone(), False
+        try:
+            yield
+        finally:
+            self._stores = True
+            self.kv_len.copy_(kept)
 
     def _split(self, qkv):
         w, kw = self.widths
@@ -329,7 +345,7 @@ class PagedAttention:
     def attention(self, i, b) -> None:
         """DecoderStack hook: b.qkv [B, q|k|v] -> b.attn [B, heads * head_dim]."""
         if self.caches[i] is not None:
-            self._run(i, b.qkv, self.q, b.attn, self.slots, self.positions, self.table, self.kv_len, None)
+            self._run(i, b.qkv, self.q, b.attn, self.slots if self._stores else self._nowhere, self.positions, self.table, self.kv_len, None)
 
     def prefill(self, i, qkv, out, q_start, positions, slots, kv_len, table=None) -> None:
         """Layer i's attention of prompts: qkv [T, q|k|v] (the output of the

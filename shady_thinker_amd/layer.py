@@ -39,6 +39,8 @@ between them.
 """
 from __future__ import annotations
 
+import contextlib
+
 from . import model as M
 from ._lib import call
 from .weights import GptqWeight
@@ -301,6 +303,9 @@ class DecoderStack:
                             layer the core's output from its qkv channels)
       post_attention(i, b)  b.o (+ residual) -> b.xm
       final(b)              b.down (+ residual) -> b.x, the lm_head's input
+      warm_up()             (by `capture` alone) a context around the eager
+                            step that it runs before it records one: hooks
+                            that keep a state put it back
     Without hooks the projections run on the buffers as they are (the
     benchmark's synthetic activations); gate/up then reads b.xm and the
     lm_head b.x."""
@@ -380,7 +385,8 @@ class DecoderStack:
         stream = torch.cuda.Stream(device=gpu.device)
         stream.wait_stream(torch.cuda.current_stream(gpu.device))
         with torch.cuda.stream(stream):
-            self.step(gpu, b, hooks)  # warm-up: first-call set-up happens outside the capture
+            with getattr(hooks, "warm_up", contextlib.nullcontext)():
+                self.step(gpu, b, hooks)  # warm-up: first-call set-up happens outside the capture
         torch.cuda.current_stream(gpu.device).wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.stream(stream):
