@@ -466,10 +466,12 @@ __global__ __launch_bounds__(kJoin * kPairs) void prompt_join_kernel(Args a) {
             if (!real || (sum[0] == 0.0f && sum[1] == 0.0f && sum[2] == 0.0f && sum[3] == 0.0f)) continue;
             const int row = it.s.q0 + tok;
             const f32x4 v = gated(a, sum, row, head, 4 * d);
+            // (added to what is there: that may be a NaN, or infinite by a value
+            // that every row of its block sees)
+            _Float16 *const to = static_cast<_Float16 *>(a.out) + ((int64_t)row * a.n_heads + head) * HD + 4 * d;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (sum[i] != 0.0f)
-                    static_cast<_Float16 *>(a.out)[((int64_t)row * a.n_heads + head) * HD + 4 * d + i] = (_Float16)v[i];
+                if (sum[i] != 0.0f) to[i] = (_Float16)((float)to[i] + v[i]);
         }
         return;
     }

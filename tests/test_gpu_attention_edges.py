@@ -119,3 +119,33 @@ def test_steps_past_the_table(gpu, cd):
         want = attention(x[:, :nh * hd].view(B, nh, hd), lambda b: now[0][places[b][:lens[b]]], lambda b: now[1][places[b][:lens[b]]],
                          [(b, 1, lens[b]) for b in range(B)], 1 / math.sqrt(hd))
         assert rel(Rows.attn.view(B, nh, hd), want) < 1e-5
+
+
+# ---------------------------------------- several things that are not finite
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,kv,hd,qd,wide", [
+    (100, 500, 128, F16, 1 << 15), (100, 4000, 128, F16, 1 << 15), (70, 400, 256, F16, 1 << 15), (300, 3000, 64, F16, 1 << 15),
+    (6, 400, 128, F16, 0), (20, 3000, 256, F16, 0)])
+def test_infinite_values_of_both_signs(gpu, rows, kv, hd, qd, wide, gated):
+    """+inf, which every row sees, and -inf in the same dim, which some see:
+    theirs is NaN. A NaN query's row stays NaN where it sees an infinity."""
+    nh, nkv, d = 6, 2, 21
+    b = Batch(gpu, [(rows, kv)], nh, nkv, hd, 16, F16, qd, wide=wide)
+    p = kv - rows + rows // 2
+    v = b.cache.v.view(-1)
+    for at, value, dim in ((10, math.inf, d), (p, -math.inf, d), (p, math.inf, d + 1)):
+        v[indices(slot_of(b, at), nkv, 16, hd)[1][0, 1, dim]] = value
+    nan_row = rows - 2
+    b.q[nan_row, nh - 1, 3] = math.nan
+    gate = torch.randn(rows, nh, hd, generator=rng(2)).to(qd) if gated else None
+    got, want = b.run(gate=gate), b.want(gate=gate)
+    see = torch.arange(rows) + kv - rows >= p
+    special = torch.zeros_like(want, dtype=torch.bool)
+    special[:, nh // 2:, d] = True
+    special[see, nh // 2:, d + 1] = True
+    special[nan_row, nh - 1] = True
+    other = slice(nh // 2, nh - 1)
+    assert (got[~see, other, d] == math.inf).all() and got[see, other, d].isnan().all()
+    assert (got[see, other, d + 1] == math.inf).all()
+    assert got[nan_row, nh - 1].isnan().all()
+    assert rel(got[~special], want[~special]) < (1e-5 if qd is F32 else 1e-3)
