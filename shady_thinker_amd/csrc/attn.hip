@@ -487,12 +487,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // (an infinite value times a weight's low part, which may be
-                // negative or 0, is not what the high part's infinity is)
-                const float low_part = half_turn(o[d][i]);
-                o[d][i] += fabsf(o[d][i]) == INFINITY ? 0.0f : low_part;
-            }
+            for (int i = 0; i < 4; ++i) o[d][i] += half_turn(o[d][i]);
     }
     if (col < PB) {
 #pragma unroll

@@ -125,7 +125,7 @@ def test_steps_past_the_table(gpu, cd):
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("rows,kv,hd,qd,wide", [
     (100, 500, 128, F16, 1 << 15), (100, 4000, 128, F16, 1 << 15), (70, 400, 256, F16, 1 << 15), (300, 3000, 64, F16, 1 << 15),
-    (6, 400, 128, F16, 0), (20, 3000, 256, F16, 0), (6, 400, 128, F32, 0), (1, 400, 64, F32, 0), (5, 3000, 256, F32, 0)])
+    (6, 400, 128, F16, 0), (20, 3000, 256, F16, 0)])
 def test_infinite_values_of_both_signs(gpu, rows, kv, hd, qd, wide, gated):
     """+inf, which every row sees, and -inf in the same dim, which some see:
     theirs is NaN. A NaN query's row stays NaN where it sees an infinity."""
