@@ -41,7 +41,7 @@ using namespace st::attn;
 
 constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit buffer data (gfx9-class)
 constexpr int kCoherent = 1 | 16;       // sc0 sc1: write through / read past this XCD's L2
-constexpr float kShift = 14.0f;         // weights are held times 2^14: f16 keeps them normal down to 2^-28
+constexpr float kShift = 14.0f;         // f16 caches: weights are held times 2^14, f16 keeps them normal down to 2^-28
 
 // Keys of a step of one wave: 32 (two tiles) of f16, 64 of int8 (the same
 // bytes; what a step costs beside its products then counts half).
@@ -224,8 +224,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
             for (int d = 0; d < (I8 ? ND / 2 : ND); ++d) f.v[u][d] = fetch16<NTL>(vp + (I8 ? 256 : 128) * d);
         }
         if constexpr (I8) {
-            int p = next[0];
-            p = q4 == 1 ? next[1] : p, p = q4 == 2 ? next[2] : p, p = q4 == 3 ? next[3] : p;
+            // (as an array the pages go through scratch memory, every step)
+            int p = next[0], n1 = next[1], n2 = next[2], n3 = next[3];
+            asm("" : "+s"(n1), "+s"(n2), "+s"(n3));
+            p = q4 == 1 ? n1 : p, p = q4 == 2 ? n2 : p, p = q4 == 3 ? n3 : p;
             const int t = tile0 + 4 * step + q4;
             const bool there = in && page_of(t, p) >= 0;
             const int64_t at = there ? a.c.scale(p, h, ((t * 16) & ((1 << a.c.page_shift) - 1)) + col) : 0;
@@ -238,7 +240,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
-    int ve = -126;  // int8: weights are held times their value scale over 2^ve
+    // int8. (256 dims: in LDS between steps, as the registers are all taken: 16
+    // sequences of up to 4000 take 33.7 us, capped 38.5, and in registers 34.9
+    // and 43.3; six of 5 drafted rows 38.1 in registers, 39.8 in LDS)
+    Held held{0.0f, 0};
+    constexpr bool kApart = I8 && !kTwo<HD> && (ONE || GEN);
+    __shared__ Held apart[kApart ? NT : 1];
+    if constexpr (kApart) apart[tid] = held;
     unsigned odd = 0;  // values that were not finite and not seen by every row
 
     auto compute = [&](F &f, int step) __attribute__((always_inline)) {
@@ -248,24 +256,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
         auto key = [&](int j) { return kl + (j & 3) + 8 * (j >> 2 & 1) + 32 * (j >> 3); };
         auto there = [&](int j) { return (f.ok >> (2 * (j >> 3) + (q4 >> 1)) & 1) != 0; };
         float x[8 * SUB];
-        float alpha = 1.0f;
+        float alpha;
         if constexpr (I8) {
-            // Scales go by LDS to the lanes that have their keys; those of
-            // values over 2^ve (kept as large as any so far needs it; scales
-            // that no row of the block sees may be anything).
-            const int k = kb + lane;
-            const bool any = (f.ok >> q4 & 1) && k <= pmax && k >= wmin;
-            const float vs = any ? f.vs : 0.0f;
-            // (one that is not finite makes its rows NaN by itself; in `top` it
-            // would drown the rows that do not see it)
-            float top = vs < INFINITY ? vs : 0.0f;
-            top = fmaxf(top, dpp<0x121>(top)), top = fmaxf(top, dpp<0x122>(top));
-            top = fmaxf(top, dpp<0x124>(top)), top = fmaxf(top, dpp<0x128>(top));
-            top = max_q4(top);
-            const int e = max(ve, uniform((int)((__float_as_uint(top) >> 23) & 255)) - 126);  // top / 2^e < 1
-            alpha = ldexpf(1.0f, ve - e);
-            ve = e;
-            scales[wave][0][lane] = f.ks, scales[wave][1][lane] = ldexpf(vs, -ve);
+            // Scales go by LDS to the lanes that have their keys.
+            scales[wave][0][lane] = f.ks, scales[wave][1][lane] = f.vs;
         }
         auto scale_of = [&](int which, int t) {  // of x[4 t] .. x[4 t + 3]
             return *reinterpret_cast<const f32x4 *>(&scales[wave][which][32 * (t >> 1) + 16 * (q4 >> 1) + 4 * (q4 & 1) + 8 * (t & 1)]);
@@ -348,12 +342,12 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
         const float mn = fmaxf(m, max_q4(mx));
         const float base = mn == -INFINITY ? 0.0f : mn;
         const float grown = exp2_(m - base);  // (0 before the first visible key)
-        alpha *= grown;
+        alpha = grown;
         m = mn;
         float p[8 * SUB], sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8 * SUB; ++j) {
-            p[j] = exp2_(x[j] - (base - kShift));
+            p[j] = exp2_(x[j] - (I8 ? base : base - kShift));
             sum += p[j];
         }
         l = fmaf(l, grown, sum);
@@ -364,10 +358,20 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[4 * t + i] *= vs[i];
             }
-            if (!full) {  // (a scale that another row sees may be a NaN)
+            if (!full) {  // (a scale that the row does not see may be anything)
 #pragma unroll
                 for (int j = 0; j < 8 * SUB; ++j) p[j] = seen >> j & 1 ? p[j] : 0.0f;
             }
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8 * SUB; ++j) top = fmaxf(top, fabsf(p[j]));
+            volatile Held *const mine = &apart[kApart ? tid : 0];
+            if constexpr (kApart) held.top = mine->top, held.e = mine->e;
+            alpha = held.next(max_q4(top), grown);
+            if constexpr (kApart) mine->top = held.top, mine->e = held.e;
+            const float down = held.down();
+#pragma unroll
+            for (int j = 0; j < 8 * SUB; ++j) p[j] *= down;
         }
         if (__ballot(alpha != 1.0f)) {
 #pragma unroll
@@ -481,7 +485,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void attn_kernel(Args a) {
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] = ldexpf(o[d][i], ve);
+            for (int i = 0; i < 4; ++i) o[d][i] = ldexpf(o[d][i], held.e);
     }
     if constexpr (SPLIT) {
 #pragma unroll

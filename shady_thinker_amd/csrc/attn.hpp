@@ -215,6 +215,29 @@ __device__ __forceinline__ unsigned not_finite(half8 v) {
     return not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
 }
 
+// int8 caches: how a row's weights, softmax weight times value scale, are held
+// in f16: over 2^e, with e such that the largest so far (`top`, in units of the
+// row's present maximum) is held between 2^3 and 2^15. Value scales may be of
+// any proportion to each other: what counts is a weight's proportion to the
+// row's largest, and only tokens that the row sees count. (e by the largest
+// scale that any row of the block sees, and never lower again: a later token
+// with values 2^20 times as large cost the rows before it 17% of their result.)
+struct Held {
+    float top;
+    int e;
+
+    // The next tile's largest weight; the maximum has grown, so that earlier
+    // weights count `grown` times what they did. Returns what the sums so far,
+    // held as before, have to be multiplied by.
+    __device__ __forceinline__ float next(float largest, float grown) {
+        top = fmaxf(top * grown, largest);
+        const int t = (int)(__float_as_uint(top) >> 23) - 126, was = e;  // top < 2^t (0, an infinity: -126, 129)
+        if (top > 0.0f && (unsigned)(t - e - 4) > 11u) e = max(t - 11, -126);
+        return was == e ? grown : ldexpf(grown, was - e);
+    }
+    __device__ __forceinline__ float down() const { return ldexpf(1.0f, -e); }
+};
+
 // Where the output's eight or four values go: times sigmoid(gate) where there
 // is one.
 __device__ __forceinline__ f32x4 gated(const Args &a, f32x4 o, int row, int head, int d) {

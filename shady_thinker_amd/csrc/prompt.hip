@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
             const int64_t at = ok ? a.c.scale(mine, h, (ct * 16) & ((1 << a.c.page_shift) - 1)) : 0;
             const float *const from = ((lane & 16) ? a.c.v_scale : a.c.k_scale) + at;
             sc = from[lane & 15];
-            sc = ok ? sc : 0.0f;
+            sc = ok ? (lane & 16) ? ldexpf(sc, -8) : sc : 0.0f;
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // m in powers of two; l: this lane's half of the sum
-    int ve = -126;                  // int8: weights are held times their value scale over 2^ve
+    Held held{0.0f, 0};             // int8
     const float c1 = GEN ? 1.0f : a.scale * kLog2e;
 
     auto compute = [&](const _Float16 *ks, const _Float16 *vs, int stage, int t, unsigned gone) __attribute__((always_inline)) {
@@ -261,27 +261,40 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
             }
         l += sum;
         if constexpr (I8) {
-            const float mine = scales[stage][1][lane % KT];
-            // (one that is not finite makes its rows NaN by itself; in `top` it
-            // would drown the rows that do not see it)
-            float top = kb + lane % KT >= blow && kb + lane % KT <= bmax && mine < INFINITY ? mine : 0.0f;
+            // (over 2^8 in LDS, so that no weight overflows)
+            auto value_scale = [&](int n, int g) {
+                return *reinterpret_cast<const f32x4 *>(&scales[stage][1][32 * n + 8 * g + 4 * hf]);
+            };
+            if (masked) {  // (those of keys that the row does not see may be anything)
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-            const int e = max(ve, (int)((__float_as_uint(top) >> 23) & 255) - 126);  // top / 2^e < 1
-            alpha = ldexpf(alpha, ve - e);
-            ve = e;
-            const float down = ldexpf(1.0f, -e);
+                for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 f = value_scale(n, g);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[n][4 * g + i] = s[n][4 * g + i] == 0.0f ? 0.0f : s[n][4 * g + i] * f[i];
+                    }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 f = value_scale(n, g);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[n][4 * g + i] *= f[i];
+                    }
+            }
+            float top = 0.0f;
 #pragma unroll
             for (int n = 0; n < NKT; ++n)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 f = *reinterpret_cast<const f32x4 *>(&scales[stage][1][32 * n + 8 * g + 4 * hf]);
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[n][i]));
+            alpha = held.next(fmaxf(top, other_half(top)), alpha);
+            const float down = held.down();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = s[n][4 * g + i] * (f[i] * down);
-                        s[n][4 * g + i] = masked && s[n][4 * g + i] == 0.0f ? 0.0f : w;
-                    }
-                }
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[n][i] *= down;
         }
         if (__ballot(alpha != 1.0f)) {
 #pragma unroll
@@ -370,7 +383,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], ve);
+            for (int i = 0; i < 16; ++i) o[d][i] = ldexpf(o[d][i], held.e + 8);
     }
     // ---- the rows, or a chunk's sums to memory, four dims of the block's pairs
     // at a time

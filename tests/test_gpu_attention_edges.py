@@ -149,3 +149,70 @@ def test_infinite_values_of_both_signs(gpu, rows, kv, hd, qd, wide, gated):
     assert (got[see, other, d + 1] == math.inf).all()
     assert got[nan_row, nh - 1].isnan().all()
     assert rel(got[~special], want[~special]) < (1e-5 if qd is F32 else 1e-3)
+
+
+# --------------------------------------- int8: value scales of any proportion
+def held(b, seq=0):
+    """A sequence's keys and values as the int8 cache holds them, 64 bits."""
+    kv = int(b.kv_len[seq])
+    page = b.cache.page_size
+    at = torch.arange(kv)
+    ki, vi, si = indices(b.table[seq][at // page] * page + at % page, b.nkv, page, b.hd)
+    c = b.cache
+    of = lambda t, i: t.cpu().flatten()[i].double()
+    return of(c.k, ki) * of(c.k_scale, si)[..., None], of(c.v, vi) * of(c.v_scale, si)[..., None]
+
+
+def plain(b, **kw):
+    k, v = held(b)
+    return attention(b.q, lambda s: k, lambda s: v, b.spans, 1 / math.sqrt(b.hd), **kw)
+
+
+INT8 = [(100, 150, 128, F16, 1 << 15), (100, 150, 64, F16, 1 << 15), (70, 120, 256, F16, 1 << 15), (100, 3000, 128, F16, 1 << 15),
+        (6, 100, 128, F32, 0), (6, 3000, 64, F32, 0), (6, 100, 256, F16, 0)]
+
+
+def each_row(got, want, tol):
+    e = [rel(got[r], want[r]) for r in range(len(want))]
+    print("largest row error", max(e))
+    assert max(e) < tol
+
+
+@pytest.mark.parametrize("ratio", [2.0**20, 2.0**45, 2.0**100])
+@pytest.mark.parametrize("rows,kv,hd,qd,wide", INT8)
+def test_value_scale_of_a_later_token(gpu, rows, kv, hd, qd, wide, ratio):
+    """A token whose values are far larger than the others' changes nothing
+    for the rows before it, in whose block it is, nor for those whose window
+    it has left."""
+    b = Batch(gpu, [(rows, kv)], 6, 2, hd, 16, I8, qd, wide=wide)
+    p = kv - rows // 2
+    si = indices(slot_of(b, p), 2, 16, hd)[2]
+    b.cache.v_scale.view(-1)[si[0]] *= ratio
+    before = torch.arange(rows) + kv - rows < p
+    tol = 1e-5 if qd is F32 else 1e-3
+    got, want = b.run(), plain(b)
+    each_row(got[before], want[before], tol)
+    if qd is F32:
+        each_row(got, want, tol)
+    got, want = b.run(window=2), plain(b, window=2)
+    out = before | (torch.arange(rows) + kv - rows >= p + 2)
+    each_row(got[out], want[out], tol)
+
+
+@pytest.mark.parametrize("ratio", [2.0**24, 2.0**30, 2.0**36])
+@pytest.mark.parametrize("rows,kv,hd,qd,wide", INT8 + [(1, 100, 128, F32, 0), (1, 4000, 128, F32, 0)])
+def test_value_scale_of_an_unlikely_token(gpu, rows, kv, hd, qd, wide, ratio):
+    """A token that every row sees, with values far larger than the others'
+    and a weight as much smaller: the others' keep their bits."""
+    nh, nkv = 6, 2
+    b = Batch(gpu, [(rows, kv)], nh, nkv, hd, 16, I8, qd, wide=wide)
+    p = 33
+    b.q[:, :, 0] = 3.0
+    ki, vi, si = indices(slot_of(b, p), nkv, 16, hd)
+    # its key: a score of about -log(ratio) from dim 0 alone
+    k = b.cache.k.view(-1)
+    k[ki[0].flatten()] = 0
+    k[ki[0, :, 0]] = -127
+    b.cache.k_scale.view(-1)[si[0]] = math.log(ratio) * math.sqrt(hd) / 3.0 / 127
+    b.cache.v_scale.view(-1)[si[0]] *= ratio
+    each_row(b.run(), plain(b), 1e-5 if qd is F32 else 1e-3)
