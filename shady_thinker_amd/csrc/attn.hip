@@ -746,7 +746,10 @@ extern "C" int st_paged_attention(st_context *ctx, const st_kv_cache *cache, con
     a.table_stride = table_stride, a.capacity = table_stride << a.c.page_shift;
     a.T = T, a.B = B, a.n_heads = n_heads, a.group = n_heads / a.c.heads;
     a.group_shift = (a.group & (a.group - 1)) == 0 ? __builtin_ctz(a.group) : -1;
-    a.window = std::min(window, 1 << 30), a.scale = scale, a.cap = cap;
+    a.window = std::min(window, 1 << 30), a.scale = scale;
+    // (a cap beyond 2^100 leaves scores as they are; one below f32's normal
+    // numbers, whose reciprocal is infinite, is as good as the least of them)
+    a.cap = cap > 0x1p100f ? 0.0f : cap > 0.0f ? std::max(cap, 0x1p-126f) : 0.0f;
     a.q_f32 = q_dtype == ST_F32, a.gate_f32 = gate_dtype == ST_F32, a.out_f32 = out_dtype == ST_F32;
     const bool i8 = cache->dtype == ST_I8, split = a.q_f32 || a.out_f32;
     if (!split && use_prompt(ctx, a)) return prompt_attention(ctx, a, i8, hd);

@@ -212,19 +212,47 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void prompt_kernel(
                 }
         }
         if constexpr (GEN) {
-            const float in = a.cap > 0.0f ? a.scale / a.cap * 2.0f * kLog2e : 0.0f, cap = a.cap * kLog2e;
+            const float in = a.cap > 0.0f ? a.scale / a.cap : 0.0f, cap = a.cap * kLog2e, per = a.scale * kLog2e;
+            // cap tanh(z) = cap (1 - 2 / (1 + e^(2 z))), z = x scale / cap: to
+            // about cap 2^-22, which up to a cap of 64 is a 30th of the weights'
+            // own rounding.
+            auto by_exp = [&](float x) __attribute__((always_inline)) {
+                return cap - 2.0f * cap * __builtin_amdgcn_rcpf(1.0f + exp2_(x * (in * 2.0f * kLog2e)));
+            };
+            // Over that, scores under a quarter of the cap by tanh's series (its
+            // next term is z^10 / 113: 2^-27).
+            auto by_series = [&](float x) __attribute__((always_inline)) {
+                const float z = x * in, t = z * z;
+                const float u = fmaf(t, fmaf(t, fmaf(t, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3);
+                return x * per * fmaf(t, u, 1.0f);
+            };
+            auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < NKT; ++n)
+                for (int n = 0; n < NKT; ++n)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = s[n][i];
-                    if (a.cap > 0.0f)  // cap tanh(x scale / cap) = cap (1 - 2 / (1 + e^(2 x scale / cap)))
-                        x = cap - 2.0f * cap * __builtin_amdgcn_rcpf(1.0f + exp2_(x * in));
-                    else
-                        x *= a.scale * kLog2e;
-                    if (a.slopes) x = fmaf(slope, (float)(key(n, i) - pos), x);
-                    s[n][i] = x;
-                }
+                    for (int i = 0; i < 16; ++i) s[n][i] = f(s[n][i]);
+            };
+            if (a.cap > 64.0f) {
+                float far = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) far = fmaxf(far, fabsf(s[n][i]));
+                if (__ballot(far * in >= 0.25f))
+                    each([&](float x) __attribute__((always_inline)) { return fabsf(x * in) < 0.25f ? by_series(x) : by_exp(x); });
+                else
+                    each(by_series);
+            } else if (a.cap > 0.0f) {
+                each(by_exp);
+            } else {
+                each([&](float x) __attribute__((always_inline)) { return x * per; });
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int n = 0; n < NKT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[n][i] = fmaf(slope, (float)(key(n, i) - pos), s[n][i]);
+            }
         }
         // (uniform) a key that some row of the wave does not see
         const bool masked = kb + KT - 1 > wmin || kb < whigh || gone;

@@ -216,3 +216,26 @@ def test_value_scale_of_an_unlikely_token(gpu, rows, kv, hd, qd, wide, ratio):
     b.cache.k_scale.view(-1)[si[0]] = math.log(ratio) * math.sqrt(hd) / 3.0 / 127
     b.cache.v_scale.view(-1)[si[0]] *= ratio
     each_row(b.run(), plain(b), 1e-5 if qd is F32 else 1e-3)
+
+
+# ------------------------------------------------------ caps of any size
+@pytest.mark.parametrize("cap", [1e-42, 1e-3, 0.7, 30.0, 1e4, 1e6, 1e12, 3e38, math.inf])
+@pytest.mark.parametrize("rows,kv,nh,hd,cd,qd,wide", [
+    (100, 300, 4, 128, F16, F16, 1 << 15), (100, 3000, 4, 128, I8, F16, 1 << 15), (70, 200, 4, 256, F16, F16, 1 << 15),
+    (70, 200, 4, 64, I8, F16, 1 << 15), (5, 300, 4, 128, F16, F32, 0), (1, 2000, 4, 64, I8, F32, 0), (9, 200, 4, 256, F16, F16, 0)])
+def test_cap_of_any_size(gpu, rows, kv, nh, hd, cd, qd, wide, cap):
+    """A cap far over the scores leaves them as they are, to f32's bits; a
+    tiny one leaves their signs; a score of 0 stays 0."""
+    b = Batch(gpu, [(rows, kv)], nh, 2, hd, 16, cd, qd, wide=wide)
+    b.q[0] = 0.0
+    want = b.want(cap=0.0 if cap == math.inf else cap)
+    each_row(b.run(cap=cap), want, 1e-5 if qd is F32 else 1e-3)
+
+
+@pytest.mark.parametrize("cd", [F16, I8])
+@pytest.mark.parametrize("q_size,cap", [(1.0, 5.0), (20.0, 5.0), (20.0, 50.0), (20.0, 200.0), (8.0, 1e5)])
+def test_capped_prompt(gpu, cd, q_size, cap):
+    """Scores far below, about and far above the cap, in one tile."""
+    b = Batch(gpu, [(100, 400)], 4, 2, 128, 16, cd, F16, q_size=q_size, wide=1 << 15)
+    b.q[::3] *= 0.02
+    each_row(b.run(cap=cap), b.want(cap=cap), 1e-3)
