@@ -44,7 +44,8 @@ def rotation(gpu, n):
 
 class Hooks(sta.PagedAttention):
     """The model's own operations around the linears; the attention hook is
-    PagedAttention's. `tokens` [B] goes in, the next ones come out in `top`."""
+    PagedAttention's. `tokens` [B] goes in; the next ones come out in `top`,
+    and in `tokens`."""
 
     def __init__(self, gpu, embedding, table, cache_dtype):
         caches = [sta.KvCache(gpu, table.numel(), 16, KV_HEADS, DIM, cache_dtype) for _ in range(LAYERS)]
@@ -77,10 +78,11 @@ class Hooks(sta.PagedAttention):
     def final(self, b):
         b.x.copy_(self.norm(self.residual + b.down))
 
-    def answer(self, b):
+    def after_logits(self, b):
         """The likeliest next token of every row, its log probability and the
-        row's entropy."""
+        row's entropy; the next step's input."""
         sta.token_logprobs(self.gpu, b.logits, entropy=self.entropy, top_ids=self.top, top_logprobs=self.logprob)
+        self.tokens.copy_(self.top[:, 0])
 
 
 def decode(gpu, stack, embedding, prompts, tokens, cache_dtype=torch.float16, graph=True):
@@ -94,9 +96,9 @@ def decode(gpu, stack, embedding, prompts, tokens, cache_dtype=torch.float16, gr
     run = stack.capture(gpu, b, h) if graph else None
     ids, lps = [], []
     for i in range(n + tokens - 1):
-        h.tokens.copy_(prompts[:, i] if i < n else h.top[:, 0])
+        if i < n:
+            h.tokens.copy_(prompts[:, i])
         run.replay() if graph else stack.step(gpu, b, h)
-        h.answer(b)
         if i >= n - 1:
             ids.append(h.top[:, 0].clone()), lps.append(h.logprob[:, 0].clone())
     if graph:

@@ -293,16 +293,18 @@ class DecoderStack:
     Between the projections a model runs its own ops (norms, attention or the
     DeltaNet core, residual adds: src/model.rs:685-690, 715-726, 758-784,
     799-802, 820-823). They are outside this path and come in as `hooks`, an
-    object with any of these methods, each called with (layer index,
-    StackBuffers) and captured into the same graph (so they must be
-    capturable stream work, e.g. torch ops on the buffers); when a hook runs,
-    b.qkv and b.attn are that layer's views:
+    object with any of these methods, called with (layer index, StackBuffers)
+    or, around the lm_head, (StackBuffers), and captured into the same graph
+    (so they must be capturable stream work, e.g. torch ops on the buffers);
+    when a hook runs, b.qkv and b.attn are that layer's views:
       pre_attention(i, b)   fill b.x (layer 0: from the embedding; later:
                             add_rmsnorm of the residual and b.down)
       attention(i, b)       b.qkv -> b.attn (self-attention; for a DeltaNet
                             layer the core's output from its qkv channels)
       post_attention(i, b)  b.o (+ residual) -> b.xm
       final(b)              b.down (+ residual) -> b.x, the lm_head's input
+      after_logits(b)       b.logits -> the answer (token_logprobs, a sampler)
+                            and, where the loop is closed, the next input
       warm_up()             (by `capture` alone) a context around the eager
                             step that it runs before it records one: hooks
                             that keep a state put it back
@@ -346,7 +348,7 @@ class DecoderStack:
     def step(self, gpu, b: StackBuffers, hooks=None) -> None:
         """One token step (all layers, then the lm_head) on b, eagerly."""
         hk = lambda name: getattr(hooks, name, None) if hooks is not None else None
-        pre, att, post, fin = hk("pre_attention"), hk("attention"), hk("post_attention"), hk("final")
+        pre, att, post, fin, after = hk("pre_attention"), hk("attention"), hk("post_attention"), hk("final"), hk("after_logits")
         m = b.batch
         for i, L in enumerate(self.layers):
             b.select(i)
@@ -376,6 +378,8 @@ class DecoderStack:
             for r0 in range(0, m, _BF16_BLOCK):
                 r1 = min(m, r0 + _BF16_BLOCK)
                 M.bf16_matvec(gpu, b.x[r0:r1], lm, b.logits[r0:r1], lm.shape[1], lm.shape[0])
+        if after:
+            after(b)
 
     def capture(self, gpu, b: StackBuffers, hooks=None) -> "StackGraph":
         """Record one token step as a HIP graph on a side stream (the calls

@@ -75,3 +75,27 @@ def test_capture_after_some_tokens(gpu, cache, outside):
         assert h.kv_len.tolist() == [i + 1] * B
         assert torch.equal(b.logits, ob.logits)
     run.release()
+
+
+def test_answers_inside_the_step(gpu):
+    """Nothing but replays after the prompt: each finds the next tokens and
+    takes them on, with their log probabilities, as the eager loop does."""
+    import decode as ex
+
+    stack, embedding = ex.build(gpu)
+    prompts = torch.arange(3 * 4, dtype=torch.int32, device=gpu.device).view(3, 4) * 37 % ex.VOCAB
+    want_ids, want_lps, _ = ex.decode(gpu, stack, embedding, prompts, 20, graph=False)
+    table = torch.arange(6, dtype=torch.int32, device=gpu.device).view(3, 2)
+    h = ex.Hooks(gpu, embedding, table, torch.float16)
+    b = stack.buffers(gpu, 3)
+    run = stack.capture(gpu, b, h)
+    for i in range(4):
+        h.tokens.copy_(prompts[:, i])
+        run.replay()
+    ids, lps = [], []
+    for i in range(20):
+        ids.append(h.top[:, 0].clone()), lps.append(h.logprob[:, 0].clone())
+        run.replay()
+        torch.cuda.synchronize()
+    run.release()
+    assert torch.equal(torch.stack(ids, 1), want_ids) and torch.equal(torch.stack(lps, 1), want_lps)
