@@ -93,7 +93,8 @@ __device__ __forceinline__ u32x2 quantise(const float (&x)[8], float &scale) {
     if (scale > 0.0f) {  // (a zero head; NaN: its scale says it)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float r = fminf(fmaxf(rintf(x[i] / scale), -127.0f), 127.0f);
+            // (an infinity over an infinite scale: 127 of its sign)
+            const float r = copysignf(fminf(fabsf(rintf(x[i] / scale)), 127.0f), x[i]);
             w[i / 4] |= ((unsigned)(int)r & 0xFFu) << (8 * (i % 4));
         }
     }
