@@ -249,7 +249,7 @@ def paged_attention(gpu, cache: KvCache, q, out, table, kv_len, q_start=None, sc
     slopes_at = _f32(slopes, "slopes", heads)
     gpu.sync_stream()
     call("st_paged_attention", gpu.handle, cache.handle, q.data_ptr(), qd, table_at, pages, len_at, start_at,
-         hd ** -0.5 if scale is None else scale, cap, window, slopes_at, gp, gd, gs, gh, out.data_ptr(), od, T, B, heads)
+         hd ** -0.5 if scale is None else scale, cap, min(window, _MAX_I32), slopes_at, gp, gd, gs, gh, out.data_ptr(), od, T, B, heads)
 
 
 def token_logprobs(gpu, logits, tokens=None, logprob=None, entropy=None, rank=None, top_ids=None, top_logprobs=None) -> None:

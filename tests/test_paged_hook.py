@@ -63,3 +63,22 @@ def test_advance_stops_at_the_table():
         assert p.kv_len.tolist() == [32, 4 + n]
         assert p.slots.tolist() == [47 if n == 0 else -1, 83 + n]
         assert p.positions.tolist() == [31 if n == 0 else 32, 3 + n]
+
+
+@pytest.mark.parametrize("window", [0, 7, 2**31 - 1, 2**31, 2**32, 2**32 + 5, 2**40])
+def test_window_of_any_size(monkeypatch, window):
+    """A window wider than 32 bits is as good as the widest of them, not what
+    its lower 32 bits say."""
+    from shady_thinker_amd import attention
+
+    class Gpu(NoGpu):
+        def sync_stream(self):
+            pass
+
+    got = []
+    monkeypatch.setattr(attention, "call", lambda name, *args: got.append(dict(zip(
+        ("gpu", "cache", "q", "q_dtype", "table", "pages", "kv_len", "q_start", "scale", "cap", "window"), args))))
+    c = sta.KvCache(G, PAGES, PAGE, NKV, HD)
+    q = torch.zeros(1, NH * HD)
+    sta.paged_attention(Gpu(), c, q, torch.empty_like(q), torch.zeros(1, 2, dtype=I32), torch.ones(1, dtype=I32), window=window)
+    assert got[0]["window"] == min(window, 2**31 - 1)
