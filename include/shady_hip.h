@@ -417,7 +417,8 @@ int st_kv_read(st_context *ctx, const st_kv_cache *cache, const int32_t *slots, 
  * kv_len[b] tokens, all of them in the cache already (so row i of n has
  * position kv_len - n + i). Replaces gqa_attention_head.wgsl:1-124,
  * gqa_reduce.wgsl:1-65 and sigmoid_mul.wgsl (src/model.rs:540-592).
- *   s_j = scale q . k_j, capped cap tanh(s_j / cap) where cap > 0, plus
+ *   s_j = scale q . k_j, capped cap tanh(s_j / cap) where cap > 0 (of any
+ *   size; past 2^100 it is none), plus
  *   slopes[head] (j - position) where slopes (f32 [n_heads]) is given;
  *   key j is visible if j <= position and, where window > 0, j > position -
  *   window; out = sum_j softmax(s)_j v_j over the visible keys (a row that
@@ -435,7 +436,10 @@ int st_kv_read(st_context *ctx, const st_kv_cache *cache, const int32_t *slots, 
  *   gate      gate_dtype, gate_stride elements between tokens,
  *             gate_head_stride between heads (the gates of the reference's
  *             gated q lie beside its queries)
- * Rows of q and out outside every sequence are left alone. f32 scores,
+ * Rows of q and out outside every sequence are left alone. What a row does
+ * not see may be anything; a NaN query, or a NaN key or scale that a row sees,
+ * makes the row and head NaN, a value that is not finite its dim infinite or
+ * NaN. f32 scores,
  * softmax and sums. With f32 q or out the products keep 22 bits of q and of
  * the softmax weights; with f16 both, the weights are rounded to f16. Chunks
  * of a long cache meet in the context workspace, in a fixed order. */

@@ -20,7 +20,18 @@
 //    that is by how many loads are in flight: the next step's are issued
 //    before this step's are used. 32/8 heads of 128, f16 cache: 31 sequences
 //    of 800 to 8191 tokens 106 us (5.4 TB/s); one of 32000 28 us (4.6 TB/s);
-//    int8, one of 65000 38.5 us (3.6 TB/s, of which 3.5 us join the chunks).
+//    int8, the same 31 72 us (4.1 TB/s), one of 65000 35 us (3.9 TB/s, of
+//    which 3.5 us join the chunks). 16 sequences of 400 to 4000 tokens, f16
+//    and int8: 8 key heads of 128 35 us (4.1 TB/s) and 31, 8 of 64 21 and 24,
+//    4 of 256 39 and 34, 32 of 128 (one query head each) 108 (5.3 TB/s) and 72.
+//    At 256 dims one step's pieces fill the registers, so loads and products
+//    take turns (and int8 spills 2 to 13 of them, f16 with a cap or slopes 3
+//    to 7; int8 with either at 128 dims 1 or 2).
+//  * f16 queries and results: the weights too are rounded to f16, one column a
+//    pair and half the products. The rounding (2.1e-4 rms of each weight,
+//    which partly averages out; their sum is of unrounded ones) is below that
+//    of the f16 result: 2.2e-4 from the 64-bit form, where results rounded once
+//    are 2.1e-4. f32 results keep 22 bits.
 //  * A short call is its chain of latencies: 32 keys in 6.2 us, of which 0.6
 //    are the item, 1.5 until the loads are out, 0.6 until they are used, 0.3
 //    the waves' meeting, 0.5 the store (the rest is the launch).
@@ -656,6 +667,12 @@ int launch_attn(st_context *ctx, Args a) {
     return st::launch_check("attn_kernel");
 }
 
+// What the host knows of the lengths is the tables' width. Where that is far
+// over them, as while a conversation is young, the next two rules take long
+// caches' forms for short ones. With tables for 32768 tokens and with tables of
+// the lengths' own width, 32/8 heads of 128, in us: one sequence of 300 tokens 6.7 and
+// 6.3, 8 of up to 1000 14.5 and 13.4, a prompt of 77 rows 13.9 and 5.6, one of
+// 300 19.5 and 17.4, 16 rows over 600 17.8 and 11.8.
 template <int HD, bool I8, bool SPLIT, bool GEN>
 int by_size(st_context *ctx, const Args &a) {
     // A cache that no more than one row block reads, and that is larger than
@@ -705,6 +722,10 @@ int plan_cut(st_context *ctx, Args &a, int pb, int hd, int step, int least, int6
     const size_t item = (size_t)heads * pb * (hd + 2) * sizeof(float);
     extra = std::min(extra, rows * (most_chunks - 1));
     extra = std::min(extra, (int64_t)(std::min<size_t>(ctx->ws_bytes, 0x7FFFFFFF) / item) - rows);
+    // (more than that are 8 workgroups a CU without a cut; but one sequence much
+    // longer than the others then is one workgroup's work in each head: 96
+    // sequences over 32 key heads of 64, one of 30000 tokens and the others of
+    // 400, take 105 us, 128 of them 211)
     a.split = extra >= 1 && rows * heads <= kSplitCounters;
     a.rows = (int)rows;
     a.G = (int)(rows + (a.split ? extra : 0));

@@ -10,7 +10,8 @@
 // so a workgroup whose 16 tokens fill a tile turns them in LDS (whole 16-byte
 // pieces, lines written by one workgroup); others go element by element.
 // 2047 tokens of 32/8 heads of 128, f16: 13.6 us (3.7 TB/s; two heads a
-// workgroup 13.8, four 15.4); one token 4.1 us, the launch. The read takes four
+// workgroup 13.8, four 15.4); one token 4.1 us, the launch (events around it; 3.2
+// in a kernel trace). The read takes four
 // heads a workgroup where there are many (16384 int8 tokens of 8 heads of 128:
 // 22.4 us, 4.5 TB/s; with one 28.5).
 #include "kvcache.hpp"

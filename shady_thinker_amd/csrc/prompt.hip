@@ -15,6 +15,20 @@
 //    the registers where they are.
 //  * The accumulators are rescaled only when a maximum has grown by 2^8
 //    (weights up to 2^8 fit f16, sums are f32).
+//  * Weights are rounded to f16 for the second product, which in f32's bits
+//    would be two (a high and a low part, as attn_kernel's for f32 results,
+//    which a caller may ask for at 10 times the time). The rounding, 2.1e-4
+//    rms of each weight, partly averages out and stays below that of the f16
+//    result: 4096 rows are 2.13e-4 from the 64-bit form, rounded once they are
+//    2.07e-4; the two are 1.5e-4 apart.
+//  * 4096 rows, f16 cache and int8, in us: 32/8 heads of 128 160-175 (0.79-0.86
+//    PFLOP/s) and 208-230, of 64 99 and 131, 16/4 of 256 245 and 303; 128 dims
+//    with a cap of 50 215-219 and 263-271, with slopes 217, with a window of
+//    512 68. Beyond the products it is the softmax: per score an exp2, and with
+//    a cap another and a reciprocal; at 64 dims there are twice as many scores
+//    a product; at 256 one wave a SIMD has nothing beside it; int8 tiles are
+//    converted again by every workgroup. (int8, 256 dims and a cap or slopes: 7 registers
+//    spilled.)
 //  * All workgroups of a key head run on one XCD where the head count allows,
 //    so a head's K and V are read from HBM once; the last rows, which see
 //    most keys, start first.

@@ -38,6 +38,21 @@ def test_nan_query(gpu, hd, cd, rows, kv):
     assert rel(got[~bad], want[~bad]) < 1e-3
 
 
+@pytest.mark.parametrize("rows,kv,hd,cd,qd", [
+    (1, 100, 128, F16, F32), (1, 4000, 128, F16, F32), (1, 9000, 256, I8, F32), (5, 4000, 64, F16, F32), (5, 4000, 128, I8, F16),
+    (3, 700, 256, F16, F16)])
+def test_nan_query_of_few_rows(gpu, rows, kv, hd, cd, qd):
+    """The same in calls of one row and of a few."""
+    b = Batch(gpu, [(rows, kv)] * 2, 4, 2, hd, 16, cd, qd)
+    r, h = rows, 3  # (the second sequence's first row)
+    b.q[r, h, 5] = math.nan
+    got, want = b.run(), b.want()
+    bad = torch.zeros(want.shape, dtype=torch.bool)
+    bad[r, h] = True
+    assert got[bad].isnan().all()
+    assert rel(got[~bad], want[~bad]) < (1e-5 if qd is F32 else 1e-3)
+
+
 @pytest.mark.parametrize("hd,cd", [(128, F16), (256, F16), (64, I8)])
 @pytest.mark.parametrize("window", [0, 40])
 def test_nan_key_alone_in_a_chunk(gpu, hd, cd, window):
