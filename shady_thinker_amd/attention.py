@@ -138,12 +138,17 @@ class KvCache:
         pages are the rows of `table` [B, pages]; torch ops, capturable.
         Positions that the table has no page for, and places of a page outside
         the cache, get a slot outside the cache, which is not written."""
+        return self._places(table, positions)[1].to(_I32)
+
+    def _places(self, table, positions):
+        """Whether the table has a page for each position; the slots, 64 bits."""
         p = positions.long()
         i = p // self.page_size
         held = i.clamp(0, table.shape[1] - 1)
         page = torch.gather(table, 1, held.view(table.shape[0], -1)).view(p.shape)
+        ok = i == held
         slot = torch.add(p, page - i, alpha=self.page_size)  # (64 bits: no product comes round)
-        return torch.where(i == held, slot, -1).clamp_(-1, _MAX_I32).to(_I32)
+        return ok, torch.where(ok, slot, -1).clamp_(-1, _MAX_I32)
 
 
 def qk_norm_rope_store(gpu, cache: KvCache, q, k, v, q_out, slots, positions=None, cos=None, sin=None, q_weight=None, k_weight=None,
@@ -315,8 +320,9 @@ class PagedAttention:
         A sequence that fills its table stays as long as that: its new tokens
         are not stored, and its row attends to those that are."""
         self.positions.copy_(self.kv_len)
-        self.slots.copy_(self.cache.slots(self.table, self.positions))
-        self.kv_len.add_(1).clamp_(max=self.table.shape[1] * self.cache.page_size)
+        ok, slots = self.cache._places(self.table, self.positions)
+        self.slots.copy_(slots)
+        self.kv_len += ok
 
     @contextlib.contextmanager
     def warm_up(self):
