@@ -20,7 +20,8 @@
 //    which a caller may ask for at 10 times the time). The rounding, 2.1e-4
 //    rms of each weight, partly averages out and stays below that of the f16
 //    result: 4096 rows are 2.13e-4 from the 64-bit form, rounded once they are
-//    2.07e-4; the two are 1.5e-4 apart.
+//    2.07e-4; the two are 1.5e-4 apart (2.7e-4 and 2.1e-4 at most in draws of
+//    all forms).
 //  * 4096 rows, f16 cache and int8, in us: 32/8 heads of 128 160-175 (0.79-0.86
 //    PFLOP/s) and 208-230, of 64 99 and 131, 16/4 of 256 245 and 303; 128 dims
 //    with a cap of 50 215-219 and 263-271, with slopes 217, with a window of
