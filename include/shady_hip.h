@@ -65,7 +65,7 @@ typedef enum { ST_F32 = 0, ST_F16 = 1, ST_BF16 = 2, ST_I8 = 3 } st_dtype;
 /* flags */
 #define ST_FLAG_ZEROS_PLUS_ONE 0x1u /* qzeros hold z - 1 (AutoGPTQ v1 files) */
 #define ST_FLAG_TILED 0x2u          /* weights in the tiled layout of st_gptq_i4_repack / st_int8_repack */
-#define ST_FLAG_NORM_PLUS_ONE 0x4u  /* st_qk_norm_rope_store: norm weights hold w - 1 (the reference's rmsnorm multiplies by 1 + w) */
+#define ST_FLAG_NORM_PLUS_ONE 0x4u  /* st_qk_norm_rope_store, st_add_rmsnorm: norm weights hold w - 1 (the reference's rmsnorm multiplies by 1 + w) */
 #define ST_FLAG_ROPE_PAIRS 0x8u     /* st_qk_norm_rope_store: rotates dims (2j, 2j + 1), not (j, j + rot / 2) */
 
 /* ------------------------------------------------------------ runtime */
@@ -348,6 +348,54 @@ int st_int8_gemm(st_context *ctx, const uint16_t *a, const int8_t *w, const floa
  * st_int8_tiled_bytes(K, N) bytes; pass ST_FLAG_TILED to st_int8_matvec. */
 size_t st_int8_tiled_bytes(int K, int N);
 int st_int8_repack(st_context *ctx, const int8_t *w, int8_t *w_tiled, int K, int N);
+
+/* ------------------------------------------ 8-bit floating point */
+
+/* e4m3 (OCP: finite, at most 448, NaN 0x7F) in blocks with float32 scales, the
+ * format of block-scaled checkpoints; no reference counterpart, as INT8.
+ *   rows    x8 [M][K] with x_scale [ceil(K / 128)][scale_stride]: token m's dims
+ *           of block b are x8 times x_scale[b][m] (a block's scales side by side
+ *           by token, scale_stride >= M of them)
+ *   weight  w [N][K] row-major with w_scale [ceil(N / 128)][ceil(K / 128)]: one
+ *           for each 128 x 128
+ * K is a multiple of 16; it and N may end inside a block. Quantising makes a
+ * block's scale max|x| / 448, at least 2^-126, and rounds x / scale to nearest,
+ * even. A block with a NaN has a NaN scale; one with an infinity an infinite
+ * scale, its infinities 448 of their sign and the rest 0. */
+
+/* r = residual + x and its RMS norm y = r / sqrt(mean(r^2) + eps) * weight
+ * (1 + weight: ST_FLAG_NORM_PLUS_ONE), to e4m3 rows (y8, y_scale), to y, or to
+ * both: replaces rmsnorm.wgsl and add_rmsnorm.wgsl (src/model.rs:685-691,
+ * 799-802, 820-823).
+ *   residual, residual_out  M rows of D of res_dtype (ST_F32 or ST_F16); the norm
+ *             is of the sum before it is rounded to it. They may be one buffer.
+ *   x         x_dtype (ST_F32 or ST_F16), or NULL, with residual_out NULL: the
+ *             norm of the residual alone
+ *   weight    f32 [D]
+ *   y         y_dtype (ST_F32 or ST_F16) or NULL; it may be x's buffer
+ *   *_stride  elements from one row to the next
+ * f32 arithmetic. D a multiple of 16, at most 32768. Pointers and strides in
+ * whole 16 bytes (y_scale: 4). */
+int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dtype, int64_t res_stride, const void *x,
+                   int x_dtype, int64_t x_stride, void *residual_out, int64_t out_stride, const float *weight,
+                   float eps, void *y, int y_dtype, int64_t y_stride, uint8_t *y8, float *y_scale,
+                   int64_t scale_stride, int M, int D, uint32_t flags);
+
+/* Rows of e4m3 of M rows a [K], or of silu(a) * b where b is given (the input
+ * of a down projection), silu(v) = v / (1 + exp(-v)); dtype ST_F32 or ST_F16,
+ * *_stride elements from one row to the next. Pointers and strides in whole 16
+ * bytes (y_scale: 4). */
+int st_fp8_quant(st_context *ctx, const void *a, const void *b, int dtype, int64_t a_stride, int64_t b_stride,
+                 uint8_t *y8, float *y_scale, int64_t scale_stride, int M, int K);
+
+/* y[m][n] = sum_b x_scale[b][m] w_scale[n / 128][b] sum_{k in b} x8[m][k] w[n][k],
+ * y [M][N] of y_dtype (ST_F32 or ST_F16), any M and N. Products are exact; sums
+ * are f32, in a fixed order. x8, w and y 16-byte aligned
+ * (scales: 4). f32 y keeps f32 sums; so does f16 y of at most 64 tokens. f16 y of
+ * more comes from the 8-bit matrix instruction, which keeps a product to 2^-13 of
+ * the largest of its eight k (rel-L2 3e-5 to 5e-5, beside 2.1e-4 of f16 itself). */
+int st_fp8_gemm(st_context *ctx, const uint8_t *x8, const float *x_scale, int64_t scale_stride, const uint8_t *w,
+                const float *w_scale, void *y, int y_dtype, int M, int K, int N);
 
 /* ----------------------------------------- key-value cache and attention */
 

@@ -96,6 +96,9 @@ _SIGNATURES = {
     "st_int8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _U32]),
     "st_int8_tiled_bytes": (_SZ, [_I, _I]),
     "st_int8_repack": (_I, [_P, _P, _P, _I, _I]),
+    "st_add_rmsnorm": (_I, [_P, _P, _I, _I64, _P, _I, _I64, _P, _I64, _P, _F, _P, _I, _I64, _P, _P, _I64, _I, _I, _U32]),
+    "st_fp8_quant": (_I, [_P, _P, _P, _I, _I64, _I64, _P, _P, _I64, _I, _I]),
+    "st_fp8_gemm": (_I, [_P, _P, _P, _I64, _P, _P, _P, _I, _I, _I, _I]),
     "st_qk_norm_rope_store": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P, _I,
                                    _I, _I, _U32]),
     "st_kv_read": (_I, [_P, _P, _P, _P, _P, _I, _I]),

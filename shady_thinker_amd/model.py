@@ -18,7 +18,7 @@ import torch
 
 from ._lib import ST_F16, ST_F32, ST_FLAG_TILED, call, lib
 from .gpu import ptr
-from .weights import GptqWeight, Int8Weight
+from .weights import Fp8Weight, GptqWeight, Int8Weight
 
 
 def _xdtype(t) -> int:
@@ -220,7 +220,8 @@ def linear(gpu, x, w, y) -> None:
     """Dispatch on the weight type: GptqWeight -> st_gptq_i4_matvec (M <= 32)
     or the prefill GEMM (M > 32: it computes on f16 activations, so f32 x is
     rounded to f16 first); Int8Weight -> st_int8_matvec (M <= 32) or
-    st_int8_gemm (M > 32, likewise on f16 activations)."""
+    st_int8_gemm (M > 32, likewise on f16 activations); Fp8Weight ->
+    st_fp8_quant of x, then st_fp8_gemm."""
     if isinstance(w, GptqWeight):
         m = _rows(x, w.K)
         if m > 32:
@@ -235,5 +236,12 @@ def linear(gpu, x, w, y) -> None:
             int8_gemm(gpu, xa, w.w, w.scale, y, w.K, w.N, w.flags)
         else:
             int8_matvec(gpu, x, w.w, w.scale, y, w.K, w.N, w.flags)
+    elif isinstance(w, Fp8Weight):
+        from .fp8 import Fp8Rows, fp8_gemm, fp8_quant
+
+        m = _rows(x, w.K)
+        rows = Fp8Rows(gpu, m, w.K)
+        fp8_quant(gpu, x.view(m, w.K), rows)
+        fp8_gemm(gpu, rows, w, y)
     else:
         raise TypeError(type(w))

@@ -5,7 +5,8 @@ on the device in the reference layout (qweight u32[K/8, N], scales f16[G, N])
 plus what the reference drops at load (src/weights.rs:372-374): qzeros and
 g_idx. An act-order g_idx is resolved at upload by st_gptq_i4_act_order
 (rows sorted by group, values unchanged). Int8Weight is the INT8
-per-channel format (no reference counterpart).
+per-channel format, Fp8Weight the 8-bit floating point one of block-scaled
+checkpoints (no reference counterparts).
 """
 from __future__ import annotations
 
@@ -223,6 +224,66 @@ class Int8Weight:
             call("st_int8_repack", gpu.handle, d_w.data_ptr(), d_t.data_ptr(), K, N)
             d_w, flags = d_t, ST_FLAG_TILED
         return cls(d_w, gpu.upload_array(np.ascontiguousarray(scale, dtype=np.float32), torch.float32), K, N, flags)
+
+    @property
+    def nbytes(self) -> int:
+        return self.w.numel() + self.scale.numel() * 4
+
+
+FP8_BLOCK = 128  # rows and columns of a weight, dims of a row, under one scale
+
+
+def fp8_blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+@dataclass
+class Fp8Weight:
+    """e4m3 weight of a block-scaled checkpoint: w float8_e4m3fn [N, K]
+    row-major, scale f32 [ceil(N / 128), ceil(K / 128)] (what such files call
+    weight_scale_inv): the weight's value is w times its block's scale."""
+
+    w: object
+    scale: object
+    K: int
+    N: int
+
+    @classmethod
+    def of(cls, w, scale) -> "Fp8Weight":
+        """A weight over the caller's device tensors."""
+        torch = _torch()
+        if w.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
+            raise TypeError(f"Fp8Weight: w {w.dtype} (need float8_e4m3fn), scale {scale.dtype} (need float32)")
+        if w.dim() != 2 or not w.is_contiguous() or w.numel() == 0 or w.shape[1] % 16:
+            raise ValueError(f"Fp8Weight: w {tuple(w.shape)} (need contiguous [N, K], K a multiple of 16)")
+        N, K = w.shape
+        need = (fp8_blocks(N), fp8_blocks(K))
+        if tuple(scale.shape) != need or not scale.is_contiguous() or scale.device != w.device:
+            raise ValueError(f"Fp8Weight: scale {tuple(scale.shape)} on {scale.device} (need contiguous {need} on {w.device})")
+        return cls(w, scale, K, N)
+
+    @classmethod
+    def upload(cls, gpu, w, scale) -> "Fp8Weight":
+        """Checkpoint tensors (torch, any device; scale float32 or bfloat16,
+        as files hold it)."""
+        torch = _torch()
+        if scale.dtype is torch.bfloat16:
+            scale = scale.float()
+        return cls.of(w.to(gpu.device).contiguous(), scale.to(gpu.device).contiguous())
+
+    @classmethod
+    def cat(cls, parts: list) -> "Fp8Weight":
+        """Linears that share their input (q / k / v, gate / up) as one along
+        N: one launch, outputs side by side. Every part but the last has whole
+        blocks of 128 rows."""
+        torch = _torch()
+        if any(p.K != parts[0].K for p in parts):
+            raise ValueError("Fp8Weight.cat: parts differ in K")
+        for p in parts[:-1]:
+            if p.N % FP8_BLOCK:
+                raise ValueError(f"Fp8Weight.cat: N={p.N} not a multiple of {FP8_BLOCK} before the last part")
+        w = torch.cat([p.w.view(torch.uint8) for p in parts]).view(torch.float8_e4m3fn)
+        return cls(w, torch.cat([p.scale for p in parts]), parts[0].K, sum(p.N for p in parts))
 
     @property
     def nbytes(self) -> int:
