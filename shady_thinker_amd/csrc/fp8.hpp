@@ -60,13 +60,23 @@ __device__ __forceinline__ void store8(void *p, int64_t at, const float (&x)[8])
     }
 }
 
-// Largest of 16 lanes side by side (a row of the DPP): v_max_u32 with the
-// row turned by 8, 4, 2 and 1 lanes.
+// Over 16 lanes side by side (a row of the DPP), the row turned by 8, 4, 2 and
+// 1 lanes: every lane gets the largest, or the sum (each lane's in an order of
+// its own: one lane's is taken).
+template <int N>
+__device__ __forceinline__ unsigned turned(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x120 + N, 0xF, 0xF, false);
+}
 template <int N>
 __device__ __forceinline__ unsigned max_turned(unsigned v) {
-    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x120 + N, 0xF, 0xF, false);
+    const unsigned o = turned<N>(v);
     return v > o ? v : o;
 }
+template <int N>
+__device__ __forceinline__ float add_turned(float v) {
+    return v + __uint_as_float(turned<N>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float row_sum(float v) { return add_turned<1>(add_turned<2>(add_turned<4>(add_turned<8>(v)))); }
 
 // The scale of a block whose 128 values lie in 16 lanes side by side, eight in
 // each: max |x| / 448, at least 2^-126. Magnitudes compare as their bits do,

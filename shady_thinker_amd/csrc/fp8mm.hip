@@ -2,21 +2,31 @@
 // blocks of the weight and of each token's 128 dims (st_fp8_gemm; no reference
 // counterpart, as INT8):
 //   y[m][n] = sum_b sx[b][m] sw[n / 128][b] sum_{k in b} x[m][k] w[n][k]
-// Two ways to sum a block's 128 products:
+// Up to 32 tokens: fp8mv.hip; up to 64 whichever is estimated faster. Here,
+// two ways to sum a block's 128 products:
 //  * v_mfma_f32_16x16x128_f8f6f4 takes the block whole. In each eight k it keeps
 //    a product to 2^-13 of the largest one's power of two (measured: a product
 //    of 2^-14 beside one of 1 is lost, in another eight it counts to 2^-23), so
 //    the sum is off by some 2^-15 of its magnitude: for f16 y, whose own
-//    rounding is 2^-12 at the mean.
-//  * f32 y: e4m3 is exact in f16, and so are the products of
-//    v_mfma_f32_16x16x32_f16 in its f32 sums. Half the rate; also for few
-//    tokens, where the weight's bytes bound the call.
-// One FMA with the block's factor adds its sum to the accumulator. The weight
-// is the A operand, so that a lane holds four neighbouring n of one token,
-// whose factor is then one register.
-#include "fp8.hpp"
+//    rounding is 2^-12 at the mean, of more than 64 tokens.
+//  * otherwise e4m3 goes to f16, exactly, and the products of
+//    v_mfma_f32_16x16x32_f16 are exact in its f32 sums. Half the rate.
+// One FMA with the block's factor adds its sum to the accumulator: 4 FMAs beside
+// an instruction of 32 cycles, which fit under it (without them 8192^3 runs
+// 454 -> 425 us). The weight is the A operand, so that a lane holds four
+// neighbouring n of one token, whose factor is then one register.
+//
+// Both kernels keep a block of both operands in LDS, brought by DMA while the
+// ones before it are multiplied. A row's 128 bytes are eight 16-byte chunks,
+// chunk j of row r at j ^ (r % 8), so that fragment reads hit every bank once.
+// Within a block the order is written out (sched_barrier): an instruction, the
+// FMAs of the one D before, now and then a DMA (all at once the waves queue for
+// the address unit: 16 cycles each). The next block's first fragments are read
+// before this one's last instructions.
+#include "fp8mm.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 #include "xcd.hpp"
 
@@ -24,228 +34,390 @@ namespace {
 
 using namespace st::f8;
 
-constexpr int kRsrcWord3 = 0x00020000;  // raw 32-bit data
-constexpr int kOutside = 0x7FFFFFF0;    // an offset past every resource: the load gives zeros
+constexpr int D = 3;      // instructions between one and its FMAs
+constexpr int kPanel = 6; // tiles along the tokens that run side by side: an XCD's 32 CUs then
+                          // share 6 strips of x and 5 of w in its L2 (4096 x 4096 x 22016: all 16 409 us, 8 390, 6 367, 4 384)
 
-struct MmArgs {
-    const uint8_t *x, *w;
-    const float *sx, *sw;
-    void *y;
-    int64_t sx_stride;
-    int M, K, N;
+struct Place {
+    int m0, n0, split;
 };
-
-// A lane's 32 elements of a fragment (16 rows x 128 k), as the matrix
-// instruction takes them.
-template <bool EXACT>
-struct Frag;
-template <>
-struct Frag<false> {
-    i32x8 v;
-    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-};
-template <>
-struct Frag<true> {
-    half8 v[4];
-    static __device__ __forceinline__ half8 eight(int lo, int hi) {
-        const half2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-        const half2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-        return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-    }
-    __device__ __forceinline__ void set(i32x4 a, i32x4 b) {
-        v[0] = eight(a.x, a.y), v[1] = eight(a.z, a.w), v[2] = eight(b.x, b.y), v[3] = eight(b.z, b.w);
-    }
-};
-__device__ __forceinline__ f32x4 mfma(const Frag<false> &a, const Frag<false> &b) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma(const Frag<true> &a, const Frag<true> &b) {
-    f32x4 p = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[j], b.v[j], p, 0, 0, 0);
-    return p;
-}
-
-// Four neighbouring n of token m.
-template <bool F32>
-__device__ __forceinline__ void store_n4(void *y, int m, int n, int N, f32x4 v) {
-    const int64_t at = (int64_t)m * N + n;
-    if (n + 4 <= N && (N & 3) == 0) {
-        if constexpr (F32)
-            *reinterpret_cast<f32x4 *>(static_cast<float *>(y) + at) = v;
-        else
-            *reinterpret_cast<half4 *>(static_cast<_Float16 *>(y) + at) = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (n + i < N) {
-            if constexpr (F32)
-                static_cast<float *>(y)[at + i] = v[i];
-            else
-                static_cast<_Float16 *>(y)[at + i] = (_Float16)v[i];
-        }
-}
-
-// Up to 16 MT tokens: a workgroup takes 16 columns, its waves every W-th block
-// of k; operands go from memory to registers. A lane's fragment is 16-byte
-// chunks c and c + 4 of a row's 128 bytes (c = lane / 16): which k that is does
-// not matter, it is the same for both operands.
-template <int MT, int W, bool F32>
-__global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
-    __shared__ f32x4 part[W][MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, c = lane >> 4;
-    const int n0 = blockIdx.x * 16;
-    const int KB = (a.K + kBlock - 1) / kBlock;
-    const __amdgpu_buffer_rsrc_t rw =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + (int64_t)n0 * a.K), (short)0, min(16, a.N - n0) * a.K, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void *)a.x, (short)0, a.M * a.K, kRsrcWord3);
-    const float *const sw = a.sw + (int64_t)(n0 / kBlock) * KB;
-    f32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0, 0, 0, 0};
-    for (int b = wave; b < KB; b += W) {
-        const int k0 = b * kBlock + c * 16;
-        const bool in0 = k0 < a.K, in1 = k0 + 64 < a.K;  // (K ends inside the last block)
-        const i32x4 w0 = __builtin_amdgcn_raw_buffer_load_b128(rw, in0 ? r * a.K + k0 : kOutside, 0, 0);
-        const i32x4 w1 = __builtin_amdgcn_raw_buffer_load_b128(rw, in1 ? r * a.K + k0 + 64 : kOutside, 0, 0);
-        const float s = sw[b];
-        Frag<true> w;
-        w.set(w0, w1);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int at = (16 * t + r) * a.K + k0;
-            const i32x4 x0 = __builtin_amdgcn_raw_buffer_load_b128(rx, in0 ? at : kOutside, 0, 0);
-            const i32x4 x1 = __builtin_amdgcn_raw_buffer_load_b128(rx, in1 ? at + 64 : kOutside, 0, 0);
-            const float f = a.sx[b * a.sx_stride + min(16 * t + r, a.M - 1)] * s;
-            Frag<true> x;
-            x.set(x0, x1);
-            acc[t] += mfma(w, x) * f;
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 64; i += 64 * W) {
-        const int t = i >> 6, l = i & 63;
-        f32x4 v = part[0][t][l];
-#pragma unroll
-        for (int w = 1; w < W; ++w) v += part[w][t][l];
-        const int m = 16 * t + (l & 15);
-        if (m < a.M) store_n4<F32>(a.y, m, n0 + 4 * (l >> 4), a.N, v);
-    }
-}
-
-// 16 bytes for each lane from a resource to LDS, at `lds` + 16 lane.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t *lds, int voff, int soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, voff, soff, 0, 0);
-}
-
-// Many tokens: a workgroup takes BM tokens x BN columns, its WM x WN waves
-// equal parts of them. A block of 128 k of both operands is in LDS while the
-// next one's comes by DMA; a row's 128 bytes are eight 16-byte chunks, chunk j
-// of row r at j ^ (r % 8), so that fragment reads hit every bank once.
-template <int BM, int BN, int WM, int WN, bool F32>
-__global__ __launch_bounds__(64 * WM * WN) void mm_kernel(MmArgs a) {
-    constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
-    constexpr int DX = BM / 8 / W, DW = BN / 8 / W;  // DMAs (8 rows) of a wave
-    static_assert(DX * 8 * W == BM && DW * 8 * W == BN, "whole DMAs a wave");
-    __shared__ __align__(1024) uint8_t s0[(BM + BN) * kBlock], s1[(BM + BN) * kBlock];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, c = lane >> 4;
-    const int KB = (a.K + kBlock - 1) / kBlock;
-    const int tm = (a.M + BM - 1) / BM;
+template <int BM, int BN>
+__device__ __forceinline__ Place place(const MmArgs &a, int splits) {
     const int id = st::xcd_order(blockIdx.x, gridDim.x);
-    const int m0 = id % tm * BM, n0 = id / tm * BN;
+    const int tiles = gridDim.x / splits, tm = (a.M + BM - 1) / BM, tn = tiles / tm;
+    const int split = id / tiles, tile = id - split * tiles;
+    const int panel = tile / (kPanel * tn), at = tile - panel * kPanel * tn, wide = min(kPanel, tm - panel * kPanel);
+    return {(panel * kPanel + at % wide) * BM, at / wide * BN, split};
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint8_t *p, int row0, int rows, int K) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (int64_t)row0 * K), (short)0, rows * K, kRsrcWord3);
+}
+
+// ------------------------------------------------------------------ a ring
+// BM x BN of y by WM x WN waves, S stages of LDS, K in slices where the tiles
+// alone leave CUs idle (f32 partial sums in the workspace, added in order by
+// reduce_kernel). Block b + S - 1 comes while b is multiplied.
+template <int BM, int BN, int WM, int WN, int S, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kernel(MmArgs a, float *part, int splits) {
+    constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, STEPS = MT * NT;
+    constexpr int DX = BM / 8 / W, DW = BN / 8 / W, ND = DX + DW;  // DMAs (8 rows) of a wave
+    static_assert(DX * 8 * W == BM && DW * 8 * W == BN && NT % 2 == 0 && BN / WN <= kBlock, "whole DMAs, one scale a wave");
+    constexpr int STAGE = (BM + BN) * kBlock;
+    __shared__ __align__(1024) uint8_t s0[STAGE], s1[STAGE], s2[STAGE], s3[S > 3 ? STAGE : 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, c = lane >> 4;
+    const int KB = (a.K + kBlock - 1) / kBlock;
+    const Place at = place<BM, BN>(a, splits);
+    const int m0 = at.m0, n0 = at.n0;
+    const int b0 = (int)((int64_t)KB * at.split / splits), b1 = (int)((int64_t)KB * (at.split + 1) / splits);
     const int wm0 = wave % WM * (BM / WM), wn0 = wave / WM * (BN / WN);
     const int rows_x = min(BM, a.M - m0), rows_w = min(BN, a.N - n0);
-    const __amdgpu_buffer_rsrc_t rx =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(a.x + (int64_t)m0 * a.K), (short)0, rows_x * a.K, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rw =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + (int64_t)n0 * a.K), (short)0, rows_w * a.K, kRsrcWord3);
-    // lane i of a DMA fills position i % 8 of its row i / 8
+    const __amdgpu_buffer_rsrc_t rx = rows_of(a.x, m0, rows_x, a.K), rw = rows_of(a.w, n0, rows_w, a.K);
+    // lane i of a DMA fills position i % 8 of its row i / 8; rows past the last repeat it
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     int vx[DX], vw[DW];
 #pragma unroll
     for (int j = 0; j < DX; ++j) vx[j] = min((wave * DX + j) * 8 + (lane >> 3), rows_x - 1) * a.K + chunk;
 #pragma unroll
     for (int j = 0; j < DW; ++j) vw[j] = min((wave * DW + j) * 8 + (lane >> 3), rows_w - 1) * a.K + chunk;
-    auto load = [&](uint8_t *s, int b) {
-        const bool in = b * kBlock + chunk < a.K;
-#pragma unroll
-        for (int j = 0; j < DX; ++j) dma16(rx, s + (wave * DX + j) * 1024, in ? vx[j] : kOutside, b * kBlock);
-#pragma unroll
-        for (int j = 0; j < DW; ++j) dma16(rw, s + BM * kBlock + (wave * DW + j) * 1024, in ? vw[j] : kOutside, b * kBlock);
+    auto dma = [&](uint8_t *s, int b, int j) {
+        const bool in = b * kBlock + chunk < a.K;  // (K ends inside the last block: zeros)
+        if (j < DW)
+            dma16(rw, s + BM * kBlock + (wave * DW + j) * 1024, in ? vw[j] : kOutside, b * kBlock);
+        else
+            dma16(rx, s + (wave * DX + j - DW) * 1024, in ? vx[j - DW] : kOutside, b * kBlock);
     };
-    const float *const sw = a.sw + (int64_t)((n0 + wn0) / kBlock) * KB;
-    const bool alive = n0 + wn0 < a.N;
-    float f[MT], fn[MT], g, gn;
-    auto load_scales = [&](float(&to)[MT], float &w, int b) {
+    auto load = [&](uint8_t *s, int b) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) to[t] = a.sx[b * a.sx_stride + min(m0 + wm0 + 16 * t + r, a.M - 1)];
-        w = alive ? sw[b] : 0.0f;
+        for (int j = 0; j < ND; ++j) dma(s, b, j);
+    };
+    const float *const sw = a.sw + (int64_t)min((n0 + wn0) / kBlock, (a.N - 1) / kBlock) * KB;
+    const float *sx[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sx[t] = a.sx + min(m0 + wm0 + 16 * t + r, a.M - 1);
+    float f[MT], fn[MT], gn;
+    auto load_scales = [&](int b) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fn[t] = sx[t][b * a.sx_stride];
+        gn = sw[b];
+    };
+    const int pos = r * kBlock + (c ^ (r & 7)) * 16;
+    auto frag = [&](const uint8_t *s, int row) {
+        Frag<EXACT> v;
+        v.set(*reinterpret_cast<const i32x4 *>(s + row * kBlock + pos), *reinterpret_cast<const i32x4 *>(s + row * kBlock + (pos ^ 64)));
+        return v;
     };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0, 0, 0, 0};
-    const int pos = (c ^ (r & 7)) * 16;
-    auto frag = [&](const uint8_t *s, int row) {
-        const uint8_t *p = s + (row + r) * kBlock;
-        Frag<F32> v;
-        v.set(*reinterpret_cast<const i32x4 *>(p + pos), *reinterpret_cast<const i32x4 *>(p + (pos ^ 64)));
-        return v;
-    };
-    auto step = [&](uint8_t *s, uint8_t *next, int b) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMAs of block b, and its scales
-        __syncthreads();                     // everyone's; and everyone has read `next`'s last block
+    Frag<EXACT> xf[MT], wf[2];
+    // Block b from s, whose first fragments are read, then those of b + 1 from
+    // `next`; block b + S - 1 to `to`, which held b - 1.
+    auto block = [&](const uint8_t *s, const uint8_t *next, uint8_t *to, int b) {
+        f32x4 p[D + 1];
+        const int bn = min(b + S - 1, b1 - 1);  // (past the end: the last again, unused)
+        load_scales(min(b + 1, b1 - 1));
 #pragma unroll
-        for (int t = 0; t < MT; ++t) f[t] = fn[t];
-        g = gn;
-        if (b + 1 < KB) {
-            load_scales(fn, gn, b + 1);
-            load(next, b + 1);
+        for (int i = 0; i < STEPS + D; ++i) {
+            const int u = i / MT, t = i % MT;
+            if (i < STEPS) {
+                if (t == 0) {
+                    if (u < NT - 1) {
+                        wf[(u + 1) & 1] = frag(s + BM * kBlock, wn0 + 16 * (u + 1));
+                    } else {
+                        // this wave's last fragments of b are read and its part of b + 1 has
+                        // come; after the barrier everyone's
+                        wait_loads<(S - 2) * ND, true>();
+                        __builtin_amdgcn_s_barrier();
+                        wf[(u + 1) & 1] = frag(next + BM * kBlock, wn0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                p[i % (D + 1)] = mfma(wf[u & 1], xf[t]);
+#pragma unroll
+                for (int j = 0; j < ND; ++j)
+                    if (i == j * (STEPS - MT) / ND) dma(to, bn, j);
+                if (u == NT - 1) xf[t] = frag(next, wm0 + 16 * t);
+            }
+            if (i >= D) {
+                const int j = i - D;
+                acc[j % MT][j / MT] += p[j % (D + 1)] * f[j % MT];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        Frag<F32> wf[NT];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) wf[u] = frag(s + BM * kBlock, wn0 + 16 * u);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const Frag<F32> xf = frag(s, wm0 + 16 * t);
-            const float fs = f[t] * g;
-#pragma unroll
-            for (int u = 0; u < NT; ++u) acc[t][u] += mfma(wf[u], xf) * fs;
-        }
+        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+        __builtin_amdgcn_sched_barrier(0);
     };
-    load_scales(fn, gn, 0);
-    load(s0, 0);
-    for (int b = 0; b < KB; b += 2) {
-        step(s0, s1, b);
-        if (b + 1 < KB) step(s1, s0, b + 1);
+    load_scales(b0);
+    load(s0, b0);
+    load(s1, min(b0 + 1, b1 - 1));
+    if constexpr (S > 3) load(s2, min(b0 + 2, b1 - 1));
+    wait_loads<(S - 2) * ND, true>();
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+    wf[0] = frag(s0 + BM * kBlock, wn0);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xf[t] = frag(s0, wm0 + 16 * t);
+    for (int b = b0; b < b1; b += S) {
+        if constexpr (S == 3) {
+            block(s0, s1, s2, b);
+            if (b + 1 < b1) block(s1, s2, s0, b + 1);
+            if (b + 2 < b1) block(s2, s0, s1, b + 2);
+        } else {
+            block(s0, s1, s3, b);
+            if (b + 1 < b1) block(s1, s2, s0, b + 1);
+            if (b + 2 < b1) block(s2, s3, s1, b + 2);
+            if (b + 3 < b1) block(s3, s0, s2, b + 3);
+        }
     }
+    wait_loads<0, true>();  // (no DMA after the wave's end)
+    void *const out = splits > 1 ? part + (int64_t)at.split * a.M * a.N : a.y;
+    const bool f32 = splits > 1 || a.f32;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = m0 + wm0 + 16 * t + r;
+        if (m < a.M)
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-            if (m < a.M) store_n4<F32>(a.y, m, n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
+            for (int u = 0; u < NT; ++u) store_n4(out, f32, m, n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
     }
 }
 
-template <int MT>
-void launch_mv(st_context *ctx, const MmArgs &a, bool f32) {
-    constexpr int W = 8;
-    const dim3 grid((unsigned)((a.N + 15) / 16)), block(64 * W);
-    f32 ? st::launch(ctx, mv_kernel<MT, W, true>, grid, block, 0, a) : st::launch(ctx, mv_kernel<MT, W, false>, grid, block, 0, a);
+// y of the slices' partial sums, four neighbours a thread, in slice order.
+__global__ __launch_bounds__(256) void reduce_kernel(const float *part, void *y, int64_t n, int splits, int f32) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if ((n & 3) == 0) {
+        if (i >= n) return;
+        f32x4 v = *reinterpret_cast<const f32x4 *>(part + i);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4 *>(part + s * n + i);
+        if (f32)
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(y) + i) = v;
+        else
+            *reinterpret_cast<half4 *>(static_cast<_Float16 *>(y) + i) = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+        return;
+    }
+    for (int64_t j = i; j < i + 4 && j < n; ++j) {
+        float v = part[j];
+        for (int s = 1; s < splits; ++s) v += part[s * n + j];
+        if (f32)
+            static_cast<float *>(y)[j] = v;
+        else
+            static_cast<_Float16 *>(y)[j] = (_Float16)v;
+    }
 }
 
-template <int BM, int BN, int WM, int WN>
-void launch_mm(st_context *ctx, const MmArgs &a, bool f32) {
-    const dim3 grid((unsigned)((a.M + BM - 1) / BM * ((a.N + BN - 1) / BN))), block(64 * WM * WN);
-    f32 ? st::launch(ctx, mm_kernel<BM, BN, WM, WN, true>, grid, block, 0, a)
-        : st::launch(ctx, mm_kernel<BM, BN, WM, WN, false>, grid, block, 0, a);
+// ------------------------------------------------------------ 256 x 256, f16 y
+// Eight waves of 64 x 128, two stages, the 8-bit instruction. x and each half of
+// w lie apart: once every wave has read x and the first half of block b (the
+// middle of the block), their places take block b + 2, the second half's at the
+// end, so that a DMA has 1 to 1.4 blocks' time (all of it after the end: 0.6 to
+// 0.9; 4096 x 4096 x 22016 373 -> 354 us).
+constexpr int WIDE = 256;
+__global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
+    constexpr int WM = 4, WN = 2, W = WM * WN, MT = WIDE / WM / 16, NT = WIDE / WN / 16, HN = WIDE / WN / 2;
+    constexpr int DX = WIDE / 8 / W, DW = WIDE / 16 / W;  // DMAs (8 rows) of a wave: of x, of each half of w
+    constexpr int STEPS = MT * NT, MID = STEPS / 2, LAST = MT * (NT - 1);
+    static_assert(MID + DX + DW < LAST && DW < MT, "a block's DMAs fit between its barriers");
+    __shared__ __align__(1024) uint8_t x0[WIDE * kBlock], x1[WIDE * kBlock];
+    __shared__ __align__(1024) uint8_t wa0[WIDE / 2 * kBlock], wa1[WIDE / 2 * kBlock], wb0[WIDE / 2 * kBlock], wb1[WIDE / 2 * kBlock];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, c = lane >> 4;
+    const int KB = (a.K + kBlock - 1) / kBlock;
+    const Place at = place<WIDE, WIDE>(a, 1);
+    const int m0 = at.m0, n0 = at.n0;
+    const int wm0 = wave % WM * (WIDE / WM), wn = wave / WM, wn0 = wn * (WIDE / WN);
+    const int rows_x = min(WIDE, a.M - m0), rows_w = min(WIDE, a.N - n0);
+    const __amdgpu_buffer_rsrc_t rx = rows_of(a.x, m0, rows_x, a.K), rw = rows_of(a.w, n0, rows_w, a.K);
+    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    int vx[DX], va[DW], vb[DW];
+#pragma unroll
+    for (int j = 0; j < DX; ++j) vx[j] = min((wave * DX + j) * 8 + (lane >> 3), rows_x - 1) * a.K + chunk;
+#pragma unroll
+    for (int j = 0; j < DW; ++j) {  // (each wave column's first 64 rows, and its last)
+        const int l = (wave * DW + j) * 8, row = l / HN * (2 * HN) + l % HN + (lane >> 3);
+        va[j] = min(row, rows_w - 1) * a.K + chunk;
+        vb[j] = min(row + HN, rows_w - 1) * a.K + chunk;
+    }
+    auto dma_x = [&](uint8_t *s, int b, int j) { dma16(rx, s + (wave * DX + j) * 1024, b * kBlock + chunk < a.K ? vx[j] : kOutside, b * kBlock); };
+    auto dma_a = [&](uint8_t *s, int b, int j) { dma16(rw, s + (wave * DW + j) * 1024, b * kBlock + chunk < a.K ? va[j] : kOutside, b * kBlock); };
+    auto dma_b = [&](uint8_t *s, int b, int j) { dma16(rw, s + (wave * DW + j) * 1024, b * kBlock + chunk < a.K ? vb[j] : kOutside, b * kBlock); };
+    const float *const sw = a.sw + (int64_t)min((n0 + wn0) / kBlock, (a.N - 1) / kBlock) * KB;
+    const float *sx[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sx[t] = a.sx + min(m0 + wm0 + 16 * t + r, a.M - 1);
+    float f[MT], fn[MT], gn;
+    auto load_scales = [&](int b) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fn[t] = sx[t][b * a.sx_stride];
+        gn = sw[b];
+    };
+    const int pos = r * kBlock + (c ^ (r & 7)) * 16;
+    auto frag = [&](const uint8_t *s, int row) {
+        Frag<false> v;
+        v.set(*reinterpret_cast<const i32x4 *>(s + row * kBlock + pos), *reinterpret_cast<const i32x4 *>(s + row * kBlock + (pos ^ 64)));
+        return v;
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0, 0, 0, 0};
+    Frag<false> xf[MT], wf[2];
+    // Block b from xs, was, wbs, whose first fragments are read, then those of
+    // b + 1 from xn and wan; block b + 2 to b's places.
+    auto block = [&](uint8_t *xs, uint8_t *was, uint8_t *wbs, const uint8_t *xn, const uint8_t *wan, int b) {
+        f32x4 p[D + 1];
+        const int b2 = min(b + 2, KB - 1);  // (past the end: the last again, unused)
+        load_scales(min(b + 1, KB - 1));
+#pragma unroll
+        for (int i = 0; i < STEPS + D; ++i) {
+            const int u = i / MT, t = i % MT;
+            if (i < STEPS) {
+                if (t == 0) {
+                    if (i == MID) {  // everyone has read x and the first half of w
+                        wait_lds();
+                        __builtin_amdgcn_s_barrier();
+                    }
+                    if (u == NT - 1) {  // everyone has read the rest, and b + 1 has come
+                        wait_loads<DX + DW, true>();
+                        __builtin_amdgcn_s_barrier();
+                        wf[(u + 1) & 1] = frag(wan, wn * HN);
+                    } else {
+                        wf[(u + 1) & 1] = u + 1 < NT / 2 ? frag(was, wn * HN + 16 * (u + 1)) : frag(wbs, wn * HN + 16 * (u + 1 - NT / 2));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                p[i % (D + 1)] = mfma(wf[u & 1], xf[t]);
+                if (i > MID && i - MID - 1 < DX) dma_x(xs, b2, i - MID - 1);
+                if (i > MID + DX && i - MID - DX - 1 < DW) dma_a(was, b2, i - MID - DX - 1);
+                if (i > LAST && i - LAST - 1 < DW) dma_b(wbs, b2, i - LAST - 1);
+                if (u == NT - 1) xf[t] = frag(xn, wm0 + 16 * t);
+            }
+            if (i >= D) {
+                const int j = i - D;
+                acc[j % MT][j / MT] += p[j % (D + 1)] * f[j % MT];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load = [&](uint8_t *xs, uint8_t *was, uint8_t *wbs, int b) {
+#pragma unroll
+        for (int j = 0; j < DX; ++j) dma_x(xs, b, j);
+#pragma unroll
+        for (int j = 0; j < DW; ++j) dma_a(was, b, j);
+#pragma unroll
+        for (int j = 0; j < DW; ++j) dma_b(wbs, b, j);
+    };
+    load_scales(0);
+    load(x0, wa0, wb0, 0);
+    load(x1, wa1, wb1, min(1, KB - 1));
+    wait_loads<DX + 2 * DW, true>();
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+    wf[0] = frag(wa0, wn * HN);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xf[t] = frag(x0, wm0 + 16 * t);
+    for (int b = 0; b < KB; b += 2) {
+        block(x0, wa0, wb0, x1, wa1, b);
+        if (b + 1 < KB) block(x1, wa1, wb1, x0, wa0, b + 1);
+    }
+    wait_loads<0, true>();
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = m0 + wm0 + 16 * t + r;
+        if (m < a.M)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) store_n4(a.y, false, m, n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
+    }
+}
+
+// ------------------------------------------------------------------ the choice
+// Estimated times (us), fitted to cold calls of 48 to 4096 tokens, K 2560 to
+// 11008, N 1024 to 65536: a launch, then for each round of workgroups a start
+// and end and K's blocks; slices add their sums' way through memory.
+enum Kind { MV, R64x64, R64x128, R128x64, R128x128, R128x256, R256x128, R256x256 };
+struct Tile {
+    Kind kind;
+    int bm, bn;
+    double ends, block8, block16;  // a round's start and end; a block by the 8-bit and the f16 instruction (0: not built)
+};
+constexpr Tile kTiles[] = {
+    {R64x64, 64, 64, 4.0, 0, 0.70},     {R64x128, 64, 128, 4.0, 0, 0.87},    {R128x64, 128, 64, 3.5, 0.51, 0.85},
+    {R128x128, 128, 128, 5.0, 0.61, 1.05}, {R128x256, 128, 256, 6.0, 1.0, 0}, {R256x128, 256, 128, 6.0, 0, 1.75},
+    {R256x256, 256, 256, 8.0, 1.5, 0},
+};
+
+struct Plan {
+    Kind kind;
+    int splits;
+};
+
+Plan plan(const st_context *ctx, const MmArgs &a) {
+    const int forced = st::tune(ctx, ST_TUNE_FP8_TILE, -1), slices = st::tune(ctx, ST_TUNE_FP8_SPLITS, -1);
+    Plan best{MV, 1};
+    const bool can_mv = a.M <= 64, exact = a.f32 || a.M <= 64;
+    if (can_mv && (forced == MV || (forced < 0 && a.M <= 32))) return best;
+    double least = can_mv ? mv_us(ctx, a) : 1e30;
+    const int KB = blocks(a.K);
+    auto built = [&](const Tile &t) { return (exact ? t.block16 : t.block8) != 0; };
+    bool force = false;
+    for (const Tile &t : kTiles) force |= t.kind == forced && built(t);
+    if (force) least = 1e30;
+    for (const Tile &t : kTiles) {
+        if (!built(t) || (force ? t.kind != forced : (t.bm == 64) != (a.M <= 64))) continue;
+        const double each = exact ? t.block16 : t.block8;
+        const int64_t tiles = (int64_t)((a.M + t.bm - 1) / t.bm) * ((a.N + t.bn - 1) / t.bn);
+        for (int s = 1; s <= 8 && s <= KB; s *= 2) {
+            const double sums = 4.0 * s * a.M * a.N;
+            if (s > 1 && (t.kind == R256x256 || sums > (double)ctx->ws_bytes)) break;
+            const double rounds = std::ceil((double)tiles * s / ctx->num_cus);
+            const double us = 3.0 + rounds * (t.ends + (KB + s - 1) / s * each) + (s > 1 ? 2.5 + sums / 5.5e6 : 0.0);
+            if (force && slices > 0 ? s <= slices : us < least) least = us, best = {t.kind, s};
+        }
+    }
+    return best;
+}
+
+template <int BM, int BN, int WM, int WN, int S, bool EXACT>
+void run_ring(st_context *ctx, const MmArgs &a, int splits) {
+    const dim3 grid((unsigned)((a.M + BM - 1) / BM * ((a.N + BN - 1) / BN) * splits));
+    st::launch(ctx, ring_kernel<BM, BN, WM, WN, S, EXACT>, grid, dim3(64 * WM * WN), 0, a, ctx->ws, splits);
+}
+
+int run(st_context *ctx, const MmArgs &a, Plan p) {
+    const bool exact = a.f32 || a.M <= 64;
+    const char *name = "fp8_ring_kernel";
+    switch (p.kind) {
+        case MV: return mv(ctx, a);
+        case R64x64: run_ring<64, 64, 2, 2, 4, true>(ctx, a, p.splits); break;
+        case R64x128: run_ring<64, 128, 2, 4, 4, true>(ctx, a, p.splits); break;
+        case R128x64:
+            exact ? run_ring<128, 64, 4, 2, 4, true>(ctx, a, p.splits) : run_ring<128, 64, 4, 2, 4, false>(ctx, a, p.splits);
+            break;
+        case R128x128:
+            exact ? run_ring<128, 128, 4, 2, 4, true>(ctx, a, p.splits) : run_ring<128, 128, 4, 2, 4, false>(ctx, a, p.splits);
+            break;
+        case R128x256: run_ring<128, 256, 4, 2, 3, false>(ctx, a, p.splits); break;
+        case R256x128: run_ring<256, 128, 4, 2, 3, true>(ctx, a, p.splits); break;
+        case R256x256: {
+            const dim3 grid((unsigned)((a.M + WIDE - 1) / WIDE * ((a.N + WIDE - 1) / WIDE)));
+            st::launch(ctx, wide_kernel, grid, dim3(512), 0, a);
+            name = "fp8_wide_kernel";
+        }
+    }
+    if (int rc = st::launch_check(name)) return rc;
+    if (p.splits == 1) return ST_OK;
+    const int64_t n = (int64_t)a.M * a.N;
+    st::launch(ctx, reduce_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, (const float *)ctx->ws, a.y, n, p.splits, a.f32);
+    return st::launch_check("fp8_reduce_kernel");
 }
 
 }  // namespace
@@ -261,14 +433,8 @@ extern "C" int st_fp8_gemm(st_context *ctx, const uint8_t *x, const float *x_sca
     if ((int64_t)blocks(M) * blocks(N) > (1 << 28)) return st::fail(ST_ERR_SHAPE, "%s: M=%d, N=%d", fn, M, N);
     if (!st::aligned16(x) || !st::aligned16(w) || !st::aligned16(y) || !aligned4(x_scale) || !aligned4(w_scale))
         return st::fail(ST_ERR_ALIGN, "%s: pointers must be 16-byte aligned (scales: 4)", fn);
-    const MmArgs a{x, w, x_scale, w_scale, y, scale_stride, M, K, N};
+    const MmArgs a{x, w, x_scale, w_scale, y, scale_stride, M, K, N, y_dtype == ST_F32};
     const st::OnDevice on(ctx);
     if (on.error != hipSuccess) return st::hip_fail(on.error, fn);
-    const bool f32 = y_dtype == ST_F32;
-    if (M <= 64) {
-        M <= 16 ? launch_mv<1>(ctx, a, f32) : M <= 32 ? launch_mv<2>(ctx, a, f32) : launch_mv<4>(ctx, a, f32);
-        return st::launch_check("mv_kernel");
-    }
-    launch_mm<128, 128, 2, 2>(ctx, a, f32);
-    return st::launch_check("mm_kernel");
+    return run(ctx, a, plan(ctx, a));
 }

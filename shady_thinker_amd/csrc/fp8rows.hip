@@ -23,18 +23,12 @@ struct NormArgs {
     int y_f32;
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
-    return v;
-}
-
 // One workgroup a row; a thread holds pieces of eight dims, blockDim.x apart,
 // from their load to the last store.
 template <bool RF32, bool XF32, int P>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
-    __shared__ float sums[16];
-    const int tid = threadIdx.x, wave = tid >> 6, waves = blockDim.x >> 6;
+    __shared__ f32x4 sums[16];  // of each wave's four rows of lanes
+    const int tid = threadIdx.x, waves = blockDim.x >> 6;
     const int64_t t = blockIdx.x;
     float r[P][8];
     float sum = 0.0f;
@@ -69,14 +63,15 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += r[p][i] * r[p][i];
     }
-    sum = wave_sum(sum);
-    if (waves > 1) {
-        if ((tid & 63) == 0) sums[wave] = sum;
-        __syncthreads();
-        sum = 0.0f;
-        for (int i = 0; i < waves; ++i) sum += sums[i];
-    }
-    const float norm = 1.0f / sqrtf(sum * a.per_d + a.eps);
+    sum = row_sum(sum);
+    if ((tid & 15) == 0) reinterpret_cast<float *>(sums)[tid >> 4] = sum;
+    __syncthreads();
+    f32x4 all = sums[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i)
+        if (i < waves) all += sums[i];
+    sum = (all.x + all.y) + (all.z + all.w);
+    const float norm = __builtin_amdgcn_rsqf(sum * a.per_d + a.eps);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const int piece = tid + p * (int)blockDim.x;
@@ -125,7 +120,7 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
             float y[8];
             rb.to(y);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] / (1.0f + __expf(-x[i])) * y[i];
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * -1.44269504f)) * y[i];
         }
     }
     const float s = block_scale(x);
@@ -138,7 +133,10 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
 
 template <bool RF32, bool XF32>
 void launch_norm(st_context *ctx, const NormArgs &a, int M) {
-    const int per = a.pieces <= 1024 ? 1 : a.pieces <= 2048 ? 2 : 4;
+    // One piece a thread up to 8192 dims (4095 rows of 4096, f32: 42.2 us; two 43.3, four 46.2; one row 2.9, 3.1, 3.7), but two
+    // of many f16 rows whose workgroups are large for what they load (4095 of 5120: 31.9 us, one 35.7, four 32.6)
+    const bool two = !RF32 && a.pieces > 512 && M >= ctx->num_cus;
+    const int per = a.pieces <= 1024 ? 1 + two : a.pieces <= 2048 ? 2 : 4;
     const dim3 block((unsigned)(((a.pieces + per - 1) / per + 63) / 64 * 64));
     if (per == 1)
         st::launch(ctx, norm_kernel<RF32, XF32, 1>, dim3((unsigned)M), block, 0, a);

@@ -23,24 +23,31 @@ _F32, _F16, _F8 = torch.float32, torch.float16, torch.float8_e4m3fn
 _DT = {_F32: ST_F32, _F16: ST_F16}
 
 
-def _on(gpu, t, name: str) -> None:
-    if t.device != gpu.device:
-        raise ValueError(f"{name}: on {t.device}, the context's device is {gpu.device}")
+# As in model.py, what is right in the common case is found by few cheap
+# tensor queries (a small call's kernel takes 3 us); what they do not pass goes
+# to a function that finds a permitted form or says what is wrong.
+def _device(gpu) -> int:
+    i = gpu.device.index
+    return -1 if i is None else i
 
 
-def _act_rows(gpu, t, name: str, m: int, k: int) -> tuple[int, int, int]:
-    """(address, dtype, elements from one row to the next) of `t` [m, k],
-    float32 or float16, a row's elements side by side."""
-    d = _DT.get(t.dtype)
-    if d is None:
+def _elsewhere(gpu, name: str, device):
+    raise ValueError(f"{name}: on {device}, the context's device is {gpu.device}")
+
+
+def _row_stride(gpu, t, name: str, m: int, k: int) -> int:
+    """Elements from one row to the next of a `t` [m, k] that the quick checks
+    did not pass: a part of wider rows, or refused."""
+    if t.dtype not in _DT:
         raise TypeError(f"{name}: dtype {t.dtype} (need float32 or float16)")
     if t.shape != (m, k):
         raise ValueError(f"{name}: shape {tuple(t.shape)} (need [{m}, {k}])")
-    _on(gpu, t, name)
+    if t.get_device() != _device(gpu):
+        _elsewhere(gpu, name, t.device)
     s = t.stride()
-    if s[1] != 1 and k > 1:
+    if s[1] != 1:
         raise ValueError(f"{name}: strides {s} (need rows of adjacent elements)")
-    return t.data_ptr(), d, s[0] if m > 1 else max(s[0], k)
+    return s[0] if m > 1 else max(s[0], k)
 
 
 class Fp8Rows:
@@ -72,7 +79,7 @@ class Fp8Rows:
                              f"[{fp8_blocks(k)}, {m}], a block's side by side, on {data.device})")
         self.data, self.scale, self.M, self.K = data, scale, m, k
         self.stride = max(scale.stride(0), m) if scale.shape[0] > 1 else m
-        self._at, self._scale_at, self.device = data.data_ptr(), scale.data_ptr(), data.device
+        self._at, self._scale_at, self._device = data.data_ptr(), scale.data_ptr(), data.get_device()
 
     def __getitem__(self, rows: slice) -> "Fp8Rows":
         """Rows [a:b] of these, sharing their memory."""
@@ -94,31 +101,43 @@ def add_rmsnorm(gpu, residual, weight, x=None, y=None, rows: Fp8Rows | None = No
     residual, residual_out (one dtype) and x [M, D] float32 or float16, rows
     of adjacent elements. The norm is of the sum before it is rounded to the
     residual's type."""
-    if residual.dim() != 2:
-        raise ValueError(f"residual: shape {tuple(residual.shape)} (need [M, D])")
-    m, d = residual.shape
-    rp, rd, rs = _act_rows(gpu, residual, "residual", m, d)
+    shape, dev = residual.shape, _device(gpu)
+    if len(shape) != 2:
+        raise ValueError(f"residual: shape {tuple(shape)} (need [M, D])")
+    m, d = shape
+    rd = _DT.get(residual.dtype)
+    rs = os_ = xs = ys = d
+    if rd is None or residual.get_device() != dev or not residual.is_contiguous():
+        rs = os_ = _row_stride(gpu, residual, "residual", m, d)
+    rp = residual.data_ptr()
     xp = op = yp = qp = sp = None
-    xd = xs = os_ = yd = ys = ss = 0
+    xd = yd = ss = 0
     if x is not None:
-        xp, xd, xs = _act_rows(gpu, x, "x", m, d)
-        if residual_out is None:
-            op, os_ = rp, rs
-        else:
+        xd = _DT.get(x.dtype)
+        if xd is None or x.shape != shape or x.get_device() != dev or not x.is_contiguous():
+            xs = _row_stride(gpu, x, "x", m, d)
+        xp, op = x.data_ptr(), rp
+        if residual_out is not None:
             if residual_out.dtype is not residual.dtype:
                 raise TypeError(f"residual_out: dtype {residual_out.dtype} (need the residual's, {residual.dtype})")
-            op, _, os_ = _act_rows(gpu, residual_out, "residual_out", m, d)
+            os_ = d
+            if residual_out.shape != shape or residual_out.get_device() != dev or not residual_out.is_contiguous():
+                os_ = _row_stride(gpu, residual_out, "residual_out", m, d)
+            op = residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out without x")
     if weight.dtype is not _F32 or weight.numel() != d or not weight.is_contiguous():
         raise ValueError(f"weight: {weight.dtype} {tuple(weight.shape)} (need contiguous float32 [{d}])")
-    _on(gpu, weight, "weight")
+    if weight.get_device() != dev:
+        _elsewhere(gpu, "weight", weight.device)
     if y is not None:
-        yp, yd, ys = _act_rows(gpu, y, "y", m, d)
+        yd = _DT.get(y.dtype)
+        if yd is None or y.shape != shape or y.get_device() != dev or not y.is_contiguous():
+            ys = _row_stride(gpu, y, "y", m, d)
+        yp = y.data_ptr()
     if rows is not None:
-        if rows.M != m or rows.K != d:
-            raise ValueError(f"rows: [{rows.M}, {rows.K}] (need [{m}, {d}])")
-        _on(gpu, rows, "rows")
+        if rows.M != m or rows.K != d or rows._device != dev:
+            raise ValueError(f"rows: [{rows.M}, {rows.K}] on {rows.data.device} (need [{m}, {d}] on {gpu.device})")
         qp, sp, ss = rows._at, rows._scale_at, rows.stride
     elif y is None:
         raise ValueError("add_rmsnorm: neither y nor rows")
@@ -131,29 +150,31 @@ def fp8_quant(gpu, a, rows: Fp8Rows, b=None) -> None:
     """rows = a, or silu(a) * b, quantised; a and b [M, K] float32 or float16
     (one dtype), rows of adjacent elements (the halves of a gate|up row will
     do)."""
-    ap, ad, as_ = _act_rows(gpu, a, "a", rows.M, rows.K)
-    bp, bs = None, 0
+    m, k, dev = rows.M, rows.K, rows._device
+    if dev != _device(gpu):
+        _elsewhere(gpu, "rows", rows.data.device)
+    ad, as_, bp, bs = _DT.get(a.dtype), k, None, k
+    if ad is None or a.shape != (m, k) or a.get_device() != dev or not a.is_contiguous():
+        as_ = _row_stride(gpu, a, "a", m, k)
     if b is not None:
         if b.dtype is not a.dtype:
             raise TypeError(f"b: dtype {b.dtype} (need a's, {a.dtype})")
-        bp, _, bs = _act_rows(gpu, b, "b", rows.M, rows.K)
-    _on(gpu, rows, "rows")
+        if b.shape != (m, k) or b.get_device() != dev or not b.is_contiguous():
+            bs = _row_stride(gpu, b, "b", m, k)
+        bp = b.data_ptr()
     gpu.sync_stream()
-    call("st_fp8_quant", gpu.handle, ap, bp, ad, as_, bs, rows._at, rows._scale_at, rows.stride, rows.M, rows.K)
+    call("st_fp8_quant", gpu.handle, a.data_ptr(), bp, ad, as_, bs, rows._at, rows._scale_at, rows.stride, m, k)
 
 
 def fp8_gemm(gpu, rows: Fp8Rows, w: Fp8Weight, y) -> None:
     """y [M, N] (float32 or float16) = rows . w^T, M of any size."""
-    if rows.K != w.K:
-        raise ValueError(f"rows of {rows.K} dims, a weight of {w.K}")
+    m, k, n, dev = rows.M, w.K, w.N, rows._device
     d = _DT.get(y.dtype)
-    if d is None:
-        raise TypeError(f"y: dtype {y.dtype} (need float32 or float16)")
-    if y.numel() != rows.M * w.N or not y.is_contiguous():
-        raise ValueError(f"y: {tuple(y.shape)}, strides {y.stride()} (need contiguous [{rows.M}, {w.N}])")
-    _on(gpu, y, "y")
-    _on(gpu, rows, "rows")
-    _on(gpu, w.w, "w")
+    if (d is None or rows.K != k or y.shape != (m, n) or not y.is_contiguous() or y.get_device() != dev or w._device != dev
+            or _device(gpu) != dev):
+        if d is None:
+            raise TypeError(f"y: dtype {y.dtype} (need float32 or float16)")
+        raise ValueError(f"y {tuple(y.shape)}, strides {y.stride()}, on {y.device} = rows [{m}, {rows.K}] on {rows.data.device} . weight "
+                         f"[{n}, {k}] on {w.w.device}: need a contiguous [{m}, {n}], all on {gpu.device}")
     gpu.sync_stream()
-    call("st_fp8_gemm", gpu.handle, rows._at, rows._scale_at, rows.stride, w.w.data_ptr(), w.scale.data_ptr(), y.data_ptr(), d, rows.M,
-         w.K, w.N)
+    call("st_fp8_gemm", gpu.handle, rows._at, rows._scale_at, rows.stride, w._at, w._scale_at, y.data_ptr(), d, m, k, n)

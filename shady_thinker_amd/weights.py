@@ -248,6 +248,9 @@ class Fp8Weight:
     K: int
     N: int
 
+    def __post_init__(self):
+        self._at, self._scale_at, self._device = self.w.data_ptr(), self.scale.data_ptr(), self.w.get_device()
+
     @classmethod
     def of(cls, w, scale) -> "Fp8Weight":
         """A weight over the caller's device tensors."""

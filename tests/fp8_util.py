@@ -71,18 +71,19 @@ def eights(x8, sx, w8, sw):
     return tot
 
 
-def check_product(y, x8, sx, w8, sw):
+def check_product(y, x8, sx, w8, sw, many=None):
     """Products are exact; a block's sum of 128 and the FMAs over the blocks
     round each once to f32 (at most a whole step in the matrix unit), the
     block's factor once, the output once. With f16 y and many tokens a product
     is cut below 2^-13 of the power of two of the largest of its eight k: seven
-    products (the largest is not cut) by at most that each."""
+    products (the largest is not cut) by at most that each; many: whether these
+    rows were part of such a call."""
     want, s = product(x8, sx, w8, sw)
     m, k = x8.shape
     bound = (2 * min(k, B) + 3 * blocks(k)) * U * s + 2.0**-149
     if y.dtype is torch.float16:
         bound = bound + want.abs() * 2.0**-11 + 2.0**-25
-        if m > 64:
+        if m > 64 if many is None else many:
             bound = bound + 7 * 2.0**-13 * eights(x8, sx, w8, sw) * (1 + 2.0**-10)
     off = (y.cpu().double() - want).abs() - bound
     assert (off <= 0).all(), (off.max(), (off > 0).sum())

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import shady_thinker_amd as sta
+from shady_thinker_amd._lib import launches
 from fp8_util import B, F8, U, blocks, check_product, check_rows, rows_of, scales, weight_of
 
 pytestmark = pytest.mark.gpu
@@ -207,6 +208,59 @@ def test_gemm(gpu, m, k, n, dtype):
     assert torch.equal(y, again)
 
 
+def tile_cases():
+    """(tile, slices, m, k, n, dtype) of every tile that is built for the type."""
+    sizes = [(33, 16, 1), (64, 400, 65), (65, 128, 3), (100, 1424, 260), (128, 144, 128), (255, 272, 257), (300, 528, 1000), (513, 2064, 129),
+             (1600, 384, 300)]
+    for m, k, n in sizes:
+        for dtype in (F32, F16):
+            for tile in (1, 2, 3, 4, 6) if dtype is F32 or m <= 64 else (3, 4, 5, 7):
+                yield from ((tile, s, m, k, n, dtype) for s in ((1, 2, 8) if tile != 7 else (1,)))
+
+
+@pytest.mark.parametrize("tile,splits,m,k,n,dtype", tile_cases())
+def test_gemm_tiles(gpu, tune, tile, splits, m, k, n, dtype):
+    """Every tile, one block of K to many in each slice, at the tiles' edges."""
+    tune(FP8_TILE=tile, FP8_SPLITS=splits)
+    x8, sx, w8, sw = gemm_case(m + k + n, m, k, n)
+    buf = torch.full((m * n + 64,), 7.0, dtype=dtype, device=DEV)
+    y = buf[:m * n].view(m, n)
+    launches()
+    sta.fp8_gemm(gpu, sta.Fp8Rows.of(x8, sx), sta.Fp8Weight.of(w8, sw), y)
+    ran = launches()
+    assert ran == ["fp8_wide_kernel" if tile == 7 else "fp8_ring_kernel"] + ["fp8_reduce_kernel"] * (splits > 1 and k > B)
+    check_product(y, x8, sx, w8, sw)
+    assert (buf[m * n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("m", [1, 8, 9, 16, 17, 32, 33, 48, 49, 64])
+@pytest.mark.parametrize("k,n", [(16, 5), (1168, 140), (2560, 1300), (400, 5400), (272, 9000), (144, 11008), (272, 13830), (144, 19456), (16, 28700)])
+def test_few_tokens_shapes(gpu, tune, m, k, n):
+    """The few tokens' kernel at widths of each of its shapes (16 to 64 columns
+    a workgroup: N over its columns' blocks, ends and scales)."""
+    tune(FP8_TILE=0)
+    x8, sx, w8, sw = gemm_case(m + k + n, m, k, n)
+    buf = torch.full((m * n + 64,), 7.0, device=DEV)
+    y = buf[:m * n].view(m, n)
+    launches()
+    sta.fp8_gemm(gpu, sta.Fp8Rows.of(x8, sx), sta.Fp8Weight.of(w8, sw), y)
+    assert launches() == ["fp8_mv_kernel"]
+    check_product(y, x8, sx, w8, sw)
+    assert (buf[m * n:] == 7.0).all()
+
+
+def test_gemm_without_room_for_slices(gpu):
+    """Slices whose partial sums do not fit the workspace are not taken (the
+    largest K and few tiles, 64 MiB)."""
+    m, k, n = 1200, 11008, 3500  # (4 slices: 67 MB, 8: 134)
+    x8, sx, w8, sw = gemm_case(3, m, k, n)
+    y = torch.empty(m, n, dtype=F16, device=DEV)
+    with gpu.tuning(FP8_TILE=4, FP8_SPLITS=8):
+        sta.fp8_gemm(gpu, sta.Fp8Rows.of(x8, sx), sta.Fp8Weight.of(w8, sw), y)
+    for at in (slice(0, 20), slice(m - 20, m)):
+        check_product(y[at], x8[at], sx[:, at], w8, sw, many=True)
+
+
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_gemm_every_place(gpu, m):
     """One-hot rows return the weight's columns exactly: every k and n has its
@@ -348,7 +402,7 @@ def test_gemm_past_32_bits(gpu):
     y = torch.empty(n, 20, dtype=F16, device=DEV)
     sta.fp8_gemm(gpu, sta.Fp8Rows.of(big, sx * 2.0**-10), sta.Fp8Weight.of(w8, sw), y)
     for at in (slice(0, 40), slice(n - 40, n)):
-        check_product(y[at], big[at], sx[:, at] * 2.0**-10, w8, sw)
+        check_product(y[at], big[at], sx[:, at] * 2.0**-10, w8, sw, many=True)
     del big, y
     x = rand(3, 50, k, dtype=F16).repeat(n // 50, 1)
     rows = sta.Fp8Rows(gpu, x.shape[0], k)
