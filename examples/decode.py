@@ -2,10 +2,12 @@
 attention and token log probabilities, captured as one HIP graph and replayed
 for each token of a batch (greedy; every token with its log probability).
 
-    python examples/decode.py [--tokens 16] [--batch 4] [--int8]
+    python examples/decode.py [--tokens 16] [--batch 4] [--int8] [--fp8]
 
 The weights are random, of a small self-attention model; what a model adds of
 its own (norms, residual adds, the embedding) are torch operations in hooks.
+With --fp8 the linears are e4m3 with block scales and the norms, residual adds
+and quantised rows are the framework's (ResidualNorms).
 """
 import argparse
 import os
@@ -26,11 +28,20 @@ def linear(gpu, rng, k, n):
     return sta.GptqWeight.upload(gpu, qw, scales.astype(np.float16), 128)
 
 
-def build(gpu, seed=0):
+def fp8_linear(gpu, rng, k, n):
+    w = torch.from_numpy(rng.standard_normal((n, k), dtype=np.float32)) / np.sqrt(k)
+    blocks = w.view(n // 128, 128, k // 128, 128)
+    scale = blocks.abs().amax((1, 3)) / 448.0
+    w8 = (blocks / scale[:, None, :, None]).to(torch.float8_e4m3fn).view(n, k)
+    return sta.Fp8Weight.upload(gpu, w8, scale)
+
+
+def build(gpu, seed=0, fp8=False):
     rng = np.random.default_rng(seed)
-    mk = lambda k, n: linear(gpu, rng, k, n)
+    mk = lambda k, n: (fp8_linear if fp8 else linear)(gpu, rng, k, n)
     q, kv = HEADS * DIM, KV_HEADS * DIM
-    layers = [sta.DecoderLinears(mk(HIDDEN, q), mk(HIDDEN, kv), mk(HIDDEN, kv), mk(q, HIDDEN), mk(HIDDEN, INTER), mk(HIDDEN, INTER),
+    layer = sta.Fp8DecoderLinears if fp8 else sta.DecoderLinears
+    layers = [layer(mk(HIDDEN, q), mk(HIDDEN, kv), mk(HIDDEN, kv), mk(q, HIDDEN), mk(HIDDEN, INTER), mk(HIDDEN, INTER),
                                  mk(INTER, HIDDEN)) for _ in range(LAYERS)]
     embedding = torch.from_numpy(rng.standard_normal((VOCAB, HIDDEN), dtype=np.float32)).to(gpu.device)
     return sta.DecoderStack(layers, mk(HIDDEN, VOCAB)), embedding
@@ -85,13 +96,27 @@ class Hooks(sta.PagedAttention):
         self.tokens.copy_(self.top[:, 0])
 
 
+class Fp8Hooks(sta.ResidualNorms, Hooks):
+    """As Hooks, with the framework's norms."""
+
+    def __init__(self, gpu, stack, embedding, table, cache_dtype):
+        super().__init__(gpu, embedding, table, cache_dtype)
+        ones = torch.ones(HIDDEN, device=gpu.device)
+        self.init_norms(gpu, stack, table.shape[0], [ones] * LAYERS, [ones] * LAYERS, ones)
+
+    def embed(self, b):
+        self.advance()
+        self.residual.copy_(self.embedding[self.tokens.long()])
+
+
 def decode(gpu, stack, embedding, prompts, tokens, cache_dtype=torch.float16, graph=True):
     """prompts [B, n] int32: `tokens` more of each, their log probabilities,
     and the last step's logits."""
     B, n = prompts.shape
     pages = -(-(n + tokens) // 16)
     table = torch.randperm(B * pages, generator=torch.Generator().manual_seed(1)).view(B, pages)
-    h = Hooks(gpu, embedding, table.to(gpu.device, torch.int32), cache_dtype)
+    table = table.to(gpu.device, torch.int32)
+    h = Fp8Hooks(gpu, stack, embedding, table, cache_dtype) if stack.layers[0].fp8 else Hooks(gpu, embedding, table, cache_dtype)
     b = stack.buffers(gpu, B)
     run = stack.capture(gpu, b, h) if graph else None
     ids, lps = [], []
@@ -111,9 +136,10 @@ def main():
     ap.add_argument("--tokens", type=int, default=16)
     ap.add_argument("--batch", type=int, default=4)
     ap.add_argument("--int8", action="store_true", help="int8 cache")
+    ap.add_argument("--fp8", action="store_true", help="e4m3 linears with block scales")
     a = ap.parse_args()
     gpu = sta.GpuContext(0)
-    stack, embedding = build(gpu)
+    stack, embedding = build(gpu, fp8=a.fp8)
     prompts = torch.arange(a.batch * 5, dtype=torch.int32, device=gpu.device).view(a.batch, 5) * 37 % VOCAB
     ids, lps, _ = decode(gpu, stack, embedding, prompts, a.tokens, torch.int8 if a.int8 else torch.float16)
     for row, lp in zip(ids.tolist(), lps.tolist()):

@@ -19,7 +19,15 @@ from .model import (  # noqa: F401
     linear,
 )
 from .attention import KvCache, PagedAttention, kv_read, paged_attention, qk_norm_rope_store, token_logprobs  # noqa: F401
-from .fp8 import Fp8Rows, add_rmsnorm, fp8_gemm, fp8_quant  # noqa: F401
-from .layer import DecoderLinears, DecoderStack, DeltaNetLinears, StackBuffers, StackGraph, layer_from_linears  # noqa: F401
-from .loader import load_gptq_checkpoint, read_gptq_checkpoint  # noqa: F401
+from .fp8 import Fp8Rows, ResidualNorms, add_rmsnorm, fp8_gemm, fp8_quant  # noqa: F401
+from .layer import (  # noqa: F401
+    DecoderLinears,
+    DecoderStack,
+    DeltaNetLinears,
+    Fp8DecoderLinears,
+    StackBuffers,
+    StackGraph,
+    layer_from_linears,
+)
+from .loader import load_fp8_checkpoint, load_gptq_checkpoint, read_gptq_checkpoint  # noqa: F401
 from .weights import Fp8Weight, GptqWeight, Int8Weight, QuantConfig  # noqa: F401

@@ -8,7 +8,8 @@ the other linears, on torch device tensors and torch's current stream:
 * `Fp8Rows`: quantised rows, e4m3 with a scale for each token and 128 dims;
 * `add_rmsnorm`: residual addition and norm, to such rows, to f32 / f16, or both;
 * `fp8_quant`: rows, or silu(a) * b, to such rows;
-* `fp8_gemm`: rows times an `Fp8Weight` (weights.py), any number of tokens.
+* `fp8_gemm`: rows times an `Fp8Weight` (weights.py), any number of tokens;
+* `ResidualNorms`: the residual and norms of a model as a DecoderStack's hooks.
 
 Errors raise ValueError / TypeError (arguments) or ShadyHipError (a call).
 """
@@ -178,3 +179,44 @@ def fp8_gemm(gpu, rows: Fp8Rows, w: Fp8Weight, y) -> None:
                          f"[{n}, {k}] on {w.w.device}: need a contiguous [{m}, {n}], all on {gpu.device}")
     gpu.sync_stream()
     call("st_fp8_gemm", gpu.handle, rows._at, rows._scale_at, rows.stride, w._at, w._scale_at, y.data_ptr(), d, m, k, n)
+
+
+class ResidualNorms:
+    """The residual stream of a model and the norms before its linears, as a
+    DecoderStack's hooks (src/model.rs:685-691, 799-802, 820-823): one launch
+    before each layer's attention side, one before its MLP, one before the
+    lm_head. Layers that read quantised rows get them from the norm.
+
+    A subclass adds `embed(b)`, which fills `residual` [batch, hidden] (float32)
+    at the start of a step, and may be a PagedAttention too. attention and mlp:
+    each layer's norm weights [hidden] float32; last: the lm_head's; one_plus:
+    they hold w - 1."""
+
+    fills_rows = True
+
+    def init_norms(self, gpu, stack, batch: int, attention, mlp, last, eps: float = 1e-6, one_plus: bool = False) -> None:
+        n = len(stack.layers)
+        if len(attention) != n or len(mlp) != n:
+            raise ValueError(f"ResidualNorms: {len(attention)} and {len(mlp)} norm weights for {n} layers")
+        self.residual = torch.zeros(batch, stack.layers[0].hidden, device=gpu.device)
+        self._norms = (gpu, eps, one_plus)
+        self._attention_norms, self._mlp_norms, self._last_norm = attention, mlp, last
+        self._fp8 = [L.fp8 for L in stack.layers] + [isinstance(stack.lm_head, Fp8Weight)]
+
+    def embed(self, b) -> None:
+        raise NotImplementedError("ResidualNorms: embed(b) fills the residual")
+
+    def _norm(self, weight, x, fp8, y, rows) -> None:
+        gpu, eps, one_plus = self._norms
+        add_rmsnorm(gpu, self.residual, weight, x, None if fp8 else y, rows if fp8 else None, eps=eps, one_plus=one_plus)
+
+    def pre_attention(self, i, b) -> None:
+        if i == 0:
+            self.embed(b)
+        self._norm(self._attention_norms[i], b.down if i else None, self._fp8[i], b.x, b.x8)
+
+    def post_attention(self, i, b) -> None:
+        self._norm(self._mlp_norms[i], b.o, self._fp8[i], b.xm, b.xm8)
+
+    def final(self, b) -> None:
+        self._norm(self._last_norm, b.down, self._fp8[-1], b.x, b.x8)

@@ -29,6 +29,10 @@ for a block of tokens:
   through the prefill GEMM, with the down projections on silu(a) * b fused
   into the GEMM's A pre-pass (`st_gptq_i4_silu_gemm`).
 
+`Fp8DecoderLinears` is a self-attention layer whose weights are e4m3 with block
+scales (no reference counterpart): its inputs are quantised rows, q|k|v and
+gate|up one product each, for any number of tokens.
+
 Attention (self or DeltaNet), norms and residuals sit between these calls in
 a model and are not part of this path; the caller passes their outputs in.
 
@@ -43,7 +47,8 @@ import contextlib
 
 from . import model as M
 from ._lib import call
-from .weights import GptqWeight
+from .fp8 import Fp8Rows, fp8_gemm, fp8_quant
+from .weights import Fp8Weight, GptqWeight
 
 _DECODE_MAX = 32     # tokens per decode call (st_gptq_i4_matvec)
 _GATE_UP_BLOCK = 32  # tokens per st_gptq_i4_gate_up_silu call
@@ -57,6 +62,8 @@ def _mv(gpu, name, x, w: GptqWeight, y) -> None:
 class _Mlp:
     """The MLP shared by both layer kinds: gate, up (one fused call) and
     down, all GptqWeights of one group size."""
+
+    fp8 = False
 
     def _init_mlp(self, gate: GptqWeight, up: GptqWeight, down: GptqWeight, hidden: int) -> None:
         if gate.K != hidden or up.K != hidden:
@@ -227,11 +234,82 @@ class DeltaNetLinears(_Mlp):
         self._mlp_prefill(gpu, x if xm is None else xm, gate_out, up_out, down_out)
 
 
+def _fp8_rows(gpu, x, k: int) -> Fp8Rows:
+    """x as quantised rows of k dims (it may be such rows already)."""
+    if isinstance(x, Fp8Rows):
+        return x
+    m = M._rows(x, k)
+    rows = Fp8Rows(gpu, m, k)
+    fp8_quant(gpu, x.view(m, k), rows)
+    return rows
+
+
+class Fp8DecoderLinears:
+    """A self-attention layer of Fp8Weights: q, k, v, o, gate, up and down. q|k|v
+    and gate|up are concatenated along N at construction (Fp8Weight.cat: all but
+    the last of each whole blocks of 128), so that a layer is four products. q
+    may be the reference's gated width (2 * nh * hd, src/model.rs:696) while o
+    reads nh * hd."""
+
+    kind = "self_attn"
+    fp8 = True
+
+    def __init__(self, q: Fp8Weight, k: Fp8Weight, v: Fp8Weight, o: Fp8Weight, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight):
+        if not (q.K == k.K == v.K == gate.K == up.K):
+            raise ValueError("q, k, v, gate and up must read the same hidden size")
+        if o.N != q.K:
+            raise ValueError("o must write the hidden size")
+        if gate.N != up.N or down.K != gate.N or down.N != q.K:
+            raise ValueError("inconsistent MLP shapes")
+        self.hidden, self.inter, self.attn_dim = q.K, gate.N, o.K
+        self.qkv, self.gate_up = Fp8Weight.cat([q, k, v]), Fp8Weight.cat([gate, up])
+        self.splits = (q.N, k.N, v.N)
+        self.o, self.down = o, down
+
+    @classmethod
+    def from_linears(cls, linears: dict, layer: int, layer_prefix: str = "model.layers") -> "Fp8DecoderLinears":
+        """From load_fp8_checkpoint's {prefix: Fp8Weight}, by the tensor names
+        of DecoderLinears.from_linears."""
+        pfx = f"{layer_prefix}.{layer}"
+        names = [f"{pfx}.self_attn.{p}_proj" for p in "qkvo"] + [f"{pfx}.mlp.{p}_proj" for p in ("gate", "up", "down")]
+        missing = [n for n in names if not isinstance(linears.get(n), Fp8Weight)]
+        if missing:
+            raise KeyError(f"Fp8DecoderLinears.from_linears: no e4m3 linear {missing[0]}")
+        return cls(*(linears[n] for n in names))
+
+    def _mlp(self, gpu, rows: Fp8Rows, gate_up_out, h: Fp8Rows, down_out) -> None:
+        fp8_gemm(gpu, rows, self.gate_up, gate_up_out)
+        fp8_quant(gpu, gate_up_out[:, :self.inter], h, gate_up_out[:, self.inter:])
+        fp8_gemm(gpu, h, self.down, down_out)
+
+    def decode(self, gpu, x, attn, qkv_out, o_out, gate_up_out, down_out, xm=None) -> None:
+        """x [M, hidden], attn [M, attn_dim] and xm (the MLP's input; default x),
+        float32, float16 or Fp8Rows; any M. Writes qkv_out [M, q+k+v], o_out
+        [M, hidden], gate_up_out [M, 2 inter] (gate, then up) and down_out
+        [M, hidden] = (silu(gate) * up).Wd, float32 (decode) or float16
+        (prefill)."""
+        rows = _fp8_rows(gpu, x, self.hidden)
+        fp8_gemm(gpu, rows, self.qkv, qkv_out)
+        fp8_gemm(gpu, _fp8_rows(gpu, attn, self.attn_dim), self.o, o_out)
+        if xm is not None:
+            rows = _fp8_rows(gpu, xm, self.hidden)
+        self._mlp(gpu, rows, gate_up_out, Fp8Rows(gpu, rows.M, self.inter), down_out)
+
+    prefill = decode
+
+    def nbytes(self) -> int:
+        return sum(w.nbytes for w in (self.qkv, self.o, self.gate_up, self.down))
+
+
 def layer_from_linears(linears: dict, layer: int, layer_prefix: str = "model.layers"):
     """The layer's linears of whichever kind it is: self-attention when
     `{layer_prefix}.{i}.self_attn.q_proj` was loaded (the reference's test,
-    src/weights.rs:247-250), DeltaNet otherwise."""
-    if f"{layer_prefix}.{layer}.self_attn.q_proj" in linears:
+    src/weights.rs:247-250; Fp8DecoderLinears when that is an Fp8Weight),
+    DeltaNet otherwise."""
+    q = linears.get(f"{layer_prefix}.{layer}.self_attn.q_proj")
+    if isinstance(q, Fp8Weight):
+        return Fp8DecoderLinears.from_linears(linears, layer, layer_prefix)
+    if q is not None:
         return DecoderLinears.from_linears(linears, layer, layer_prefix)
     return DeltaNetLinears.from_linears(linears, layer, layer_prefix)
 
@@ -244,7 +322,8 @@ class StackBuffers:
     or the DeltaNet core's output), o (the output projection's), xm (normed
     hidden of the MLP, input of gate/up), h = silu(gate) * up, down, logits;
     and, for DeltaNet layers at several tokens, z (in_proj_z's output, rows
-    of its own).
+    of its own). For Fp8DecoderLinears: the quantised x8, xm8, attn8 (as attn)
+    and h8 (Fp8Rows), and gate_up (the product's output).
 
     Layers of different kinds have different widths: qkv and attn are
     per-layer views (`qkv_of(i)`, `attn_of(i)`) of one buffer of the widest
@@ -268,6 +347,16 @@ class StackBuffers:
         self.x, self.o, self.xm = mk(L0.hidden), mk(L0.hidden), mk(L0.hidden)
         self.h, self.down = mk(L0.inter), mk(L0.hidden)
         self.logits = mk(stack.vocab)
+        f8 = [L for L in stack.layers if L.fp8]
+        rows = lambda n: Fp8Rows(gpu, batch, n)
+        self.x8 = rows(L0.hidden) if f8 or isinstance(stack.lm_head, Fp8Weight) else None
+        if f8:
+            self.xm8, self.h8, self.gate_up = rows(L0.hidden), rows(L0.inter), mk(2 * L0.inter)
+            by_width = {L.attn_dim: rows(L.attn_dim) for L in f8}
+            self._attn8 = [by_width[L.attn_dim] if L.fp8 else None for L in stack.layers]
+            self.attn8 = self._attn8[0]
+        else:
+            self.xm8, self.attn8, self._attn8 = None, None, [None] * len(stack.layers)
 
     def qkv_of(self, i: int):
         return self._qkv[i]
@@ -277,7 +366,7 @@ class StackBuffers:
 
     def select(self, i: int) -> None:
         """Make layer i's views the current `qkv` and `attn`."""
-        self.qkv, self.attn = self._qkv[i], self._attn[i]
+        self.qkv, self.attn, self.attn8 = self._qkv[i], self._attn[i], self._attn8[i]
 
 
 class DecoderStack:
@@ -287,8 +376,9 @@ class DecoderStack:
     on the host and submits once per linear (src/model.rs:348-353, 682-834:
     self-attention q/k/v :694-714 and o :727-729, DeltaNet in_proj_qkv/z
     :749-756 and out_proj :786-791, gate/up/down :803-812, lm_head :824-834).
-    Layers are DecoderLinears or DeltaNetLinears, in any mix (the
-    reference's hybrid models).
+    Layers are DecoderLinears, DeltaNetLinears or Fp8DecoderLinears, in any mix
+    (the reference's hybrid models); the lm_head is a GptqWeight, an Fp8Weight
+    or bf16.
 
     Between the projections a model runs its own ops (norms, attention or the
     DeltaNet core, residual adds: src/model.rs:685-690, 715-726, 758-784,
@@ -308,6 +398,9 @@ class DecoderStack:
       warm_up()             (by `capture` alone) a context around the eager
                             step that it runs before it records one: hooks
                             that keep a state put it back
+    Hooks with a true attribute `fills_rows` (ResidualNorms) fill b.x8 and b.xm8
+    for layers that read quantised rows (and b.x8 for such an lm_head), in
+    place of b.x and b.xm; otherwise the step quantises b.x and b.xm.
     Without hooks the projections run on the buffers as they are (the
     benchmark's synthetic activations); gate/up then reads b.xm and the
     lm_head b.x."""
@@ -322,6 +415,10 @@ class DecoderStack:
         self.layers = layers
         self.lm_head = lm_head
         if isinstance(lm_head, GptqWeight):
+            if lm_head.K != L0.hidden:
+                raise ValueError("DecoderStack: lm_head K differs from the hidden size")
+            self.vocab = lm_head.N
+        elif isinstance(lm_head, Fp8Weight):
             if lm_head.K != L0.hidden:
                 raise ValueError("DecoderStack: lm_head K differs from the hidden size")
             self.vocab = lm_head.N
@@ -342,18 +439,32 @@ class DecoderStack:
         return StackBuffers(gpu, self, batch)
 
     def nbytes(self) -> int:
-        lm = self.lm_head.nbytes if isinstance(self.lm_head, GptqWeight) else self.lm_head.numel() * 2
+        lm = self.lm_head.nbytes if isinstance(self.lm_head, (GptqWeight, Fp8Weight)) else self.lm_head.numel() * 2
         return sum(L.nbytes() for L in self.layers) + lm
 
     def step(self, gpu, b: StackBuffers, hooks=None) -> None:
         """One token step (all layers, then the lm_head) on b, eagerly."""
         hk = lambda name: getattr(hooks, name, None) if hooks is not None else None
         pre, att, post, fin, after = hk("pre_attention"), hk("attention"), hk("post_attention"), hk("final"), hk("after_logits")
-        m = b.batch
+        m, filled = b.batch, getattr(hooks, "fills_rows", False)
         for i, L in enumerate(self.layers):
             b.select(i)
             if pre:
                 pre(i, b)
+            if L.fp8:
+                if not filled:
+                    fp8_quant(gpu, b.x, b.x8)
+                fp8_gemm(gpu, b.x8, L.qkv, b.qkv)
+                if att:
+                    att(i, b)
+                fp8_quant(gpu, b.attn, b.attn8)
+                fp8_gemm(gpu, b.attn8, L.o, b.o)
+                if post:
+                    post(i, b)
+                if not filled:
+                    fp8_quant(gpu, b.xm, b.xm8)
+                L._mlp(gpu, b.xm8, b.gate_up, b.h8, b.down)
+                continue
             _mv(gpu, "qkv_proj", b.x, L.qkv, b.qkv)
             if att:
                 att(i, b)
@@ -374,6 +485,10 @@ class DecoderStack:
         lm = self.lm_head
         if isinstance(lm, GptqWeight):
             _mv(gpu, "lm_head", b.x, lm, b.logits)
+        elif isinstance(lm, Fp8Weight):
+            if not filled:
+                fp8_quant(gpu, b.x, b.x8)
+            fp8_gemm(gpu, b.x8, lm, b.logits)
         else:
             for r0 in range(0, m, _BF16_BLOCK):
                 r1 = min(m, r0 + _BF16_BLOCK)

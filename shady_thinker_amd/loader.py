@@ -1,4 +1,5 @@
-"""GPTQ safetensors checkpoints -> device weights for this backend.
+"""Safetensors checkpoints, GPTQ and e4m3 with block scales, -> device weights
+for this backend.
 
 Mirrors the reference loader for the quantized linears (`load_weights`,
 src/weights.rs:315-547): every `*.safetensors` shard in the model directory
@@ -16,6 +17,10 @@ non-act-order files, this loader honours both:
 Files are read with the safetensors library (no pickle). Only GPTQ linears
 and bf16 2-D weights named like the lm_head / embeddings are returned; norms,
 attention and the rest are outside this path.
+
+`load_fp8_checkpoint` reads block-scaled 8-bit files (no reference
+counterpart): `{prefix}.weight` in float8_e4m3fn with `{prefix}.weight_scale_inv`
+for each 128 x 128, the block size config.json's quantization_config says.
 """
 from __future__ import annotations
 
@@ -26,7 +31,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from .weights import GptqWeight, QuantConfig, check_gptq_tensors
+from .weights import FP8_BLOCK, Fp8Weight, GptqWeight, QuantConfig, check_gptq_tensors
 
 _GPTQ_PARTS = ("qweight", "scales", "qzeros", "g_idx")
 
@@ -117,4 +122,40 @@ def load_gptq_checkpoint(gpu, model_dir: str, tiled: bool = True) -> tuple[dict,
                                           tiled=tiled)
     torch = gpu.torch
     bf16 = {name: torch.from_numpy(w.view(np.int16)).to(gpu.device) for name, w in ck.bf16.items()}
+    return linears, bf16
+
+
+def load_fp8_checkpoint(gpu, model_dir: str) -> tuple[dict, dict]:
+    """Upload every e4m3 linear with block scales (`{prefix: Fp8Weight}`) and
+    the bf16 lm_head / embedding weights (`{name: device int16 tensor [N, K]}`)."""
+    import torch
+    from safetensors import safe_open
+
+    path = os.path.join(model_dir, "config.json")
+    if os.path.exists(path):
+        with open(path) as f:
+            block = json.load(f).get("quantization_config", {}).get("weight_block_size", [FP8_BLOCK] * 2)
+        if list(block) != [FP8_BLOCK] * 2:
+            raise ValueError(f"config.json: weight_block_size {block}, only {[FP8_BLOCK] * 2} is supported")
+    weights, scales, bf16 = {}, {}, {}
+    for shard in _shards(model_dir):
+        with safe_open(shard, framework="pt") as f:
+            for name in f.keys():
+                stem, _, part = name.rpartition(".")
+                if part == "weight_scale_inv":
+                    scales[stem] = f.get_tensor(name)
+                elif part == "weight":
+                    kind = f.get_slice(name).get_dtype()
+                    if kind == "F8_E4M3":
+                        weights[stem] = f.get_tensor(name)
+                    elif kind == "BF16" and ("lm_head" in stem or "embed_tokens" in stem):
+                        bf16[name] = f.get_tensor(name).view(torch.int16).to(gpu.device)
+    if set(weights) != set(scales):
+        raise ValueError(f"{sorted(set(weights) ^ set(scales))[0]}: needs both weight (float8_e4m3fn) and weight_scale_inv")
+    linears = {}
+    for stem, w in weights.items():
+        try:
+            linears[stem] = Fp8Weight.upload(gpu, w, scales[stem])
+        except (ValueError, TypeError) as e:
+            raise type(e)(f"{stem}: {e}") from None
     return linears, bf16

@@ -188,3 +188,65 @@ GEMM = dict(ctx=CTX, x=P, x_scale=P, scale_stride=M, w=P, w_scale=P, y=P, y_dtyp
     (dict(w=ODD), ST_ERR_ALIGN), (dict(y=ODD), ST_ERR_ALIGN), (dict(x_scale=4097), ST_ERR_ALIGN), (dict(w_scale=4098), ST_ERR_ALIGN)])
 def test_c_gemm(kw, rc):
     assert st("st_fp8_gemm", *{**GEMM, **kw}.values()) == rc
+
+
+# ------------------------------------------------------- layers and checkpoints
+def parts(h=256, q=256, kv=128, i=384):
+    mk = lambda n, k: weight(n, k)
+    return dict(q=mk(q, h), k=mk(kv, h), v=mk(kv, h), o=mk(h, q), gate=mk(i, h), up=mk(i, h), down=mk(h, i))
+
+
+def test_layer_construction():
+    layer = sta.Fp8DecoderLinears(**parts())
+    assert (layer.qkv.N, layer.splits, layer.gate_up.N, layer.hidden, layer.inter, layer.attn_dim) == (512, (256, 128, 128), 768, 256, 384, 256)
+    assert layer.nbytes() > 0
+    for name, w in (("k", weight(128, 272)), ("o", weight(272, 256)), ("up", weight(256, 256)), ("down", weight(256, 400)), ("q", weight(64, 256))):
+        with pytest.raises(ValueError):
+            sta.Fp8DecoderLinears(**{**parts(), name: w})
+
+
+def test_layer_by_names():
+    names = {"q": "self_attn.q_proj", "k": "self_attn.k_proj", "v": "self_attn.v_proj", "o": "self_attn.o_proj", "gate": "mlp.gate_proj",
+             "up": "mlp.up_proj", "down": "mlp.down_proj"}
+    linears = {f"model.layers.3.{names[n]}": w for n, w in parts().items()}
+    assert isinstance(sta.layer_from_linears(linears, 3), sta.Fp8DecoderLinears)
+    linears.pop("model.layers.3.mlp.up_proj")
+    with pytest.raises(KeyError):
+        sta.layer_from_linears(linears, 3)
+
+
+def test_stack_refusals():
+    layer = sta.Fp8DecoderLinears(**parts())
+    with pytest.raises(ValueError):
+        sta.DecoderStack([layer], weight(100, 272))
+    with pytest.raises(ValueError):
+        sta.DecoderStack([layer, sta.Fp8DecoderLinears(**parts(i=256))], weight(100, 256))
+    stack = sta.DecoderStack([layer], weight(100, 256))
+    with pytest.raises(ValueError):
+        sta.ResidualNorms().init_norms(G, stack, 1, [], [torch.ones(256)], torch.ones(256))
+    with pytest.raises(NotImplementedError):
+        sta.ResidualNorms().embed(None)
+
+
+def save(path, tensors, config=None):
+    import json
+
+    from safetensors.torch import save_file
+
+    save_file(tensors, path / "model.safetensors")
+    if config is not None:
+        (path / "config.json").write_text(json.dumps(config))
+
+
+def test_checkpoint_refusals(tmp_path):
+    w, s = weight_of(torch.randn(40, 144))
+    good = {"a.weight": w, "a.weight_scale_inv": s}
+    save(tmp_path, good, {"quantization_config": {"weight_block_size": [128, 128]}})
+    linears, bf16 = sta.load_fp8_checkpoint(G, str(tmp_path))
+    assert list(linears) == ["a"] and torch.equal(linears["a"].w.float(), w.float()) and not bf16
+    for bad, config in (({"a.weight": w}, None), ({"a.weight_scale_inv": s}, None), ({**good, "a.weight_scale_inv": s[:, :1].contiguous()}, None),
+                        (good, {"quantization_config": {"weight_block_size": [64, 128]}}), ({**good, "a.weight_scale_inv": s.half()}, None)):
+        (tmp_path / "config.json").unlink(missing_ok=True)
+        save(tmp_path, bad, config)
+        with pytest.raises((ValueError, TypeError)):
+            sta.load_fp8_checkpoint(G, str(tmp_path))
