@@ -216,98 +216,236 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float *part, void *y,
 // middle of the block), their places take block b + 2, the second half's at the
 // end, so that a DMA has 1 to 1.4 blocks' time (all of it after the end: 0.6 to
 // 0.9; 4096 x 4096 x 22016 373 -> 354 us).
+//
+// A workgroup for each CU takes tiles until none is left, and their blocks of k
+// are one stream: the next tile's first blocks come during the last ones of
+// this, and its products run while y is on its way. The tiles that are left for
+// the last round are halved along the tokens where that gives every CU one.
+// Against a workgroup a tile: 4096 x 4096 x 22016 (5.4 tiles a CU) 353 -> 333 us,
+// 512 x 11008 x 4096 108 -> 98, 4096 x 11008 x 4096 (exactly one) 158 -> 161,
+// 8192^3 (four) 445 -> 455: the stream costs some 2 % where the tiles come out even.
 constexpr int WIDE = 256;
+
+struct Item {
+    int m0, n0, rows;  // rows 0: none
+};
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }  // (a quotient comes from the vector unit)
+
 __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
     constexpr int WM = 4, WN = 2, W = WM * WN, MT = WIDE / WM / 16, NT = WIDE / WN / 16, HN = WIDE / WN / 2;
     constexpr int DX = WIDE / 8 / W, DW = WIDE / 16 / W;  // DMAs (8 rows) of a wave: of x, of each half of w
     constexpr int STEPS = MT * NT, MID = STEPS / 2, LAST = MT * (NT - 1);
     static_assert(MID + DX + DW < LAST && DW < MT, "a block's DMAs fit between its barriers");
-    __shared__ __align__(1024) uint8_t x0[WIDE * kBlock], x1[WIDE * kBlock];
-    __shared__ __align__(1024) uint8_t wa0[WIDE / 2 * kBlock], wa1[WIDE / 2 * kBlock], wb0[WIDE / 2 * kBlock], wb1[WIDE / 2 * kBlock];
+    // two places each for x and the halves of w
+    constexpr int XP = WIDE * kBlock, WP = WIDE / 2 * kBlock, X0 = 0, X1 = XP, A0 = 2 * XP, A1 = A0 + WP, B0 = A1 + WP, B1 = B0 + WP;
+    __shared__ __align__(1024) uint8_t lds[B1 + WP];
+    __shared__ __align__(16) float sx[2][W][64], sw[2][W][64];  // scales: of two blocks each wave's tokens', of two runs of 64 blocks w's
+    __shared__ __align__(1024) half8 turn_of[W][8 * 16];  // eight tokens of a wave's 128 columns, on their way to y
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
-    const int KB = (a.K + kBlock - 1) / kBlock;
-    const Place at = place<WIDE, WIDE>(a, 1);
-    const int m0 = at.m0, n0 = at.n0;
-    const int wm0 = wave % WM * (WIDE / WM), wn = wave / WM, wn0 = wn * (WIDE / WN);
-    const int rows_x = min(WIDE, a.M - m0), rows_w = min(WIDE, a.N - n0);
-    const __amdgpu_buffer_rsrc_t rx = rows_of(a.x, m0, rows_x, a.K), rw = rows_of(a.w, n0, rows_w, a.K);
+    const int KB = (a.K + kBlock - 1) / kBlock;  // (at least 2)
+    // (waves w and w + 4 share a SIMD: of half a tile each SIMD has one)
+    const int wn = wave % WN, wm0 = wave / WN * (WIDE / WM), wn0 = wn * (WIDE / WN);
+
+    // This workgroup's tiles: an XCD takes a run of them, its CUs one after the other.
+    const int tm = (a.M + WIDE - 1) / WIDE, tn = (a.N + WIDE - 1) / WIDE, tiles = tm * tn;
+    const int xcd = blockIdx.x % 8, slot = blockIdx.x / 8, slots = gridDim.x / 8;
+    const int mine = tiles / 8 + (xcd < tiles % 8 ? 1 : 0), base = xcd * (tiles / 8) + min(xcd, tiles % 8);
+    const int full = uniform(mine / slots), left = mine - full * slots;
+    const bool halves = 2 * left <= slots;
+    const int items = full + (slot < (halves ? 2 * left : left) ? 1 : 0);
+    auto item = [&](int i) {
+        if (i >= items) return Item{0, 0, 0};
+        const bool half = i == full && halves;
+        const int tile = base + i * slots + (half ? slot / 2 : slot);
+        const int panel = uniform(tile / (kPanel * tn)), at = tile - panel * kPanel * tn, wide = min(kPanel, tm - panel * kPanel);
+        const int column = uniform(at / wide), m0 = (panel * kPanel + at - column * wide) * WIDE + (half ? slot % 2 * (WIDE / 2) : 0);
+        return Item{m0, column * WIDE, max(min(half ? WIDE / 2 : WIDE, a.M - m0), 0)};
+    };
+
+    // What the DMAs read: a lane's first row of x, and of w (each wave column's
+    // first 64 rows are the first half); rows past the tile's last lie outside the resources.
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    int vx[DX], va[DW], vb[DW];
-#pragma unroll
-    for (int j = 0; j < DX; ++j) vx[j] = min((wave * DX + j) * 8 + (lane >> 3), rows_x - 1) * a.K + chunk;
-#pragma unroll
-    for (int j = 0; j < DW; ++j) {  // (each wave column's first 64 rows, and its last)
-        const int l = (wave * DW + j) * 8, row = l / HN * (2 * HN) + l % HN + (lane >> 3);
-        va[j] = min(row, rows_w - 1) * a.K + chunk;
-        vb[j] = min(row + HN, rows_w - 1) * a.K + chunk;
-    }
-    auto dma_x = [&](uint8_t *s, int b, int j) { dma16(rx, s + (wave * DX + j) * 1024, b * kBlock + chunk < a.K ? vx[j] : kOutside, b * kBlock); };
-    auto dma_a = [&](uint8_t *s, int b, int j) { dma16(rw, s + (wave * DW + j) * 1024, b * kBlock + chunk < a.K ? va[j] : kOutside, b * kBlock); };
-    auto dma_b = [&](uint8_t *s, int b, int j) { dma16(rw, s + (wave * DW + j) * 1024, b * kBlock + chunk < a.K ? vb[j] : kOutside, b * kBlock); };
-    const float *const sw = a.sw + (int64_t)min((n0 + wn0) / kBlock, (a.N - 1) / kBlock) * KB;
-    const float *sx[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) sx[t] = a.sx + min(m0 + wm0 + 16 * t + r, a.M - 1);
+    int vx, vw;
+    Rsrc rx, rw;
+    const unsigned part_x = lds_at(lds + wave * DX * 1024), part_w = lds_at(lds + wave * DW * 1024);  // the wave's part of a place
+    unsigned lds_x = part_x, lds_w = part_w;
+    auto point = [&](Item t) {
+        vx = vw = kOutside;
+        if (t.rows == 0) return;  // (the resources stay: an offset is outside only while they hold the uniform offset)
+        rx = rsrc(a.x + (int64_t)t.m0 * a.K, t.rows * a.K), rw = rsrc(a.w + (int64_t)t.n0 * a.K, min(WIDE, a.N - t.n0) * a.K);
+        const int l = wave * DW * 8;
+        vx = (wave * DX * 8 + (lane >> 3)) * a.K + chunk;
+        vw = (l / HN * (2 * HN) + l % HN + (lane >> 3)) * a.K + chunk;
+        settle(rx, rw);
+    };
+    static_assert(HN % (DW * 8) == 0, "a wave's rows of w are neighbours");
+    auto dma = [&](Rsrc rs, unsigned to, int v, int b) { lds16(rs, to, b * kBlock + chunk < a.K ? v : kOutside, b * kBlock); };
+    auto dma_x = [&](int to, int b, int j) { dma(rx, lds_x + to + j * 1024, vx + j * 8 * a.K, b); };
+    auto dma_a = [&](int to, int b, int j) { dma(rw, lds_w + to + j * 1024, vw + j * 8 * a.K, b); };
+    auto dma_b = [&](int to, int b, int j) { dma(rw, lds_w + to + j * 1024, vw + (HN + j * 8) * a.K, b); };
+    // The scales of block b of a tile: its wave's 64 tokens' to sx[q]; at the first
+    // of 64 blocks w's of all of them to the other half of sw.
+    int half = 1;
+    auto load_scales = [&](Item t, int b, int q) {
+        const int rows = max(min(a.M - t.m0, WIDE), 1), nb = min((t.n0 + wn0) / kBlock, (a.N - 1) / kBlock);
+        lds4(rsrc(a.sx + b * a.sx_stride + t.m0, rows * 4), lds_at(sx[q][wave]), (wm0 + lane) * 4);
+        if (b % 64 == 0) {
+            half ^= 1;
+            lds4(rsrc(a.sw + (int64_t)nb * KB + b, min(KB - b, 64) * 4), lds_at(sw[half][wave]), lane * 4);
+        }
+    };
     float f[MT], fn[MT], gn;
-    auto load_scales = [&](int b) {
+    auto read_scales = [&](int b, int q) {
+        gn = sw[half][wave][b % 64];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) fn[t] = sx[t][b * a.sx_stride];
-        gn = sw[b];
+        for (int t = 0; t < MT; ++t) fn[t] = sx[q][wave][16 * t + r];
+    };
+    auto take_scales = [&] {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
     };
     const int pos = r * kBlock + (c ^ (r & 7)) * 16;
-    auto frag = [&](const uint8_t *s, int row) {
+    auto frag = [&](int from, int row) {
+        const uint8_t *const s = lds + from + row * kBlock;
         Frag<false> v;
-        v.set(*reinterpret_cast<const i32x4 *>(s + row * kBlock + pos), *reinterpret_cast<const i32x4 *>(s + row * kBlock + (pos ^ 64)));
+        v.set(*reinterpret_cast<const i32x4 *>(s + pos), *reinterpret_cast<const i32x4 *>(s + (pos ^ 64)));
         return v;
     };
     f32x4 acc[MT][NT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0, 0, 0, 0};
     Frag<false> xf[MT], wf[2];
-    // Block b from xs, was, wbs, whose first fragments are read, then those of
-    // b + 1 from xn and wan; block b + 2 to b's places.
-    auto block = [&](uint8_t *xs, uint8_t *was, uint8_t *wbs, const uint8_t *xn, const uint8_t *wan, int b) {
-        f32x4 p[D + 1];
-        const int b2 = min(b + 2, KB - 1);  // (past the end: the last again, unused)
-        load_scales(min(b + 1, KB - 1));
+    Item now = item(0);
+    if (now.rows == 0) return;  // (the whole workgroup)
+    int i_item = 0, b = 0;
+    bool active = wm0 < now.rows;
+    auto clear = [&] {
 #pragma unroll
-        for (int i = 0; i < STEPS + D; ++i) {
-            const int u = i / MT, t = i % MT;
-            if (i < STEPS) {
-                if (t == 0) {
-                    if (i == MID) {  // everyone has read x and the first half of w
-                        wait_lds();
-                        __builtin_amdgcn_s_barrier();
-                    }
-                    if (u == NT - 1) {  // everyone has read the rest, and b + 1 has come
-                        wait_loads<DX + DW, true>();
-                        __builtin_amdgcn_s_barrier();
-                        wf[(u + 1) & 1] = frag(wan, wn * HN);
-                    } else {
-                        wf[(u + 1) & 1] = u + 1 < NT / 2 ? frag(was, wn * HN + 16 * (u + 1)) : frag(wbs, wn * HN + 16 * (u + 1 - NT / 2));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                p[i % (D + 1)] = mfma(wf[u & 1], xf[t]);
-                if (i > MID && i - MID - 1 < DX) dma_x(xs, b2, i - MID - 1);
-                if (i > MID + DX && i - MID - DX - 1 < DW) dma_a(was, b2, i - MID - DX - 1);
-                if (i > LAST && i - LAST - 1 < DW) dma_b(wbs, b2, i - LAST - 1);
-                if (u == NT - 1) xf[t] = frag(xn, wm0 + 16 * t);
-            }
-            if (i >= D) {
-                const int j = i - D;
-                acc[j % MT][j / MT] += p[j % (D + 1)] * f[j % MT];
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0, 0, 0, 0};
+    };
+
+    // Block b from xs, was, wbs, whose first fragments are read, then the next
+    // block's from xn and wan; the one after that to b's places.
+    auto block = [&](int q, int xs, int was, int wbs, int xn, int wan) {
+        int b2 = b + 2;
+        if (b2 >= KB) {
+            b2 -= KB;
+            if (b2 == 0) point(item(i_item + 1));
         }
+        lds_x = part_x, lds_w = part_w;
+        asm volatile("" : "+s"(lds_x), "+s"(lds_w));  // (added to where they are used: 24 places are too many to keep)
+        const bool last = b + 1 == KB;
+        auto next_scales = [&] { load_scales(last ? item(i_item + 1) : now, last ? 0 : b + 1, q ^ 1); };
+        if (active) {
+            f32x4 p[D + 1];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+            for (int i = 0; i < STEPS + D; ++i) {
+                const int u = i / MT, t = i % MT;
+                if (i < STEPS) {
+                    if (t == 0) {
+                        if (i == MID) {  // everyone has read x and the first half of w
+                            wait_lds();
+                            __builtin_amdgcn_s_barrier();
+                        }
+                        if (u == NT - 1) {  // everyone has read the rest, and the next block has come
+                            wait_loads<DX + DW, true>();
+                            __builtin_amdgcn_s_barrier();
+                            read_scales(last ? 0 : b + 1, q ^ 1);
+                            wf[(u + 1) & 1] = frag(wan, wn * HN);
+                        } else {
+                            wf[(u + 1) & 1] = u + 1 < NT / 2 ? frag(was, wn * HN + 16 * (u + 1)) : frag(wbs, wn * HN + 16 * (u + 1 - NT / 2));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    p[i % (D + 1)] = mfma(wf[u & 1], xf[t]);
+                    if (i == 1) next_scales();
+                    if (i > MID && i - MID - 1 < DX) dma_x(xs, b2, i - MID - 1);
+                    if (i > MID + DX && i - MID - DX - 1 < DW) dma_a(was, b2, i - MID - DX - 1);
+                    if (i > LAST && i - LAST - 1 < DW) dma_b(wbs, b2, i - LAST - 1);
+                    if (u == NT - 1) xf[t] = frag(xn, wm0 + 16 * t);
+                }
+                if (i >= D) {
+                    const int j = i - D;
+                    acc[j % MT][j / MT] += p[j % (D + 1)] * f[j % MT];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {  // (none of the wave's rows are in the tile)
+            next_scales();
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+            settle(rx, rw);
+#pragma unroll
+            for (int j = 0; j < DX; ++j) dma_x(xs, b2, j);
+#pragma unroll
+            for (int j = 0; j < DW; ++j) dma_a(was, b2, j);
+            wait_loads<DX + DW, true>();
+            __builtin_amdgcn_s_barrier();
+            settle(rx, rw);
+#pragma unroll
+            for (int j = 0; j < DW; ++j) dma_b(wbs, b2, j);
+            read_scales(last ? 0 : b + 1, q ^ 1);
+            wf[0] = frag(wan, wn * HN);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xf[t] = frag(xn, wm0 + 16 * t);
+        }
+        take_scales();
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto load = [&](uint8_t *xs, uint8_t *was, uint8_t *wbs, int b) {
+    // y of the tile: eight tokens at a time turned in LDS, so that 16 lanes write
+    // a token's 256 bytes (chunk j of token m at j ^ 2 m; as the lanes hold them,
+    // four neighbours each, a store went one lane at a time).
+    auto write = [&] {
+        const bool whole = now.n0 + wn0 + WIDE / WN <= a.N && a.N % 8 == 0;
+        half8 *const s = turn_of[wave];
+        int r = lane & 15, c = lane >> 4;
+        asm volatile("" : "+v"(r), "+v"(c));  // (its addresses do not wait in registers through the blocks)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int m = now.m0 + wm0 + 16 * t;
+            const int rows = min(now.rows - wm0 - 16 * t, 16);
+            if (whole) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (r / 8 == h)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u) {
+                            const f32x4 v = acc[t][u];
+                            reinterpret_cast<half4 *>(s + r % 8 * 16 + ((2 * u + c / 2) ^ (2 * (r % 8))))[c & 1] =
+                                half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+                        }
+                    wait_lds();
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int row = 4 * j + c;
+                        const half8 v = s[row * 16 + (r ^ (2 * row))];
+                        if (8 * h + row < rows)
+                            *reinterpret_cast<half8 *>(static_cast<_Float16 *>(a.y) + (int64_t)(m + 8 * h + row) * a.N + now.n0 + wn0 + 8 * r) = v;
+                    }
+                    wait_lds();
+                }
+            } else if (r < rows) {
+#pragma unroll
+                for (int u = 0; u < NT; ++u) store_n4(a.y, false, m + r, now.n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
+            }
+        }
+    };
+    // After a block: whether it was the last of all.
+    auto done = [&] {
+        if (++b < KB) return false;
+        if (active) write();
+        if (++i_item == items) return true;
+        now = item(i_item);
+        if (now.rows == 0) return true;  // (half a tile past the last token)
+        active = wm0 < now.rows;
+        b = 0;
+        clear();
+        return false;
+    };
+
+    point(now);
+    auto load = [&](int xs, int was, int wbs, int b) {
 #pragma unroll
         for (int j = 0; j < DX; ++j) dma_x(xs, b, j);
 #pragma unroll
@@ -315,28 +453,25 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
 #pragma unroll
         for (int j = 0; j < DW; ++j) dma_b(wbs, b, j);
     };
-    load_scales(0);
-    load(x0, wa0, wb0, 0);
-    load(x1, wa1, wb1, min(1, KB - 1));
+    load_scales(now, 0, 0);
+    settle(rx, rw);
+    load(X0, A0, B0, 0);
+    load(X1, A1, B1, 1);
+    clear();
     wait_loads<DX + 2 * DW, true>();
     __builtin_amdgcn_s_barrier();
+    read_scales(0, 0);
+    take_scales();
+    wf[0] = frag(A0, wn * HN);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
-    wf[0] = frag(wa0, wn * HN);
-#pragma unroll
-    for (int t = 0; t < MT; ++t) xf[t] = frag(x0, wm0 + 16 * t);
-    for (int b = 0; b < KB; b += 2) {
-        block(x0, wa0, wb0, x1, wa1, b);
-        if (b + 1 < KB) block(x1, wa1, wb1, x0, wa0, b + 1);
+    for (int t = 0; t < MT; ++t) xf[t] = frag(X0, wm0 + 16 * t);
+    while (true) {
+        block(0, X0, A0, B0, X1, A1);
+        if (done()) break;
+        block(1, X1, A1, B1, X0, A0);
+        if (done()) break;
     }
-    wait_loads<0, true>();
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + wm0 + 16 * t + r;
-        if (m < a.M)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) store_n4(a.y, false, m, n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
-    }
+    wait_loads<0, true>();  // (no DMA after the wave's end)
 }
 
 // ------------------------------------------------------------------ the choice
@@ -367,7 +502,8 @@ Plan plan(const st_context *ctx, const MmArgs &a) {
     if (can_mv && (forced == MV || (forced < 0 && a.M <= 32))) return best;
     double least = can_mv ? mv_us(ctx, a) : 1e30;
     const int KB = blocks(a.K);
-    auto built = [&](const Tile &t) { return (exact ? t.block16 : t.block8) != 0; };
+    // (the 256 x 256 kernel brings two blocks of K at once)
+    auto built = [&](const Tile &t) { return (exact ? t.block16 : t.block8) != 0 && (t.kind != R256x256 || KB > 1); };
     bool force = false;
     for (const Tile &t : kTiles) force |= t.kind == forced && built(t);
     if (force) least = 1e30;
@@ -408,8 +544,7 @@ int run(st_context *ctx, const MmArgs &a, Plan p) {
         case R128x256: run_ring<128, 256, 4, 2, 3, false>(ctx, a, p.splits); break;
         case R256x128: run_ring<256, 128, 4, 2, 3, true>(ctx, a, p.splits); break;
         case R256x256: {
-            const dim3 grid((unsigned)((a.M + WIDE - 1) / WIDE * ((a.N + WIDE - 1) / WIDE)));
-            st::launch(ctx, wide_kernel, grid, dim3(512), 0, a);
+            st::launch(ctx, wide_kernel, dim3((unsigned)(std::max(ctx->num_cus, 8) / 8 * 8)), dim3(512), 0, a);
             name = "fp8_wide_kernel";
         }
     }

@@ -59,6 +59,35 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t *lds, in
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, voff, soff, 0, 0);
 }
 
+// A buffer resource (uniform) and loads from it to LDS by assembly: of the
+// builtin's loads in flight the compiler does not know which part of LDS each
+// fills, so before reads of any it waits for more than it must. Nothing is
+// written to registers; wait_loads says when they have come, and a loop with
+// these has no other vector loads (whose waits would count them) and no other
+// use of m0. A resource that may come out of the vector unit (a lane it was kept
+// in) needs five wait states before it is read: settle().
+typedef i32x4 Rsrc;
+__device__ __forceinline__ Rsrc scalar(Rsrc r) {
+    return Rsrc{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y), __builtin_amdgcn_readfirstlane(r.z), kRsrcWord3};
+}
+__device__ __forceinline__ Rsrc rsrc(const void *p, unsigned bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    return scalar(Rsrc{(int)(unsigned)at, (int)(unsigned)((at >> 32) & 0xFFFF), (int)bytes, kRsrcWord3});
+}
+__device__ __forceinline__ unsigned lds_at(const void *p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+__device__ __forceinline__ void settle(Rsrc &a, Rsrc &b) {
+    a = scalar(a), b = scalar(b);
+    asm volatile("s_nop 4" : "+s"(a), "+s"(b));
+}
+__device__ __forceinline__ void lds16(Rsrc r, unsigned lds, int voff, int soff) {  // (r settled)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+}
+__device__ __forceinline__ void lds4(Rsrc r, unsigned lds, int voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(scalar(r)) : "memory");
+}
+
 // s_waitcnt: at most n vector loads in flight (LDS reads too: none).
 template <int N, bool LDS>
 __device__ __forceinline__ void wait_loads() {

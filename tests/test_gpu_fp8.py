@@ -211,11 +211,14 @@ def test_gemm(gpu, m, k, n, dtype):
 def tile_cases():
     """(tile, slices, m, k, n, dtype) of every tile that is built for the type."""
     sizes = [(33, 16, 1), (64, 400, 65), (65, 128, 3), (100, 1424, 260), (128, 144, 128), (255, 272, 257), (300, 528, 1000), (513, 2064, 129),
-             (1600, 384, 300)]
+             (1600, 384, 300), (700, 256, 1300), (2300, 400, 2568)]
     for m, k, n in sizes:
         for dtype in (F32, F16):
             for tile in (1, 2, 3, 4, 6) if dtype is F32 or m <= 64 else (3, 4, 5, 7):
-                yield from ((tile, s, m, k, n, dtype) for s in ((1, 2, 8) if tile != 7 else (1,)))
+                if tile != 7:
+                    yield from ((tile, s, m, k, n, dtype) for s in (1, 2, 8))
+                elif k > B:  # (the 256 x 256 kernel: two blocks of K at least, no slices)
+                    yield tile, 1, m, k, n, dtype
 
 
 @pytest.mark.parametrize("tile,splits,m,k,n,dtype", tile_cases())
