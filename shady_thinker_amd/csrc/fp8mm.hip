@@ -50,21 +50,56 @@ __device__ __forceinline__ Place place(const MmArgs &a, int splits) {
     return {(panel * kPanel + at % wide) * BM, at / wide * BN, split};
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint8_t *p, int row0, int rows, int K) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)(p + (int64_t)row0 * K), (short)0, rows * K, kRsrcWord3);
+// 16 tokens' sums (16 NT columns of a wave) to y, turned in LDS R tokens at a
+// time, so that neighbouring lanes write a row's 16-byte chunks; as the lanes
+// hold them, four neighbours each, a store went one lane at a time (4096 x 4096 x
+// 22016 in tiles of 128 x 256: 387 -> 366 us). Chunk j of row r is at j ^ (r %
+// chunks). (N a multiple of 16 bytes.)
+template <typename T, int R, int NT>
+__device__ __forceinline__ void turned(i32x4 *s, const f32x4 (&v)[NT], T *y, int m, int rows, int n, int N) {
+    constexpr int PER = 16 / sizeof(T), CHUNKS = 16 * NT / PER, ROWS = 64 / CHUNKS;
+    static_assert(CHUNKS <= 64 && R % ROWS == 0, "whole rows");
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (its addresses do not wait in registers through the blocks)
+    const int r = lane & 15, c = lane >> 4, j = lane % CHUNKS;
+#pragma unroll
+    for (int h = 0; h < 16; h += R) {
+        if (r / R * R == h) {
+            const int row = r - h;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                if constexpr (sizeof(T) == 4)
+                    reinterpret_cast<f32x4 *>(s)[row * CHUNKS + ((4 * u + c) ^ (row % CHUNKS))] = v[u];
+                else
+                    reinterpret_cast<half4 *>(s + row * CHUNKS + ((2 * u + c / 2) ^ (row % CHUNKS)))[c & 1] =
+                        half4{(_Float16)v[u].x, (_Float16)v[u].y, (_Float16)v[u].z, (_Float16)v[u].w};
+            }
+        }
+        wait_lds();
+#pragma unroll
+        for (int i = 0; i < R; i += ROWS) {
+            const int row = i + lane / CHUNKS;
+            const i32x4 w = s[row * CHUNKS + (j ^ (row % CHUNKS))];
+            if (h + row < rows && n + j * PER < N) *reinterpret_cast<i32x4 *>(y + (int64_t)(m + h + row) * N + n + j * PER) = w;
+        }
+        wait_lds();
+    }
 }
 
 // ------------------------------------------------------------------ a ring
 // BM x BN of y by WM x WN waves, S stages of LDS, K in slices where the tiles
 // alone leave CUs idle (f32 partial sums in the workspace, added in order by
-// reduce_kernel). Block b + S - 1 comes while b is multiplied.
+// reduce_kernel). Block b + S - 1 comes while b is multiplied. What bounds it is
+// the DMAs' way from the L2s (14 to 17 TB/s of all CUs; without the products and
+// their reads 512 x 11008 x 4096 takes 28 us of 33).
 template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kernel(MmArgs a, float *part, int splits) {
     constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, STEPS = MT * NT;
     constexpr int DX = BM / 8 / W, DW = BN / 8 / W, ND = DX + DW;  // DMAs (8 rows) of a wave
     static_assert(DX * 8 * W == BM && DW * 8 * W == BN && NT % 2 == 0 && BN / WN <= kBlock, "whole DMAs, one scale a wave");
     constexpr int STAGE = (BM + BN) * kBlock;
-    __shared__ __align__(1024) uint8_t s0[STAGE], s1[STAGE], s2[STAGE], s3[S > 3 ? STAGE : 16];
+    __shared__ __align__(1024) uint8_t lds[S * STAGE];
+    __shared__ __align__(16) float sx[S][W][64], sw[2][W][64];  // scales: each wave's tokens', and the weight's of two runs of blocks
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
     const int KB = (a.K + kBlock - 1) / kBlock;
@@ -73,7 +108,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kerne
     const int b0 = (int)((int64_t)KB * at.split / splits), b1 = (int)((int64_t)KB * (at.split + 1) / splits);
     const int wm0 = wave % WM * (BM / WM), wn0 = wave / WM * (BN / WN);
     const int rows_x = min(BM, a.M - m0), rows_w = min(BN, a.N - n0);
-    const __amdgpu_buffer_rsrc_t rx = rows_of(a.x, m0, rows_x, a.K), rw = rows_of(a.w, n0, rows_w, a.K);
+    Rsrc rx = rsrc(a.x + (int64_t)m0 * a.K, rows_x * a.K), rw = rsrc(a.w + (int64_t)n0 * a.K, rows_w * a.K);
     // lane i of a DMA fills position i % 8 of its row i / 8; rows past the last repeat it
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     int vx[DX], vw[DW];
@@ -81,29 +116,40 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kerne
     for (int j = 0; j < DX; ++j) vx[j] = min((wave * DX + j) * 8 + (lane >> 3), rows_x - 1) * a.K + chunk;
 #pragma unroll
     for (int j = 0; j < DW; ++j) vw[j] = min((wave * DW + j) * 8 + (lane >> 3), rows_w - 1) * a.K + chunk;
-    auto dma = [&](uint8_t *s, int b, int j) {
+    const unsigned part_x = lds_at(lds + wave * DX * 1024), part_w = lds_at(lds + BM * kBlock + wave * DW * 1024);
+    unsigned lds_x = part_x, lds_w = part_w;  // the wave's part of stage 0
+    auto dma = [&](int s, int b, int j) {
         const bool in = b * kBlock + chunk < a.K;  // (K ends inside the last block: zeros)
         if (j < DW)
-            dma16(rw, s + BM * kBlock + (wave * DW + j) * 1024, in ? vw[j] : kOutside, b * kBlock);
+            lds16(rw, lds_w + s * STAGE + j * 1024, in ? vw[j] : kOutside, b * kBlock);
         else
-            dma16(rx, s + (wave * DX + j - DW) * 1024, in ? vx[j - DW] : kOutside, b * kBlock);
+            lds16(rx, lds_x + s * STAGE + (j - DW) * 1024, in ? vx[j - DW] : kOutside, b * kBlock);
     };
-    auto load = [&](uint8_t *s, int b) {
+    auto load = [&](int s, int b) {
 #pragma unroll
         for (int j = 0; j < ND; ++j) dma(s, b, j);
     };
-    const float *const sw = a.sw + (int64_t)min((n0 + wn0) / kBlock, (a.N - 1) / kBlock) * KB;
-    const float *sx[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) sx[t] = a.sx + min(m0 + wm0 + 16 * t + r, a.M - 1);
+    // A block's scales of the tokens come with it (loads end in order: those asked
+    // for later would hold up the DMAs before them: 77 x 5120 x 13824 in tiles of
+    // 128 x 64 19.6 -> 16.9 us), the weight's of a run of blocks
+    // (and of the one after it) during the run before.
+    const int rows_s = max(min(a.M - m0 - wm0, 64), 1), nb = min((n0 + wn0) / kBlock, (a.N - 1) / kBlock);
+    const float *const sx0 = a.sx + min(m0 + wm0, a.M - 1);
+    auto load_scales = [&](int s, int b) { lds4(rsrc(sx0 + b * a.sx_stride, rows_s * 4), lds_at(sx[s][wave]), lane * 4); };
+    auto load_run = [&](int run, int half) { lds4(rsrc(a.sw + (int64_t)nb * KB + run, min(KB - run, 64) * 4), lds_at(sw[half][wave]), lane * 4); };
     float f[MT], fn[MT], gn;
-    auto load_scales = [&](int b) {
+    auto read_scales = [&](int s, int half, int at) {
+        gn = sw[half][wave][at];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) fn[t] = sx[t][b * a.sx_stride];
-        gn = sw[b];
+        for (int t = 0; t < MT; ++t) fn[t] = sx[s][wave][16 * t + r];
+    };
+    auto take_scales = [&] {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
     };
     const int pos = r * kBlock + (c ^ (r & 7)) * 16;
-    auto frag = [&](const uint8_t *s, int row) {
+    auto frag = [&](int from, int row) {
+        const uint8_t *const s = lds + from;
         Frag<EXACT> v;
         v.set(*reinterpret_cast<const i32x4 *>(s + row * kBlock + pos), *reinterpret_cast<const i32x4 *>(s + row * kBlock + (pos ^ 64)));
         return v;
@@ -114,33 +160,36 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kerne
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0, 0, 0, 0};
     Frag<EXACT> xf[MT], wf[2];
-    // Block b from s, whose first fragments are read, then those of b + 1 from
-    // `next`; block b + S - 1 to `to`, which held b - 1.
-    auto block = [&](const uint8_t *s, const uint8_t *next, uint8_t *to, int b) {
+    // Block b from stage s, whose first fragments are read, then those of b + 1
+    // from `next`; block b + S - 1 to `to`, which held b - 1.
+    auto block = [&](int s, int next, int to, int b, int run, int half) {
         f32x4 p[D + 1];
         const int bn = min(b + S - 1, b1 - 1);  // (past the end: the last again, unused)
-        load_scales(min(b + 1, b1 - 1));
+        lds_x = part_x, lds_w = part_w;
+        asm volatile("" : "+s"(lds_x), "+s"(lds_w));  // (added to where they are used)
 #pragma unroll
         for (int i = 0; i < STEPS + D; ++i) {
             const int u = i / MT, t = i % MT;
             if (i < STEPS) {
                 if (t == 0) {
                     if (u < NT - 1) {
-                        wf[(u + 1) & 1] = frag(s + BM * kBlock, wn0 + 16 * (u + 1));
+                        wf[(u + 1) & 1] = frag(s * STAGE + BM * kBlock, wn0 + 16 * (u + 1));
                     } else {
                         // this wave's last fragments of b are read and its part of b + 1 has
                         // come; after the barrier everyone's
-                        wait_loads<(S - 2) * ND, true>();
+                        wait_loads<(S - 2) * (ND + 1), true>();
                         __builtin_amdgcn_s_barrier();
-                        wf[(u + 1) & 1] = frag(next + BM * kBlock, wn0);
+                        read_scales(next, half, b + 1 - run);
+                        wf[(u + 1) & 1] = frag(next * STAGE + BM * kBlock, wn0);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 p[i % (D + 1)] = mfma(wf[u & 1], xf[t]);
+                if (i == 0) load_scales(to, bn);
 #pragma unroll
                 for (int j = 0; j < ND; ++j)
                     if (i == j * (STEPS - MT) / ND) dma(to, bn, j);
-                if (u == NT - 1) xf[t] = frag(next, wm0 + 16 * t);
+                if (u == NT - 1) xf[t] = frag(next * STAGE, wm0 + 16 * t);
             }
             if (i >= D) {
                 const int j = i - D;
@@ -148,42 +197,48 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kerne
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
+        take_scales();
         __builtin_amdgcn_sched_barrier(0);
     };
-    load_scales(b0);
-    load(s0, b0);
-    load(s1, min(b0 + 1, b1 - 1));
-    if constexpr (S > 3) load(s2, min(b0 + 2, b1 - 1));
-    wait_loads<(S - 2) * ND, true>();
+    settle(rx, rw);
+    load_run(b0, 0);
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+        load_scales(s, min(b0 + s, b1 - 1));
+        load(s, min(b0 + s, b1 - 1));
+    }
+    wait_loads<(S - 2) * (ND + 1), true>();
     __builtin_amdgcn_s_barrier();
+    read_scales(0, 0, 0);
+    take_scales();
+    wf[0] = frag(BM * kBlock, wn0);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) f[t] = fn[t] * gn;
-    wf[0] = frag(s0 + BM * kBlock, wn0);
+    for (int t = 0; t < MT; ++t) xf[t] = frag(0, wm0 + 16 * t);
+    constexpr int RUN = 48;
+    static_assert(RUN % S == 0 && RUN < 64, "whole turns of the ring; the next run's first is among the lanes");
+    for (int run = b0, half = 0; run < b1; run += RUN, half ^= 1) {
+        if (run + RUN < b1) load_run(run + RUN, half ^ 1);
+        for (int b = run; b < min(run + RUN, b1); b += S)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xf[t] = frag(s0, wm0 + 16 * t);
-    for (int b = b0; b < b1; b += S) {
-        if constexpr (S == 3) {
-            block(s0, s1, s2, b);
-            if (b + 1 < b1) block(s1, s2, s0, b + 1);
-            if (b + 2 < b1) block(s2, s0, s1, b + 2);
-        } else {
-            block(s0, s1, s3, b);
-            if (b + 1 < b1) block(s1, s2, s0, b + 1);
-            if (b + 2 < b1) block(s2, s3, s1, b + 2);
-            if (b + 3 < b1) block(s3, s0, s2, b + 3);
-        }
+            for (int s = 0; s < S; ++s)
+                if (b + s < b1) block(s, (s + 1) % S, (s + S - 1) % S, b + s, run, half);
     }
     wait_loads<0, true>();  // (no DMA after the wave's end)
     void *const out = splits > 1 ? part + (int64_t)at.split * a.M * a.N : a.y;
     const bool f32 = splits > 1 || a.f32;
+    __builtin_amdgcn_s_barrier();  // (the stages are read: each wave turns its sums there)
+    static_assert(S * STAGE >= W * 16 * NT * 64, "a place for each wave");
+    i32x4 *const turn = reinterpret_cast<i32x4 *>(lds) + wave * (NT * 64);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int m = m0 + wm0 + 16 * t + r;
-        if (m < a.M)
+        const int m = m0 + wm0 + 16 * t, n = n0 + wn0, rows = a.M - m;
+        if (f32 && a.N % 4 == 0)
+            turned<float, 16>(turn, acc[t], static_cast<float *>(out), m, rows, n, a.N);
+        else if (!f32 && a.N % 8 == 0)
+            turned<_Float16, 16>(turn, acc[t], static_cast<_Float16 *>(out), m, rows, n, a.N);
+        else if (r < rows)
 #pragma unroll
-            for (int u = 0; u < NT; ++u) store_n4(out, f32, m, n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
+            for (int u = 0; u < NT; ++u) store_n4(out, f32, m + r, n + 16 * u + 4 * c, a.N, acc[t][u]);
     }
 }
 
@@ -240,7 +295,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
     constexpr int XP = WIDE * kBlock, WP = WIDE / 2 * kBlock, X0 = 0, X1 = XP, A0 = 2 * XP, A1 = A0 + WP, B0 = A1 + WP, B1 = B0 + WP;
     __shared__ __align__(1024) uint8_t lds[B1 + WP];
     __shared__ __align__(16) float sx[2][W][64], sw[2][W][64];  // scales: of two blocks each wave's tokens', of two runs of 64 blocks w's
-    __shared__ __align__(1024) half8 turn_of[W][8 * 16];  // eight tokens of a wave's 128 columns, on their way to y
+    __shared__ __align__(1024) i32x4 turn_of[W][8 * 16];  // eight tokens of a wave's 128 columns, on their way to y
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
     const int KB = (a.K + kBlock - 1) / kBlock;  // (at least 2)
@@ -393,42 +448,16 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
         take_scales();
         __builtin_amdgcn_sched_barrier(0);
     };
-    // y of the tile: eight tokens at a time turned in LDS, so that 16 lanes write
-    // a token's 256 bytes (chunk j of token m at j ^ 2 m; as the lanes hold them,
-    // four neighbours each, a store went one lane at a time).
     auto write = [&] {
-        const bool whole = now.n0 + wn0 + WIDE / WN <= a.N && a.N % 8 == 0;
-        half8 *const s = turn_of[wave];
-        int r = lane & 15, c = lane >> 4;
-        asm volatile("" : "+v"(r), "+v"(c));  // (its addresses do not wait in registers through the blocks)
+        const int n = now.n0 + wn0;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int m = now.m0 + wm0 + 16 * t;
-            const int rows = min(now.rows - wm0 - 16 * t, 16);
-            if (whole) {
+            const int m = now.m0 + wm0 + 16 * t, rows = now.rows - wm0 - 16 * t;
+            if (a.N % 8 == 0)
+                turned<_Float16, 8>(turn_of[wave], acc[t], static_cast<_Float16 *>(a.y), m, rows, n, a.N);
+            else if (r < rows)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (r / 8 == h)
-#pragma unroll
-                        for (int u = 0; u < NT; ++u) {
-                            const f32x4 v = acc[t][u];
-                            reinterpret_cast<half4 *>(s + r % 8 * 16 + ((2 * u + c / 2) ^ (2 * (r % 8))))[c & 1] =
-                                half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
-                        }
-                    wait_lds();
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int row = 4 * j + c;
-                        const half8 v = s[row * 16 + (r ^ (2 * row))];
-                        if (8 * h + row < rows)
-                            *reinterpret_cast<half8 *>(static_cast<_Float16 *>(a.y) + (int64_t)(m + 8 * h + row) * a.N + now.n0 + wn0 + 8 * r) = v;
-                    }
-                    wait_lds();
-                }
-            } else if (r < rows) {
-#pragma unroll
-                for (int u = 0; u < NT; ++u) store_n4(a.y, false, m + r, now.n0 + wn0 + 16 * u + 4 * c, a.N, acc[t][u]);
-            }
+                for (int u = 0; u < NT; ++u) store_n4(a.y, false, m + r, n + 16 * u + 4 * c, a.N, acc[t][u]);
         }
     };
     // After a block: whether it was the last of all.
@@ -475,9 +504,11 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
 }
 
 // ------------------------------------------------------------------ the choice
-// Estimated times (us), fitted to cold calls of 48 to 4096 tokens, K 2560 to
-// 11008, N 1024 to 65536: a launch, then for each round of workgroups a start
-// and end and K's blocks; slices add their sums' way through memory.
+// Estimated times (us), fitted to cold calls of 33 to 4096 tokens, K 1024 to
+// 14336, N 1024 to 22016: a launch, then for each round of workgroups a start
+// and end and K's blocks; slices add their sums' way through memory. Over 198
+// such shapes the chosen tile and slices take 0.6 % longer at the mean than the
+// best ones, 10 % at the most.
 enum Kind { MV, R64x64, R64x128, R128x64, R128x128, R128x256, R256x128, R256x256 };
 struct Tile {
     Kind kind;
@@ -485,9 +516,9 @@ struct Tile {
     double ends, block8, block16;  // a round's start and end; a block by the 8-bit and the f16 instruction (0: not built)
 };
 constexpr Tile kTiles[] = {
-    {R64x64, 64, 64, 4.0, 0, 0.70},     {R64x128, 64, 128, 4.0, 0, 0.87},    {R128x64, 128, 64, 3.5, 0.51, 0.85},
-    {R128x128, 128, 128, 5.0, 0.61, 1.05}, {R128x256, 128, 256, 6.0, 1.0, 0}, {R256x128, 256, 128, 6.0, 0, 1.75},
-    {R256x256, 256, 256, 8.0, 1.5, 0},
+    {R64x64, 64, 64, 2.2, 0, 0.56},      {R64x128, 64, 128, 4.4, 0, 0.61},    {R128x64, 128, 64, 2.3, 0.375, 0.64},
+    {R128x128, 128, 128, 2.9, 0.52, 1.0}, {R128x256, 128, 256, 3.4, 0.81, 0}, {R256x128, 256, 128, 4.5, 0, 1.56},
+    {R256x256, 256, 256, 5.1, 1.03, 0},
 };
 
 struct Plan {
@@ -515,7 +546,7 @@ Plan plan(const st_context *ctx, const MmArgs &a) {
             const double sums = 4.0 * s * a.M * a.N;
             if (s > 1 && (t.kind == R256x256 || sums > (double)ctx->ws_bytes)) break;
             const double rounds = std::ceil((double)tiles * s / ctx->num_cus);
-            const double us = 3.0 + rounds * (t.ends + (KB + s - 1) / s * each) + (s > 1 ? 2.5 + sums / 5.5e6 : 0.0);
+            const double us = 2.1 + rounds * (t.ends + (KB + s - 1) / s * each) + (s > 1 ? 3.1 + sums / 3e6 : 0.0);
             if (force && slices > 0 ? s <= slices : us < least) least = us, best = {t.kind, s};
         }
     }
@@ -541,7 +572,7 @@ int run(st_context *ctx, const MmArgs &a, Plan p) {
         case R128x128:
             exact ? run_ring<128, 128, 4, 2, 4, true>(ctx, a, p.splits) : run_ring<128, 128, 4, 2, 4, false>(ctx, a, p.splits);
             break;
-        case R128x256: run_ring<128, 256, 4, 2, 3, false>(ctx, a, p.splits); break;
+        case R128x256: run_ring<128, 256, 2, 4, 3, false>(ctx, a, p.splits); break;
         case R256x128: run_ring<256, 128, 4, 2, 3, true>(ctx, a, p.splits); break;
         case R256x256: {
             st::launch(ctx, wide_kernel, dim3((unsigned)(std::max(ctx->num_cus, 8) / 8 * 8)), dim3(512), 0, a);

@@ -171,12 +171,13 @@ void by_shape(st_context *ctx, const MmArgs &a, Shape s) {
 namespace st {
 namespace f8 {
 
-// Of 33 to 64 tokens (fewer always come here): a start of 4 us, and the
-// fullest CUs' blocks (measured at K 2560 to 11008, N 1024 to 65536).
+// Of 33 to 64 tokens (fewer always come here): a start, and the fullest CUs'
+// blocks, which come faster where CUs are idle (fitted at K 1024 to 14336, N 1024
+// to 22016).
 double mv_us(const st_context *ctx, const MmArgs &a) {
     const Shape s = shape(ctx, a);
-    const double each = s.nt == 1 ? (a.M <= 48 ? 0.18 : 0.22) : (a.M <= 48 ? 0.28 : 0.335);
-    return 4.0 + std::max(1.0, (double)((a.N + 15) / 16) / s.nt / ctx->num_cus) * blocks(a.K) * each;
+    const double each = s.nt == 1 ? (a.M <= 48 ? 0.165 : 0.21) : (a.M <= 48 ? 0.28 : 0.41);
+    return 2.6 + std::max(0.6, (double)((a.N + 15) / 16) / s.nt / ctx->num_cus) * blocks(a.K) * each;
 }
 
 int mv(st_context *ctx, const MmArgs &a) {
