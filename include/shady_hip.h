@@ -374,10 +374,12 @@ int st_int8_repack(st_context *ctx, const int8_t *w, int8_t *w_tiled, int K, int
  *   x         x_dtype (ST_F32 or ST_F16), or NULL, with residual_out NULL: the
  *             norm of the residual alone
  *   weight    f32 [D]
- *   y         y_dtype (ST_F32 or ST_F16) or NULL; it may be x's buffer
+ *   y         y_dtype (ST_F32 or ST_F16) or NULL; it may be x's buffer, or the
+ *             residual's where the sum does not go there
  *   *_stride  elements from one row to the next
- * f32 arithmetic. D a multiple of 16, at most 32768. Pointers and strides in
- * whole 16 bytes (y_scale: 4). */
+ * Buffers that are one have one type and stride. f32 arithmetic. M less than
+ * 2^22; D a multiple of 16, at most 32768. Pointers and strides in whole 16 bytes
+ * (y_scale: 4). */
 int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dtype, int64_t res_stride, const void *x,
                    int x_dtype, int64_t x_stride, void *residual_out, int64_t out_stride, const float *weight,
                    float eps, void *y, int y_dtype, int64_t y_stride, uint8_t *y8, float *y_scale,
@@ -385,17 +387,18 @@ int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dtype, int64_t
 
 /* Rows of e4m3 of M rows a [K], or of silu(a) * b where b is given (the input
  * of a down projection), silu(v) = v / (1 + exp(-v)); dtype ST_F32 or ST_F16,
- * *_stride elements from one row to the next. Pointers and strides in whole 16
- * bytes (y_scale: 4). */
+ * *_stride elements from one row to the next. Less than 2^24 units of a row's
+ * 2048 dims. Pointers and strides in whole 16 bytes (y_scale: 4). */
 int st_fp8_quant(st_context *ctx, const void *a, const void *b, int dtype, int64_t a_stride, int64_t b_stride,
                  uint8_t *y8, float *y_scale, int64_t scale_stride, int M, int K);
 
 /* y[m][n] = sum_b x_scale[b][m] w_scale[n / 128][b] sum_{k in b} x8[m][k] w[n][k],
- * y [M][N] of y_dtype (ST_F32 or ST_F16), any M and N. Products are exact; sums
- * are f32, in a fixed order. x8, w and y 16-byte aligned
- * (scales: 4). f32 y keeps f32 sums; so does f16 y of at most 64 tokens. f16 y of
- * more comes from the 8-bit matrix instruction, which keeps a product to 2^-13 of
- * the largest of its eight k (rel-L2 3e-5 to 5e-5, beside 2.1e-4 of f16 itself). */
+ * y [M][N] of y_dtype (ST_F32 or ST_F16), any M and N (at most 2^28, and fewer
+ * than 2^22 blocks of 128 x 128 of y). Products are exact; sums are f32, in a
+ * fixed order. x8, w and y 16-byte aligned (scales: 4). f32 y keeps f32 sums; so
+ * does f16 y of at most 64 tokens. f16 y of more comes from the 8-bit matrix
+ * instruction, which keeps a product to 2^-13 of the largest of its eight k
+ * (rel-L2 3e-5 to 5e-5, beside 2.1e-4 of f16 itself). */
 int st_fp8_gemm(st_context *ctx, const uint8_t *x8, const float *x_scale, int64_t scale_stride, const uint8_t *w,
                 const float *w_scale, void *y, int y_dtype, int M, int K, int N);
 

@@ -34,6 +34,7 @@ namespace {
 
 using namespace st::f8;
 
+constexpr int kMostRows = 1 << 28;
 constexpr int D = 3;      // instructions between one and its FMAs
 constexpr int kPanel = 6; // tiles along the tokens that run side by side: an XCD's 32 CUs then
                           // share 6 strips of x and 5 of w in its L2 (4096 x 4096 x 22016: all 16 409 us, 8 390, 6 367, 4 384)
@@ -596,7 +597,9 @@ extern "C" int st_fp8_gemm(st_context *ctx, const uint8_t *x, const float *x_sca
     if (M < 1 || N < 1 || K < 16 || K % 16 || K > (1 << 22))
         return st::fail(ST_ERR_SHAPE, "%s: M=%d, K=%d (a multiple of 16, at most 2^22), N=%d", fn, M, K, N);
     if (scale_stride < M) return st::fail(ST_ERR_SHAPE, "%s: a block's scales overlap the next one's", fn);
-    if ((int64_t)blocks(M) * blocks(N) > (1 << 28)) return st::fail(ST_ERR_SHAPE, "%s: M=%d, N=%d", fn, M, N);
+    // (a launch is of fewer than 2^32 threads; the smallest tile is 128 x 64 for 512, of at most 64 tokens 32 columns for 256)
+    if (M > kMostRows || N > kMostRows || (int64_t)blocks(M) * blocks(N) >= (1 << 22))
+        return st::fail(ST_ERR_SHAPE, "%s: M=%d, N=%d (each at most 2^28, fewer than 2^22 blocks of 128 x 128)", fn, M, N);
     if (!st::aligned16(x) || !st::aligned16(w) || !st::aligned16(y) || !aligned4(x_scale) || !aligned4(w_scale))
         return st::fail(ST_ERR_ALIGN, "%s: pointers must be 16-byte aligned (scales: 4)", fn);
     const MmArgs a{x, w, x_scale, w_scale, y, scale_stride, M, K, N, y_dtype == ST_F32};

@@ -171,6 +171,14 @@ extern "C" int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dty
     if (!st::aligned16(residual) || !st::aligned16(x) || !st::aligned16(residual_out) || !st::aligned16(weight) || !st::aligned16(y) ||
         !st::aligned16(y8) || !aligned4(y_scale))
         return st::fail(ST_ERR_ALIGN, "%s: pointers must be 16-byte aligned (y_scale: 4)", fn);
+    // (a row's outputs may be written before another's inputs are read: in one buffer they are the same row's)
+    if (y && ((y == x && (y_dtype != x_dtype || y_stride != x_stride)) ||
+              (y == residual && (y_dtype != res_dtype || y_stride != res_stride))))
+        return st::fail(ST_ERR_INVALID, "%s: y in an input's buffer with another type or stride", fn);
+    if (x && residual_out == residual && out_stride != res_stride)
+        return st::fail(ST_ERR_INVALID, "%s: residual_out in residual's buffer with another stride", fn);
+    if (y && y == residual_out) return st::fail(ST_ERR_INVALID, "%s: y in residual_out's buffer", fn);
+    if ((int64_t)M * 1024 > 0xFFFFFFFF) return st::fail(ST_ERR_SHAPE, "%s: M=%d (fewer than 2^22)", fn, M);
     NormArgs a{};
     a.res = residual, a.x = x, a.res_out = residual_out, a.weight = weight, a.y = y, a.y8 = y8, a.scale = y_scale;
     a.res_stride = res_stride, a.x_stride = x_stride, a.out_stride = out_stride, a.y_stride = y_stride, a.scale_stride = scale_stride;
@@ -199,7 +207,7 @@ extern "C" int st_fp8_quant(st_context *ctx, const void *a, const void *b, int d
     QuantArgs q{};
     q.a = a, q.b = b, q.a_stride = a_stride, q.b_stride = b_stride, q.scale_stride = scale_stride;
     q.y8 = y8, q.scale = y_scale, q.pieces = K / 8, q.units = (K / 8 + 255) / 256;
-    if ((int64_t)M * q.units > 0x7FFFFFFF) return st::fail(ST_ERR_SHAPE, "%s: M=%d rows of %d are too many", fn, M, K);
+    if ((int64_t)M * q.units * 256 > 0xFFFFFFFF) return st::fail(ST_ERR_SHAPE, "%s: M=%d rows of %d are too many", fn, M, K);
     const st::OnDevice on(ctx);
     if (on.error != hipSuccess) return st::hip_fail(on.error, fn);
     const dim3 grid((unsigned)(M * q.units)), block(256);

@@ -134,8 +134,8 @@ def load_fp8_checkpoint(gpu, model_dir: str) -> tuple[dict, dict]:
     path = os.path.join(model_dir, "config.json")
     if os.path.exists(path):
         with open(path) as f:
-            block = json.load(f).get("quantization_config", {}).get("weight_block_size", [FP8_BLOCK] * 2)
-        if list(block) != [FP8_BLOCK] * 2:
+            block = (json.load(f).get("quantization_config") or {}).get("weight_block_size", [FP8_BLOCK] * 2)
+        if block != [FP8_BLOCK] * 2:
             raise ValueError(f"config.json: weight_block_size {block}, only {[FP8_BLOCK] * 2} is supported")
     weights, scales, bf16 = {}, {}, {}
     for shard in _shards(model_dir):

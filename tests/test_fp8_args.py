@@ -158,7 +158,11 @@ NORM = dict(ctx=CTX, residual=P, res_dtype=ST_F32, res_stride=K, x=P, x_dtype=ST
     (dict(out_stride=-K), ST_ERR_SHAPE), (dict(y_stride=K - 4), ST_ERR_SHAPE), (dict(scale_stride=M - 1), ST_ERR_SHAPE),
     (dict(res_stride=K + 2), ST_ERR_ALIGN), (dict(x_stride=K + 1), ST_ERR_ALIGN), (dict(y_dtype=ST_F16, y_stride=K + 4), ST_ERR_ALIGN),
     (dict(residual=ODD), ST_ERR_ALIGN), (dict(x=ODD), ST_ERR_ALIGN), (dict(residual_out=ODD), ST_ERR_ALIGN), (dict(weight=ODD), ST_ERR_ALIGN),
-    (dict(y=ODD), ST_ERR_ALIGN), (dict(y8=ODD), ST_ERR_ALIGN), (dict(y_scale=4097), ST_ERR_ALIGN)])
+    (dict(y=ODD), ST_ERR_ALIGN), (dict(y8=ODD), ST_ERR_ALIGN), (dict(y_scale=4097), ST_ERR_ALIGN),
+    (dict(x=2 * P, y=2 * P, y_stride=2 * K), ST_ERR_INVALID), (dict(x=2 * P, y=2 * P, y_dtype=ST_F16), ST_ERR_INVALID),
+    (dict(x=2 * P, y=3 * P, out_stride=2 * K), ST_ERR_INVALID), (dict(x=2 * P, y=P), ST_ERR_INVALID),
+    (dict(x=2 * P, y=4 * P, residual_out=4 * P), ST_ERR_INVALID), (dict(x=Z, residual_out=Z, y=P, y_stride=2 * K), ST_ERR_INVALID),
+    (dict(x=2 * P, y=3 * P, m=1 << 22, scale_stride=1 << 22), ST_ERR_SHAPE)])
 def test_c_norm(kw, rc):
     assert st("st_add_rmsnorm", *{**NORM, **kw}.values()) == rc
 
@@ -170,7 +174,8 @@ QUANT = dict(ctx=CTX, a=P, b=P, dtype=ST_F16, a_stride=K, b_stride=K, y8=P, y_sc
     (dict(ctx=Z), ST_ERR_INVALID), (dict(a=Z), ST_ERR_INVALID), (dict(y8=Z), ST_ERR_INVALID), (dict(y_scale=Z), ST_ERR_INVALID),
     (dict(dtype=ST_BF16), ST_ERR_INVALID), (dict(m=0), ST_ERR_SHAPE), (dict(m=-1), ST_ERR_SHAPE), (dict(k=K + 8), ST_ERR_SHAPE),
     (dict(k=0), ST_ERR_SHAPE), (dict(a_stride=K - 8), ST_ERR_SHAPE), (dict(b_stride=0), ST_ERR_SHAPE), (dict(scale_stride=0), ST_ERR_SHAPE),
-    (dict(m=2**31 - 1, k=1 << 22, a_stride=1 << 22, b_stride=1 << 22, scale_stride=2**31), ST_ERR_SHAPE), (dict(a_stride=K + 4), ST_ERR_ALIGN),
+    (dict(m=2**31 - 1, k=1 << 22, a_stride=1 << 22, b_stride=1 << 22, scale_stride=2**31), ST_ERR_SHAPE),
+    (dict(m=1 << 24, scale_stride=1 << 24), ST_ERR_SHAPE), (dict(a_stride=K + 4), ST_ERR_ALIGN),
     (dict(b_stride=K + 1), ST_ERR_ALIGN), (dict(a=ODD), ST_ERR_ALIGN), (dict(b=ODD), ST_ERR_ALIGN), (dict(y8=ODD), ST_ERR_ALIGN),
     (dict(y_scale=4098), ST_ERR_ALIGN)])
 def test_c_quant(kw, rc):
@@ -184,7 +189,9 @@ GEMM = dict(ctx=CTX, x=P, x_scale=P, scale_stride=M, w=P, w_scale=P, y=P, y_dtyp
     (dict(ctx=Z), ST_ERR_INVALID), (dict(x=Z), ST_ERR_INVALID), (dict(x_scale=Z), ST_ERR_INVALID), (dict(w=Z), ST_ERR_INVALID),
     (dict(w_scale=Z), ST_ERR_INVALID), (dict(y=Z), ST_ERR_INVALID), (dict(y_dtype=ST_BF16), ST_ERR_INVALID), (dict(m=0), ST_ERR_SHAPE),
     (dict(n=0), ST_ERR_SHAPE), (dict(k=0), ST_ERR_SHAPE), (dict(k=K + 8), ST_ERR_SHAPE), (dict(k=(1 << 22) + 16), ST_ERR_SHAPE),
-    (dict(scale_stride=M - 1), ST_ERR_SHAPE), (dict(m=2**31 - 1, n=2**31 - 1, scale_stride=2**31), ST_ERR_SHAPE), (dict(x=ODD), ST_ERR_ALIGN),
+    (dict(scale_stride=M - 1), ST_ERR_SHAPE), (dict(m=2**31 - 1, n=2**31 - 1, scale_stride=2**31), ST_ERR_SHAPE),
+    (dict(m=2**31 - 1, scale_stride=2**31), ST_ERR_SHAPE), (dict(n=2**31 - 1), ST_ERR_SHAPE), (dict(m=1 << 18, n=1 << 18, scale_stride=1 << 18), ST_ERR_SHAPE),
+    (dict(x=ODD), ST_ERR_ALIGN),
     (dict(w=ODD), ST_ERR_ALIGN), (dict(y=ODD), ST_ERR_ALIGN), (dict(x_scale=4097), ST_ERR_ALIGN), (dict(w_scale=4098), ST_ERR_ALIGN)])
 def test_c_gemm(kw, rc):
     assert st("st_fp8_gemm", *{**GEMM, **kw}.values()) == rc
@@ -244,8 +251,11 @@ def test_checkpoint_refusals(tmp_path):
     save(tmp_path, good, {"quantization_config": {"weight_block_size": [128, 128]}})
     linears, bf16 = sta.load_fp8_checkpoint(G, str(tmp_path))
     assert list(linears) == ["a"] and torch.equal(linears["a"].w.float(), w.float()) and not bf16
+    save(tmp_path, good, {"quantization_config": None})
+    assert list(sta.load_fp8_checkpoint(G, str(tmp_path))[0]) == ["a"]
     for bad, config in (({"a.weight": w}, None), ({"a.weight_scale_inv": s}, None), ({**good, "a.weight_scale_inv": s[:, :1].contiguous()}, None),
-                        (good, {"quantization_config": {"weight_block_size": [64, 128]}}), ({**good, "a.weight_scale_inv": s.half()}, None)):
+                        (good, {"quantization_config": {"weight_block_size": [64, 128]}}),
+                        (good, {"quantization_config": {"weight_block_size": None}}), ({**good, "a.weight_scale_inv": s.half()}, None)):
         (tmp_path / "config.json").unlink(missing_ok=True)
         save(tmp_path, bad, config)
         with pytest.raises((ValueError, TypeError)):

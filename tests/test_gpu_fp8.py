@@ -165,6 +165,20 @@ def test_norm_in_place_and_out_of_place(gpu):
         assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_norm_over_the_residual(gpu, dtype):
+    """y in the residual's buffer (no sum goes there): the bits of a buffer of
+    its own."""
+    m, d = 5, 1040
+    r, x, w = rand(1, m, d, dtype=dtype), rand(2, m, d), rand(3, d)
+    for add in (None, x):
+        ro = None if add is None else torch.empty_like(r)
+        want, y = torch.empty_like(r), r.clone()
+        sta.add_rmsnorm(gpu, r, w, add, want, residual_out=ro)
+        sta.add_rmsnorm(gpu, y, w, add, y, residual_out=ro)
+        assert torch.equal(y, want)
+
+
 def test_norm_rows_keep_to_themselves(gpu):
     """A row of zeros, one with an infinity, one with a NaN, a large one."""
     m, d = 6, 1040
@@ -386,6 +400,36 @@ def test_norm_product_chain(gpu):
                 mlp()
                 torch.cuda.synchronize()
                 want = out.clone()
+
+
+def test_graphs_share_the_workspace(gpu):
+    """Two captured products in slices of K, whose partial sums meet in the
+    context's workspace: replayed in turn, with eager products between them."""
+    calls = []
+    for seed, (m, k, n, dtype) in enumerate([(130, 2064, 264, F16), (77, 1424, 300, F32), (200, 2064, 130, F16)]):
+        case = gemm_case(seed, m, k, n)
+        y = torch.empty(m, n, dtype=dtype, device=DEV)
+        calls.append((sta.Fp8Rows.of(*case[:2]), sta.Fp8Weight.of(*case[2:]), y))
+    with gpu.tuning(FP8_TILE=4, FP8_SPLITS=4):
+        for c in calls:
+            sta.fp8_gemm(gpu, *c)
+        torch.cuda.synchronize()
+        want = [y.clone() for _, _, y in calls]
+        for (x, w, y), v in zip(calls, want):
+            check_product(v, x.data, x.scale, w.w, w.scale, many=v.dtype is F16)
+        graphs = []
+        for c in calls[:2]:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                sta.fp8_gemm(gpu, *c)
+        for turn in range(3):
+            for _, _, y in calls:
+                y.zero_()
+            graphs[turn % 2].replay()
+            sta.fp8_gemm(gpu, *calls[2])
+            graphs[1 - turn % 2].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, v) for (_, _, y), v in zip(calls, want))
 
 
 def test_gemm_past_32_bits(gpu):
