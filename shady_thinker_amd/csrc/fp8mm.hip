@@ -505,21 +505,27 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
 }
 
 // ------------------------------------------------------------------ the choice
-// Estimated times (us), fitted to cold calls of 33 to 4096 tokens, K 1024 to
-// 14336, N 1024 to 22016: a launch, then for each round of workgroups a start
-// and end and K's blocks; slices add their sums' way through memory. Over 198
-// such shapes the chosen tile and slices take 0.6 % longer at the mean than the
-// best ones, 10 % at the most.
+// Estimated times (us), fitted to calls of 65 to 4096 tokens, K 1024 to 14336, N
+// 1024 to 22016, weights cold or in the last cache: a launch, then for each round
+// of workgroups a start and end and K's blocks, which take longer where all CUs
+// load at once; slices add their sums' way through memory. Over 171 such shapes
+// the chosen tile and slices take 0.2 to 0.5 % longer at the mean than the best
+// ones (two boxes, cold and not), 17 % at the most.
 enum Kind { MV, R64x64, R64x128, R128x64, R128x128, R128x256, R256x128, R256x256 };
+struct Rate {
+    double few, all;  // a block on few of the CUs, on all (0: not built)
+};
 struct Tile {
     Kind kind;
     int bm, bn;
-    double ends, block8, block16;  // a round's start and end; a block by the 8-bit and the f16 instruction (0: not built)
+    double ends;  // a round's start and end
+    Rate by8, by16;
 };
 constexpr Tile kTiles[] = {
-    {R64x64, 64, 64, 2.2, 0, 0.56},      {R64x128, 64, 128, 4.4, 0, 0.61},    {R128x64, 128, 64, 2.3, 0.375, 0.64},
-    {R128x128, 128, 128, 2.9, 0.52, 1.0}, {R128x256, 128, 256, 3.4, 0.81, 0}, {R256x128, 256, 128, 4.5, 0, 1.56},
-    {R256x256, 256, 256, 5.1, 1.03, 0},
+    {R64x64, 64, 64, 1.7, {0.28, 0.29}, {0.55, 0.48}},     {R64x128, 64, 128, 2.9, {0.30, 0.38}, {0.59, 0.63}},
+    {R128x64, 128, 64, 3.1, {0.33, 0.37}, {0.64, 0.63}},   {R128x128, 128, 128, 3.8, {0.44, 0.61}, {0.97, 1.02}},
+    {R128x256, 128, 256, 4.2, {0.81, 0.90}, {0, 0}},       {R256x128, 256, 128, 3.6, {0, 0}, {1.63, 1.76}},
+    {R256x256, 256, 256, 3.1, {1.06, 1.06}, {0, 0}},
 };
 
 struct Plan {
@@ -535,19 +541,21 @@ Plan plan(const st_context *ctx, const MmArgs &a) {
     double least = can_mv ? mv_us(ctx, a) : 1e30;
     const int KB = blocks(a.K);
     // (the 256 x 256 kernel brings two blocks of K at once)
-    auto built = [&](const Tile &t) { return (exact ? t.block16 : t.block8) != 0 && (t.kind != R256x256 || KB > 1); };
+    auto built = [&](const Tile &t) { return (exact ? t.by16 : t.by8).all != 0 && (t.kind != R256x256 || KB > 1); };
     bool force = false;
     for (const Tile &t : kTiles) force |= t.kind == forced && built(t);
     if (force) least = 1e30;
     for (const Tile &t : kTiles) {
-        if (!built(t) || (force ? t.kind != forced : (t.bm == 64) != (a.M <= 64))) continue;
-        const double each = exact ? t.block16 : t.block8;
+        if (!built(t) || (force ? t.kind != forced : a.M <= 64 && t.bm != 64)) continue;
+        const Rate rate = exact ? t.by16 : t.by8;
         const int64_t tiles = (int64_t)((a.M + t.bm - 1) / t.bm) * ((a.N + t.bn - 1) / t.bn);
         for (int s = 1; s <= 8 && s <= KB; s *= 2) {
             const double sums = 4.0 * s * a.M * a.N;
             if (s > 1 && (t.kind == R256x256 || sums > (double)ctx->ws_bytes)) break;
-            const double rounds = std::ceil((double)tiles * s / ctx->num_cus);
-            const double us = 2.1 + rounds * (t.ends + (KB + s - 1) / s * each) + (s > 1 ? 3.1 + sums / 3e6 : 0.0);
+            const int64_t rounds = tiles * s / ctx->num_cus;
+            const double rest = (double)(tiles * s % ctx->num_cus) / ctx->num_cus;
+            const auto round = [&](double on) { return t.ends + (KB + s - 1) / s * std::max(rate.few, rate.all * on); };
+            const double us = 2.5 + rounds * round(1.0) + (rest > 0 ? round(rest) : 0.0) + (s > 1 ? 2.7 + sums / 4.1e6 : 0.0);
             if (force && slices > 0 ? s <= slices : us < least) least = us, best = {t.kind, s};
         }
     }
@@ -565,8 +573,12 @@ int run(st_context *ctx, const MmArgs &a, Plan p) {
     const char *name = "fp8_ring_kernel";
     switch (p.kind) {
         case MV: return mv(ctx, a);
-        case R64x64: run_ring<64, 64, 2, 2, 4, true>(ctx, a, p.splits); break;
-        case R64x128: run_ring<64, 128, 2, 4, 4, true>(ctx, a, p.splits); break;
+        case R64x64:
+            exact ? run_ring<64, 64, 2, 2, 4, true>(ctx, a, p.splits) : run_ring<64, 64, 2, 2, 4, false>(ctx, a, p.splits);
+            break;
+        case R64x128:
+            exact ? run_ring<64, 128, 2, 4, 4, true>(ctx, a, p.splits) : run_ring<64, 128, 2, 4, 4, false>(ctx, a, p.splits);
+            break;
         case R128x64:
             exact ? run_ring<128, 64, 4, 2, 4, true>(ctx, a, p.splits) : run_ring<128, 64, 4, 2, 4, false>(ctx, a, p.splits);
             break;

@@ -228,7 +228,7 @@ def tile_cases():
              (1600, 384, 300), (700, 256, 1300), (2300, 400, 2568)]
     for m, k, n in sizes:
         for dtype in (F32, F16):
-            for tile in (1, 2, 3, 4, 6) if dtype is F32 or m <= 64 else (3, 4, 5, 7):
+            for tile in (1, 2, 3, 4, 6) if dtype is F32 or m <= 64 else (1, 2, 3, 4, 5, 7):
                 if tile != 7:
                     yield from ((tile, s, m, k, n, dtype) for s in (1, 2, 8))
                 elif k > B:  # (the 256 x 256 kernel: two blocks of K at least, no slices)
