@@ -2,7 +2,7 @@
 // blocks of the weight and of each token's 128 dims (st_fp8_gemm; no reference
 // counterpart, as INT8):
 //   y[m][n] = sum_b sx[b][m] sw[n / 128][b] sum_{k in b} x[m][k] w[n][k]
-// Up to 32 tokens: fp8mv.hip; up to 64 whichever is estimated faster. Here,
+// Up to 48 tokens: fp8mv.hip; up to 64 whichever is estimated faster. Here,
 // two ways to sum a block's 128 products:
 //  * v_mfma_f32_16x16x128_f8f6f4 takes the block whole. In each eight k it keeps
 //    a product to 2^-13 of the largest one's power of two (measured: a product
@@ -537,7 +537,7 @@ Plan plan(const st_context *ctx, const MmArgs &a) {
     const int forced = st::tune(ctx, ST_TUNE_FP8_TILE, -1), slices = st::tune(ctx, ST_TUNE_FP8_SPLITS, -1);
     Plan best{MV, 1};
     const bool can_mv = a.M <= 64, exact = a.f32 || a.M <= 64;
-    if (can_mv && (forced == MV || (forced < 0 && a.M <= 32))) return best;
+    if (can_mv && (forced == MV || (forced < 0 && a.M <= 48))) return best;
     double least = can_mv ? mv_us(ctx, a) : 1e30;
     const int KB = blocks(a.K);
     // (the 256 x 256 kernel brings two blocks of K at once)

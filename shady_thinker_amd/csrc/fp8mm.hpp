@@ -51,21 +51,16 @@ __device__ __forceinline__ f32x4 mfma(const Frag<true> &a, const Frag<true> &b) 
     return p;
 }
 
-// 16 bytes for each lane from a resource to LDS, at `lds` + 16 lane. Eight
-// lanes take a row's 128 bytes: loads to registers in the fragments' order
-// (neighbouring lanes in different rows) went one lane at a time, 64 cycles an
-// instruction (16 tokens x 4096 x 22016: 24.9 us; through LDS 20.1).
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t *lds, int voff, int soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, voff, soff, 0, 0);
-}
-
-// A buffer resource (uniform) and loads from it to LDS by assembly: of the
-// builtin's loads in flight the compiler does not know which part of LDS each
-// fills, so before reads of any it waits for more than it must. Nothing is
-// written to registers; wait_loads says when they have come, and a loop with
-// these has no other vector loads (whose waits would count them) and no other
-// use of m0. A resource that may come out of the vector unit (a lane it was kept
-// in) needs five wait states before it is read: settle().
+// A buffer resource (uniform) and loads from it to LDS, at `lds` + 16 (or 4)
+// lane. Eight lanes take a row's 128 bytes: loads to registers in the fragments'
+// order (neighbouring lanes in different rows) went one lane at a time, 64 cycles
+// an instruction (16 tokens x 4096 x 22016: 24.9 us; through LDS 20.1). By
+// assembly: of the builtin's loads in flight the compiler does not know which
+// part of LDS each fills, so before reads of any it waits for more than it must.
+// Nothing is written to registers; wait_loads says when they have come, and a
+// loop with these has no other vector loads (whose waits would count them) and
+// no other use of m0. A resource that may come out of the vector unit (a lane it
+// was kept in) needs five wait states before it is read: settle().
 typedef i32x4 Rsrc;
 __device__ __forceinline__ Rsrc scalar(Rsrc r) {
     return Rsrc{__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y), __builtin_amdgcn_readfirstlane(r.z), kRsrcWord3};

@@ -2,19 +2,28 @@
 // weight's bytes.
 //
 // A workgroup takes 16 NT columns, its W waves every W-th block of 128 k. A
-// wave brings its blocks of both operands to LDS by DMA, S of them ahead, in
-// slots of its own: it waits for its own loads only, and the waves meet once,
-// when their sums are added in order. A row's 128 bytes are eight 16-byte
-// chunks, chunk j of row r at j ^ (r % 8), so that fragment reads hit every
-// bank once. e4m3 goes to f16 exactly and f16 products are exact in the matrix
-// instruction's f32 sums (the 8-bit instruction's are not, see fp8mm.hip).
+// wave brings its blocks of both operands and their scales to LDS by DMA, S of
+// them ahead, in slots of its own: it waits for its own loads only (and not for
+// the other slots', whose number the waits count), and the waves meet once, when
+// their sums are added in order. A row's 128 bytes are eight 16-byte chunks,
+// chunk j of row r at j ^ (r % 8), so that fragment reads hit every bank once.
+// e4m3 goes to f16 exactly and f16 products are exact in the matrix instruction's
+// f32 sums (the 8-bit instruction's are not, see fp8mm.hip).
 //
-// Sizes of columns and waves (MI355X, cold weights; us of (NT, W)):
-//   16 columns, 16 or 8 waves: up to a tile a CU (one token 4096 x 4096: (1, 16) 5.9, (1, 8) 7.1, (2, 8) 6.9, (2, 4) 8.3)
+// Workgroups begin at different blocks of k: side by side at the same one, their
+// rows' 128 bytes lie K apart, where K is a multiple of a few KiB in few channels
+// of memory and caches (one token 8192 x 8192: 17.2 -> 13.5 us, 5.0 TB/s; 4096 x
+// 22016 18.9 -> 17.2, 5.2 TB/s; 11008 x 4096 12.0 -> 11.5, 3.9 TB/s; cold weights).
+//
+// Sizes of columns and waves (MI355X, cold weights; us of (NT, W), measured with
+// two slots each and the same first block):
+//   16 columns, 16 or 8 waves: up to a tile a CU (one token 4096 x 4096: (1, 16) 5.9, (1, 8) 7.1, (2, 8) 6.9, (2, 4) 8.3);
+//   a workgroup a CU, so three slots and more where they fit (11008 x 4096: 13.2 -> 12.0)
 //   16 columns, fewer waves, several workgroups a CU: up to 1.2
-//   32 columns, 8 waves: up to 2 (4096 x 8192: (2, 8) 9.6, (1, 8) 10.9, (2, 4) 10.1)
+//   32 columns, 8 waves: up to 2 (4096 x 8192: (2, 8) 9.6, (1, 8) 10.9, (2, 4) 10.1), three slots (8192 x 8192: 18.2 -> 17.2)
 //   then four waves and 32, 48 or 64 columns, whichever leaves the fullest CU
-//   the fewest (4096 x 22016: 48 20.2, 32 20.7, 64 21.1; 28672: 64 24.4, 32 26.3, 48 28.2)
+//   the fewest (4096 x 22016: 48 20.2, 32 20.7, 64 21.1; 28672: 64 24.4, 32 26.3, 48 28.2);
+//   several workgroups a CU, so two slots (three, 48 columns: 15.8 -> 18.2, the weights in the last cache)
 #include "fp8mm.hpp"
 
 #include <algorithm>
@@ -23,27 +32,23 @@ namespace {
 
 using namespace st::f8;
 
-constexpr int S = 2;  // slots of a wave (three: 4096 x 22016, 48 columns 15.8 -> 18.2 us: fewer workgroups a CU)
-
-// X8: at most eight tokens, one DMA of x for a block.
-template <int MT, bool X8, int NT, int W>
+// X8: at most eight tokens, one DMA of x for a block. S: slots of a wave.
+template <int MT, bool X8, int NT, int W, int S>
 __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
     constexpr int XD = X8 ? 1 : 2 * MT, ND = 2 * NT + XD;  // DMAs of a slot, eight rows each
-    constexpr int SLOT = ND * 1024;
+    constexpr int SLOT = ND * 1024, PART = W * SLOT;
+    constexpr bool CROSS = NT == 3;  // columns on both sides of a border between the weight's blocks
     static_assert(!X8 || MT == 1, "eight tokens are one fragment");
     static_assert(SLOT >= MT * NT * 1024, "the waves' sums fit the first slots");
-    __shared__ __align__(1024) uint8_t s0[W * SLOT], s1[W * SLOT];
+    __shared__ __align__(1024) uint8_t lds[S * PART];
+    __shared__ __align__(16) float sx[S][W][64], sw[CROSS ? 2 : 1][W][64];  // scales: the slots' tokens', the weight's of each wave's next 64 blocks
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
     const int n0 = blockIdx.x * (16 * NT);
     const int KB = (a.K + kBlock - 1) / kBlock;
     const int rows_w = min(16 * NT, a.N - n0);
-    const __amdgpu_buffer_rsrc_t rw =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + (int64_t)n0 * a.K), (short)0, rows_w * a.K, kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void *)a.x, (short)0, a.M * a.K, kRsrcWord3);
-    // (the columns' blocks: two where 48 columns lie across a border)
+    Rsrc rw = rsrc(a.w + (int64_t)n0 * a.K, rows_w * a.K), rx = rsrc(a.x, a.M * a.K);
     const int nb = n0 / kBlock, nb_last = (a.N - 1) / kBlock, cross = (nb + 1) * kBlock - n0;  // columns before the border
-    const float *const sw0 = a.sw + (int64_t)nb * KB, *const sw1 = a.sw + (int64_t)min(nb + 1, nb_last) * KB;
     // lane i of a DMA fills position i % 8 of its row i / 8; rows past the last repeat it
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     int vw[2 * NT], vx[XD];
@@ -51,21 +56,24 @@ __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
     for (int j = 0; j < 2 * NT; ++j) vw[j] = min(8 * j + (lane >> 3), rows_w - 1) * a.K + chunk;
 #pragma unroll
     for (int j = 0; j < XD; ++j) vx[j] = min(8 * j + (lane >> 3), a.M - 1) * a.K + chunk;
-    struct Scales {
-        float x[MT], w0, w1;
-    } f0, f1;
-    auto load = [&](uint8_t *s, Scales &f, int b) {
-        uint8_t *const at = s + wave * SLOT;
-        const bool in = b * kBlock + chunk < a.K;  // (K ends inside the last block; past it: zeros)
-        const int bs = min(b, KB - 1), so = bs * kBlock;
+    const unsigned part = lds_at(lds + wave * SLOT);
+    const int mine = (KB - wave + W - 1) / W;
+    // (the block it begins with: another one for the XCDs' workgroups, and within an XCD)
+    const int first = mine > 1 && mine <= 64 ? (int)((blockIdx.x / 8 + blockIdx.x) % mine) : 0;
+    auto turn = [&](int i) { return i + first < mine ? i + first : i + first - mine; };
+    auto load = [&](int s, int i) {  // the wave's block i to slot s (past the last: zeros)
+        const int b = i < mine ? wave + turn(i) * W : KB, bs = min(b, KB - 1), so = bs * kBlock;
+        const bool in = b * kBlock + chunk < a.K;  // (K ends inside the last block)
+        lds4(rsrc(a.sx + bs * a.sx_stride, a.M * 4), lds_at(sx[s][wave]), lane * 4);
 #pragma unroll
-        for (int j = 0; j < 2 * NT; ++j) dma16(rw, at + j * 1024, in ? vw[j] : kOutside, so);
+        for (int j = 0; j < 2 * NT; ++j) lds16(rw, part + s * PART + j * 1024, in ? vw[j] : kOutside, so);
 #pragma unroll
-        for (int j = 0; j < XD; ++j) dma16(rx, at + (2 * NT + j) * 1024, in ? vx[j] : kOutside, so);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) f.x[t] = a.sx[bs * a.sx_stride + min(16 * t + r, a.M - 1)];
-        f.w0 = sw0[bs];
-        if constexpr (NT == 3) f.w1 = sw1[bs];
+        for (int j = 0; j < XD; ++j) lds16(rx, part + s * PART + (2 * NT + j) * 1024, in ? vx[j] : kOutside, so);
+    };
+    auto load_sw = [&](int i) {  // the weight's scales of the wave's blocks i to i + 63
+        const int v = (wave + (i + lane) * W) * 4;
+        lds4(rsrc(a.sw + (int64_t)nb * KB, KB * 4), lds_at(sw[0][wave]), v);
+        if constexpr (CROSS) lds4(rsrc(a.sw + (int64_t)min(nb + 1, nb_last) * KB, KB * 4), lds_at(sw[1][wave]), v);
     };
     const int pos = r * kBlock + (c ^ (r & 7)) * 16;
     const int xpos = (X8 ? r & 7 : r) * kBlock + (c ^ (r & 7)) * 16;
@@ -79,43 +87,49 @@ __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
         v.set(*reinterpret_cast<const i32x4 *>(at + p), *reinterpret_cast<const i32x4 *>(at + (p ^ 64)));
         return v;
     };
-    auto step = [&](uint8_t *s, Scales &f, int b) {
-        const uint8_t *const at = s + wave * SLOT;
-        wait_loads<(S - 1) * ND, false>();  // (the other slot's may be in flight)
+    auto step = [&](int s, int i) {
+        const uint8_t *const at = lds + s * PART + wave * SLOT;
+        if (i % 64 == 0 && i) {
+            load_sw(i);
+            wait_loads<0, false>();
+        }
+        wait_loads<(S - 1) * (ND + 1), false>();  // (the other slots' may be in flight)
+        const int is = turn(i) % 64;
+        const float w0 = sw[0][wave][is], w1 = CROSS ? sw[CROSS][wave][is] : 0.0f;
         Frag<true> w[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) w[u] = frag(at + u * 2048, pos);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const Frag<true> x = frag(at + (2 * NT + 2 * t) * 1024, xpos);
+            const float f = sx[s][wave][16 * t + r];
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const float g = NT == 3 && 16 * u >= cross ? f.w1 : f.w0;
-                acc[t][u] += mfma(w[u], x) * (f.x[t] * g);
-            }
+            for (int u = 0; u < NT; ++u) acc[t][u] += mfma(w[u], x) * (f * (CROSS && 16 * u >= cross ? w1 : w0));
         }
         wait_lds();  // (the fragments are read: the slot may be filled)
-        load(s, f, b + S * W);
+        load(s, i + S);
     };
-    load(s0, f0, wave);
-    load(s1, f1, wave + W);
-    for (int b = wave; b < KB; b += S * W) {
-        step(s0, f0, b);
-        if (b + W < KB) step(s1, f1, b + W);
-    }
+    settle(rw, rx);
+    load_sw(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s) load(s, s);
+    for (int i = 0; i < mine; i += S)
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (i + s < mine) step(s, i + s);
     wait_loads<0, true>();
     __syncthreads();
-    f32x4 *const part = reinterpret_cast<f32x4 *>(s0);
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int u = 0; u < NT; ++u) part[(wave * MT * NT + t * NT + u) * 64 + lane] = acc[t][u];
+        for (int u = 0; u < NT; ++u) sums[(wave * MT * NT + t * NT + u) * 64 + lane] = acc[t][u];
     __syncthreads();
     for (int i = threadIdx.x; i < MT * NT * 64; i += 64 * W) {
         const int q = i >> 6, l = i & 63;
-        f32x4 v = part[i];
+        f32x4 v = sums[i];
 #pragma unroll
-        for (int w = 1; w < W; ++w) v += part[w * MT * NT * 64 + i];
+        for (int w = 1; w < W; ++w) v += sums[w * MT * NT * 64 + i];
         const int m = 16 * (q / NT) + (l & 15);
         if (m < a.M) store_n4(a.y, a.f32, m, n0 + 16 * (q % NT) + 4 * (l >> 4), a.N, v);
     }
@@ -123,19 +137,16 @@ __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
 
 struct Shape {
     int nt, w;
+    bool deep;  // a workgroup a CU: its slots may fill LDS
 };
 
 Shape shape(const st_context *ctx, const MmArgs &a) {
     const int tiles = (a.N + 15) / 16, cus = ctx->num_cus, KB = blocks(a.K);
-    if (tiles <= cus) {
-        // 16 waves where they share the blocks evenly (of 2560, 20 blocks: 8 waves 4.3 us, 16 4.4; of 4096: 7.1, 5.9)
-        const bool even = 10 * ((KB + 15) / 16 * 16) <= 11 * KB;
-        return {1, a.M <= 16 && even ? 16 : 8};
-    }
-    if (a.M > 32) return {2, 4};
-    if (5 * tiles <= 6 * cus) return {1, a.M <= 16 ? 8 : 4};  // (several workgroups a CU: no second round for a few)
-    if (tiles <= 2 * cus) return {2, 8};
-    Shape best{2, 4};
+    if (tiles <= cus) return {1, a.M <= 16 && KB >= 16 ? 16 : 8, true};  // (11008 x 4096: 16 waves 12.0 us, 8 12.3)
+    if (a.M > 32) return {2, 4, false};
+    if (5 * tiles <= 6 * cus) return {1, a.M <= 16 ? 8 : 4, false};  // (several workgroups a CU: no second round for a few)
+    if (tiles <= 2 * cus) return {2, 8, false};
+    Shape best{2, 4, false};
     int least = 1 << 30;
     for (int nt = 2; nt <= (a.M <= 16 ? 4 : 3); ++nt) {
         const int cost = ((tiles + nt - 1) / nt + cus - 1) / cus * nt;  // tiles of the fullest CU
@@ -144,23 +155,26 @@ Shape shape(const st_context *ctx, const MmArgs &a) {
     return best;
 }
 
-template <int MT, bool X8, int NT, int W>
+template <int MT, bool X8, int NT, int W, int S = 2>
 void run(st_context *ctx, const MmArgs &a) {
-    st::launch(ctx, mv_kernel<MT, X8, NT, W>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, a);
+    st::launch(ctx, mv_kernel<MT, X8, NT, W, S>, dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(64 * W), 0, a);
 }
 
 template <int MT, bool X8>
 void by_shape(st_context *ctx, const MmArgs &a, Shape s) {
-    if constexpr (MT > 2) {
+    if constexpr (MT == 4) {
+        s.nt == 1 ? run<MT, X8, 1, 7, 2>(ctx, a) : run<MT, X8, 2, 4, 2>(ctx, a);
+    } else if constexpr (MT == 3) {
         s.nt == 1 ? run<MT, X8, 1, 8>(ctx, a) : run<MT, X8, 2, 4>(ctx, a);
     } else {
         if constexpr (MT == 1) {
-            if (s.nt == 1 && s.w == 16) return run<MT, X8, 1, 16>(ctx, a);
+            if (s.deep) return s.w == 16 ? run<MT, X8, 1, 16, X8 ? 3 : 2>(ctx, a) : run<MT, X8, 1, 8, 4>(ctx, a);
+            if (s.nt == 1) return run<MT, X8, 1, 8>(ctx, a);
             if (s.nt == 4) return run<MT, X8, 4, 4>(ctx, a);
+        } else {
+            if (s.nt == 1) return s.deep ? run<MT, X8, 1, 8, 3>(ctx, a) : run<MT, X8, 1, 4>(ctx, a);
         }
-        if constexpr (MT == 2)
-            if (s.nt == 1 && s.w == 4) return run<MT, X8, 1, 4>(ctx, a);
-        if (s.nt == 1) return run<MT, X8, 1, 8>(ctx, a);
+        if constexpr (MT == 1) if (s.nt == 2 && s.w == 8) return run<MT, X8, 2, 8, 3>(ctx, a);
         if (s.nt == 2) return s.w == 8 ? run<MT, X8, 2, 8>(ctx, a) : run<MT, X8, 2, 4>(ctx, a);
         run<MT, X8, 3, 4>(ctx, a);
     }
@@ -171,13 +185,12 @@ void by_shape(st_context *ctx, const MmArgs &a, Shape s) {
 namespace st {
 namespace f8 {
 
-// Of 33 to 64 tokens (fewer always come here): a start, and the fullest CUs'
+// Of 49 to 64 tokens (fewer always come here): a start, and the fullest CUs'
 // blocks, which come faster where CUs are idle (fitted at K 1024 to 14336, N 1024
 // to 22016).
 double mv_us(const st_context *ctx, const MmArgs &a) {
     const Shape s = shape(ctx, a);
-    const double each = s.nt == 1 ? (a.M <= 48 ? 0.165 : 0.21) : (a.M <= 48 ? 0.28 : 0.41);
-    return 2.6 + std::max(0.6, (double)((a.N + 15) / 16) / s.nt / ctx->num_cus) * blocks(a.K) * each;
+    return 2.3 + std::max(0.6, (double)((a.N + 15) / 16) / s.nt / ctx->num_cus) * blocks(a.K) * (s.nt == 1 ? 0.205 : 0.345);
 }
 
 int mv(st_context *ctx, const MmArgs &a) {

@@ -266,6 +266,20 @@ def test_few_tokens_shapes(gpu, tune, m, k, n):
     assert (buf[m * n:] == 7.0).all()
 
 
+@pytest.mark.parametrize("m,k,n", [(3, 131200, 20), (12, 66048, 33), (20, 66048, 40), (40, 66048, 17), (64, 33280, 24), (5, 33280, 8720),
+                                   (60, 33280, 8200), (300, 33280, 130)])
+def test_gemm_of_many_blocks(gpu, m, k, n):
+    """More blocks of K than a wave, or a slice, holds scales of at once."""
+    x8, sx = rows_of(rand(1, m, k))
+    w8 = rand(2, n, k, dtype=F16).to(F8)
+    sw = torch.rand(blocks(n), blocks(k), device=DEV) + 0.5
+    y = torch.empty(m, n, device=DEV)
+    sta.fp8_gemm(gpu, sta.Fp8Rows.of(x8, sx), sta.Fp8Weight.of(w8, sw), y)
+    n0 = (n - 1) // B * B
+    check_product(y[:, n0:], x8, sx, w8[n0:], sw[n0 // B:])
+    check_product(y[:, :20], x8, sx, w8[:20], sw[:1])
+
+
 def test_gemm_without_room_for_slices(gpu):
     """Slices whose partial sums do not fit the workspace are not taken (the
     largest K and few tiles, 64 MiB)."""
