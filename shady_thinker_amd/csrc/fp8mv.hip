@@ -12,14 +12,16 @@
 //
 // Workgroups begin at different blocks of k: side by side at the same one, their
 // rows' 128 bytes lie K apart, where K is a multiple of a few KiB in few channels
-// of memory and caches (one token 8192 x 8192: 17.2 -> 13.5 us, 5.0 TB/s; 4096 x
-// 22016 18.9 -> 17.2, 5.2 TB/s; 11008 x 4096 12.0 -> 11.5, 3.9 TB/s; cold weights).
+// of memory and caches (one token 8192 x 8192: 17.2 -> 13.5 us, 4096 x 22016 18.9
+// -> 17.2). One token now takes (cold weights, in a captured graph) 2048 x 2048
+// 3.4 us, 4096 x 4096 5.7, 11008 x 4096 10.5 (4.3 TB/s), 8192 x 8192 13.6 (4.9),
+// 4096 x 22016 17.1 (5.3).
 //
 // Sizes of columns and waves (MI355X, cold weights; us of (NT, W), measured with
 // two slots each and the same first block):
-//   16 columns, 16 or 8 waves: up to a tile a CU (one token 4096 x 4096: (1, 16) 5.9, (1, 8) 7.1, (2, 8) 6.9, (2, 4) 8.3);
-//   a workgroup a CU, so three slots and more where they fit (11008 x 4096: 13.2 -> 12.0)
-//   16 columns, fewer waves, several workgroups a CU: up to 1.2
+//   16 columns, 8 waves: up to a tile a CU (one token 4096 x 4096: (1, 8) 7.1, (2, 8) 6.9, (2, 4) 8.3); a workgroup a
+//   CU, so three slots and more where they fit (11008 x 4096: 13.4 -> 10.8; 16 waves of three: 11.7)
+//   16 columns, 4 or 8 waves, several workgroups a CU: up to 1.2
 //   32 columns, 8 waves: up to 2 (4096 x 8192: (2, 8) 9.6, (1, 8) 10.9, (2, 4) 10.1), three slots (8192 x 8192: 18.2 -> 17.2)
 //   then four waves and 32, 48 or 64 columns, whichever leaves the fullest CU
 //   the fewest (4096 x 22016: 48 20.2, 32 20.7, 64 21.1; 28672: 64 24.4, 32 26.3, 48 28.2);
@@ -61,14 +63,15 @@ __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
     // (the block it begins with: another one for the XCDs' workgroups, and within an XCD)
     const int first = mine > 1 && mine <= 64 ? (int)((blockIdx.x / 8 + blockIdx.x) % mine) : 0;
     auto turn = [&](int i) { return i + first < mine ? i + first : i + first - mine; };
-    auto load = [&](int s, int i) {  // the wave's block i to slot s (past the last: zeros)
-        const int b = i < mine ? wave + turn(i) * W : KB, bs = min(b, KB - 1), so = bs * kBlock;
+    auto load = [&](int s, int i) {  // the wave's block i to slot s
+        if (i >= mine) return;
+        const int b = wave + turn(i) * W;
         const bool in = b * kBlock + chunk < a.K;  // (K ends inside the last block)
-        lds4(rsrc(a.sx + bs * a.sx_stride, a.M * 4), lds_at(sx[s][wave]), lane * 4);
+        lds4(rsrc(a.sx + b * a.sx_stride, a.M * 4), lds_at(sx[s][wave]), lane * 4);
 #pragma unroll
-        for (int j = 0; j < 2 * NT; ++j) lds16(rw, part + s * PART + j * 1024, in ? vw[j] : kOutside, so);
+        for (int j = 0; j < 2 * NT; ++j) lds16(rw, part + s * PART + j * 1024, in ? vw[j] : kOutside, b * kBlock);
 #pragma unroll
-        for (int j = 0; j < XD; ++j) lds16(rx, part + s * PART + (2 * NT + j) * 1024, in ? vx[j] : kOutside, so);
+        for (int j = 0; j < XD; ++j) lds16(rx, part + s * PART + (2 * NT + j) * 1024, in ? vx[j] : kOutside, b * kBlock);
     };
     auto load_sw = [&](int i) {  // the weight's scales of the wave's blocks i to i + 63
         const int v = (wave + (i + lane) * W) * 4;
@@ -93,7 +96,13 @@ __global__ __launch_bounds__(64 * W) void mv_kernel(MmArgs a) {
             load_sw(i);
             wait_loads<0, false>();
         }
-        wait_loads<(S - 1) * (ND + 1), false>();  // (the other slots' may be in flight)
+        // (the other slots' may be in flight)
+        static_assert(S <= 4, "a wait for each number of them");
+        const int others = min(S - 1, mine - 1 - i);
+        if (others == 0) wait_loads<0, false>();
+        if (others == 1) wait_loads<ND + 1, false>();
+        if (others == 2) wait_loads<2 * (ND + 1), false>();
+        if (others == 3) wait_loads<3 * (ND + 1), false>();
         const int is = turn(i) % 64;
         const float w0 = sw[0][wave][is], w1 = CROSS ? sw[CROSS][wave][is] : 0.0f;
         Frag<true> w[NT];
@@ -141,8 +150,8 @@ struct Shape {
 };
 
 Shape shape(const st_context *ctx, const MmArgs &a) {
-    const int tiles = (a.N + 15) / 16, cus = ctx->num_cus, KB = blocks(a.K);
-    if (tiles <= cus) return {1, a.M <= 16 && KB >= 16 ? 16 : 8, true};  // (11008 x 4096: 16 waves 12.0 us, 8 12.3)
+    const int tiles = (a.N + 15) / 16, cus = ctx->num_cus;
+    if (tiles <= cus) return {1, 8, true};
     if (a.M > 32) return {2, 4, false};
     if (5 * tiles <= 6 * cus) return {1, a.M <= 16 ? 8 : 4, false};  // (several workgroups a CU: no second round for a few)
     if (tiles <= 2 * cus) return {2, 8, false};
@@ -168,7 +177,7 @@ void by_shape(st_context *ctx, const MmArgs &a, Shape s) {
         s.nt == 1 ? run<MT, X8, 1, 8>(ctx, a) : run<MT, X8, 2, 4>(ctx, a);
     } else {
         if constexpr (MT == 1) {
-            if (s.deep) return s.w == 16 ? run<MT, X8, 1, 16, X8 ? 3 : 2>(ctx, a) : run<MT, X8, 1, 8, 4>(ctx, a);
+            if (s.deep) return run<MT, X8, 1, 8, 4>(ctx, a);
             if (s.nt == 1) return run<MT, X8, 1, 8>(ctx, a);
             if (s.nt == 4) return run<MT, X8, 4, 4>(ctx, a);
         } else {

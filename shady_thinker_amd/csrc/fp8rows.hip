@@ -2,6 +2,15 @@
 // st_add_rmsnorm (the residual's addition and the norm before a linear; the
 // reference's rmsnorm.wgsl / add_rmsnorm.wgsl, src/model.rs:685-691, 799, 820)
 // and st_fp8_quant (rows, or silu(a) b, before the output and down projections).
+//   r = residual + x,  y = r (mean r^2 + eps)^-1/2 (weight + 0 or 1)
+//   s_b = max |y_k| / 448 over the block b,  q_k = e4m3(y_k / s_b)
+// Bound by HBM: every value is read and written once, in registers between. 4096
+// rows: norms of 4096 dims, f32 43.0 us (5.1 TB/s), f16 25.2 (4.7), of 8192 f32
+// 80.6 (5.4), silu of 11008 46.4 (4.9); a copy of 1 GiB runs at 5.1. A row is a
+// workgroup of the norm (its sum goes through LDS once), 256 threads of 2048 dims
+// one of the quantising. Few rows are a launch and a chain of latencies: one row
+// of 4096 3.2 us, one of silu of 11008 2.4. f32 arithmetic; a value is rounded
+// once to e4m3 (2^-4), the residual once to its type.
 #include "fp8.hpp"
 
 #include <algorithm>
