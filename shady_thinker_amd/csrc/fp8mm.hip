@@ -322,7 +322,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
     // What the DMAs read: a lane's first row of x, and of w (each wave column's
     // first 64 rows are the first half); rows past the tile's last lie outside the resources.
     const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    int vx, vw;
+    unsigned vx, vw;
     Rsrc rx, rw;
     const unsigned part_x = lds_at(lds + wave * DX * 1024), part_w = lds_at(lds + wave * DW * 1024);  // the wave's part of a place
     unsigned lds_x = part_x, lds_w = part_w;
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
         settle(rx, rw);
     };
     static_assert(HN % (DW * 8) == 0, "a wave's rows of w are neighbours");
-    auto dma = [&](Rsrc rs, unsigned to, int v, int b) { lds16(rs, to, b * kBlock + chunk < a.K ? v : kOutside, b * kBlock); };
+    auto dma = [&](Rsrc rs, unsigned to, unsigned v, int b) { lds16(rs, to, b * kBlock + chunk < a.K ? v : (unsigned)kOutside, b * kBlock); };
     auto dma_x = [&](int to, int b, int j) { dma(rx, lds_x + to + j * 1024, vx + j * 8 * a.K, b); };
     auto dma_a = [&](int to, int b, int j) { dma(rw, lds_w + to + j * 1024, vw + j * 8 * a.K, b); };
     auto dma_b = [&](int to, int b, int j) { dma(rw, lds_w + to + j * 1024, vw + (HN + j * 8) * a.K, b); };
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(512, 2) void wide_kernel(MmArgs a) {
 // of workgroups a start and end and K's blocks, which take longer where all CUs
 // load at once; slices add their sums' way through memory. Over 171 such shapes
 // the chosen tile and slices take 0.2 to 0.5 % longer at the mean than the best
-// ones (two boxes, cold and not), 17 % at the most.
+// ones (two cards, cold and not), 17 % at the most.
 enum Kind { MV, R64x64, R64x128, R128x64, R128x128, R128x256, R256x128, R256x256 };
 struct Rate {
     double few, all;  // a block on few of the CUs, on all (0: not built)

@@ -76,7 +76,7 @@ __device__ __forceinline__ void settle(Rsrc &a, Rsrc &b) {
     a = scalar(a), b = scalar(b);
     asm volatile("s_nop 4" : "+s"(a), "+s"(b));
 }
-__device__ __forceinline__ void lds16(Rsrc r, unsigned lds, int voff, int soff) {  // (r settled)
+__device__ __forceinline__ void lds16(Rsrc r, unsigned lds, unsigned voff, int soff) {  // (r settled)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
 __device__ __forceinline__ void lds4(Rsrc r, unsigned lds, int voff) {

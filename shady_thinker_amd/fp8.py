@@ -78,9 +78,17 @@ class Fp8Rows:
         if scale.shape != (fp8_blocks(k), m) or (m > 1 and scale.stride(1) != 1) or scale.device != data.device:
             raise ValueError(f"Fp8Rows: scale {tuple(scale.shape)}, strides {scale.stride()}, on {scale.device} (need "
                              f"[{fp8_blocks(k)}, {m}], a block's side by side, on {data.device})")
-        self.data, self.scale, self.M, self.K = data, scale, m, k
+        self._data, self._scale, self.M, self.K = data, scale, m, k
         self.stride = max(scale.stride(0), m) if scale.shape[0] > 1 else m
         self._at, self._scale_at, self._device = data.data_ptr(), scale.data_ptr(), data.get_device()
+
+    @property
+    def data(self):
+        return self._data
+
+    @property
+    def scale(self):
+        return self._scale
 
     def __getitem__(self, rows: slice) -> "Fp8Rows":
         """Rows [a:b] of these, sharing their memory."""

@@ -237,7 +237,7 @@ def fp8_blocks(n: int) -> int:
     return -(-n // FP8_BLOCK)
 
 
-@dataclass
+@dataclass(frozen=True)
 class Fp8Weight:
     """e4m3 weight of a block-scaled checkpoint: w float8_e4m3fn [N, K]
     row-major, scale f32 [ceil(N / 128), ceil(K / 128)] (what such files call
@@ -249,21 +249,23 @@ class Fp8Weight:
     N: int
 
     def __post_init__(self):
-        self._at, self._scale_at, self._device = self.w.data_ptr(), self.scale.data_ptr(), self.w.get_device()
+        torch, w, scale = _torch(), self.w, self.scale
+        if w.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
+            raise TypeError(f"Fp8Weight: w {w.dtype} (need float8_e4m3fn), scale {scale.dtype} (need float32)")
+        if tuple(w.shape) != (self.N, self.K) or not w.is_contiguous() or w.numel() == 0 or self.K % 16:
+            raise ValueError(f"Fp8Weight: w {tuple(w.shape)} (need contiguous [{self.N}, {self.K}], K a multiple of 16)")
+        need = (fp8_blocks(self.N), fp8_blocks(self.K))
+        if tuple(scale.shape) != need or not scale.is_contiguous() or scale.device != w.device:
+            raise ValueError(f"Fp8Weight: scale {tuple(scale.shape)} on {scale.device} (need contiguous {need} on {w.device})")
+        for name, value in (("_at", w.data_ptr()), ("_scale_at", scale.data_ptr()), ("_device", w.get_device())):
+            object.__setattr__(self, name, value)
 
     @classmethod
     def of(cls, w, scale) -> "Fp8Weight":
         """A weight over the caller's device tensors."""
-        torch = _torch()
-        if w.dtype is not torch.float8_e4m3fn or scale.dtype is not torch.float32:
-            raise TypeError(f"Fp8Weight: w {w.dtype} (need float8_e4m3fn), scale {scale.dtype} (need float32)")
-        if w.dim() != 2 or not w.is_contiguous() or w.numel() == 0 or w.shape[1] % 16:
-            raise ValueError(f"Fp8Weight: w {tuple(w.shape)} (need contiguous [N, K], K a multiple of 16)")
-        N, K = w.shape
-        need = (fp8_blocks(N), fp8_blocks(K))
-        if tuple(scale.shape) != need or not scale.is_contiguous() or scale.device != w.device:
-            raise ValueError(f"Fp8Weight: scale {tuple(scale.shape)} on {scale.device} (need contiguous {need} on {w.device})")
-        return cls(w, scale, K, N)
+        if w.dim() != 2:
+            raise ValueError(f"Fp8Weight: w {tuple(w.shape)} (need [N, K])")
+        return cls(w, scale, w.shape[1], w.shape[0])
 
     @classmethod
     def upload(cls, gpu, w, scale) -> "Fp8Weight":

@@ -72,6 +72,18 @@ def test_weight_refusals(w, scale):
         sta.Fp8Weight.of(w, scale)
 
 
+def test_tensors_stay():
+    """What a handle's pointers are of is not exchanged, and a weight is what it
+    says, however it is made."""
+    r, w = rows(), weight()
+    for obj, name in ((r, "data"), (r, "scale"), (w, "w"), (w, "scale"), (w, "K")):
+        with pytest.raises(AttributeError):
+            setattr(obj, name, getattr(obj, name))
+    for k, n in ((K + 16, N), (K, N + 1), (N, K)):
+        with pytest.raises(ValueError):
+            sta.Fp8Weight(w.w, w.scale, k, n)
+
+
 def test_weight_upload_and_cat():
     a, b = weight_of(torch.randn(256, K)), weight_of(torch.randn(40, K))
     w = sta.Fp8Weight.cat([sta.Fp8Weight.upload(G, *a), sta.Fp8Weight.upload(G, b[0], b[1].to(torch.bfloat16))])
