@@ -199,7 +199,8 @@ namespace f8 {
 // to 22016).
 double mv_us(const st_context *ctx, const MmArgs &a) {
     const Shape s = shape(ctx, a);
-    return 2.3 + std::max(0.6, (double)((a.N + 15) / 16) / s.nt / ctx->num_cus) * blocks(a.K) * (s.nt == 1 ? 0.205 : 0.345);
+    const double rounds = (double)((a.N + 15) / 16) / s.nt / ctx->num_cus;
+    return 2.3 + std::max(0.6, rounds) * blocks(a.K) * (s.nt == 1 ? 0.205 : rounds <= 1.0 ? 0.28 : 0.345);
 }
 
 int mv(st_context *ctx, const MmArgs &a) {

@@ -446,6 +446,30 @@ def test_graphs_share_the_workspace(gpu):
             assert all(torch.equal(y, v) for (_, _, y), v in zip(calls, want))
 
 
+def test_two_contexts_at_once(gpu):
+    """Contexts of their own on streams of their own, products in slices and
+    norms in flight on both: each keeps its workspace."""
+    other, out = sta.GpuContext(0), []
+    for ctx, seed in ((gpu, 1), (other, 2)):
+        m, k, n = 100, 2064, 520
+        x8, sx, w8, sw = gemm_case(seed, m, k, n)
+        r, w = rand(seed, m, k), rand(seed + 5, k)
+        out.append((ctx, torch.cuda.Stream(), sta.Fp8Rows.of(x8, sx), sta.Fp8Weight.of(w8, sw), torch.empty(m, n, dtype=F16, device=DEV), r, w,
+                    sta.Fp8Rows(ctx, m, k)))
+    torch.cuda.synchronize()
+    with gpu.tuning(FP8_TILE=4, FP8_SPLITS=4), other.tuning(FP8_TILE=4, FP8_SPLITS=4):
+        for _ in range(10):
+            for ctx, stream, x, w, y, r, gain, rows in out:
+                with torch.cuda.stream(stream):
+                    sta.fp8_gemm(ctx, x, w, y)
+                    sta.add_rmsnorm(ctx, r, gain, rows=rows)
+        torch.cuda.synchronize()
+    for _, _, x, w, y, r, gain, rows in out:
+        check_product(y, x.data, x.scale, w.w, w.scale)
+        s = r.double().cpu()
+        check_rows(rows.data, rows.scale, s / torch.sqrt((s * s).mean(-1, keepdim=True) + 1e-6) * gain.double().cpu(), norm_err(r.shape[1]))
+
+
 def test_gemm_past_32_bits(gpu):
     """A weight and rows of more than 2^32 bytes: the last columns and rows."""
     k, n = 32768, 135000
