@@ -12,8 +12,9 @@
 //  * otherwise e4m3 goes to f16, exactly, and the products of
 //    v_mfma_f32_16x16x32_f16 are exact in its f32 sums. Half the rate.
 // One FMA with the block's factor adds its sum to the accumulator: 4 FMAs beside
-// an instruction of 32 cycles, which fit under it (without them 8192^3 runs
-// 454 -> 425 us). The weight is the A operand, so that a lane holds four
+// an instruction of 32 cycles, which fit under it but draw power (8192^3, a
+// workgroup a tile: 454 us, without them 425; instructions alone on random
+// operands 3.9 PFLOP/s, with them 3.6). The weight is the A operand, so that a lane holds four
 // neighbouring n of one token, whose factor is then one register.
 //
 // Both kernels keep a block of both operands in LDS, brought by DMA while the
@@ -37,7 +38,7 @@ using namespace st::f8;
 constexpr int kMostRows = 1 << 28;
 constexpr int D = 3;      // instructions between one and its FMAs
 constexpr int kPanel = 6; // tiles along the tokens that run side by side: an XCD's 32 CUs then
-                          // share 6 strips of x and 5 of w in its L2 (4096 x 4096 x 22016: all 16 409 us, 8 390, 6 367, 4 384)
+                          // share 6 strips of x and 5 of w in its L2 (4096 x 4096 x 22016 in 128 x 256: all 387 us, 8 381, 6 370, 4 384; in 256 x 256: 348, 343, 338, 338)
 
 struct Place {
     int m0, n0, split;
