@@ -27,7 +27,6 @@
 #include "fp8mm.hpp"
 
 #include <algorithm>
-#include <cmath>
 
 #include "xcd.hpp"
 
