@@ -361,9 +361,10 @@ int st_int8_repack(st_context *ctx, const int8_t *w, int8_t *w_tiled, int K, int
  *   weight  w [N][K] row-major with w_scale [ceil(N / 128)][ceil(K / 128)]: one
  *           for each 128 x 128
  * K is a multiple of 16; it and N may end inside a block. Quantising makes a
- * block's scale max|x| / 448, at least 2^-126, and rounds x / scale to nearest,
- * even. A block with a NaN has a NaN scale; one with an infinity an infinite
- * scale, its infinities 448 of their sign and the rest 0. */
+ * block's scale max|x| times the f32 nearest to 1 / 448, at least 2^-126, and
+ * rounds the f32 quotient x / scale to nearest, even. A block with a NaN has a
+ * NaN scale; one with an infinity an infinite scale, its infinities 448 of their
+ * sign and the rest 0. */
 
 /* r = residual + x and its RMS norm y = r / sqrt(mean(r^2) + eps) * weight
  * (1 + weight: ST_FLAG_NORM_PLUS_ONE), to e4m3 rows (y8, y_scale), to y, or to

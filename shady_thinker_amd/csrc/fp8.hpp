@@ -79,8 +79,9 @@ __device__ __forceinline__ float add_turned(float v) {
 __device__ __forceinline__ float row_sum(float v) { return add_turned<1>(add_turned<2>(add_turned<4>(add_turned<8>(v)))); }
 
 // The scale of a block whose 128 values lie in 16 lanes side by side, eight in
-// each: max |x| / 448, at least 2^-126. Magnitudes compare as their bits do,
-// with NaN above infinity, so that a NaN in a block makes its scale NaN.
+// each: max |x| times the f32 nearest to 1 / 448, at least 2^-126. Magnitudes
+// compare as their bits do, with NaN above infinity, so that a NaN in a block
+// makes its scale NaN.
 __device__ __forceinline__ float block_scale(const float (&x)[8]) {
     unsigned m = 0;
 #pragma unroll
@@ -93,15 +94,22 @@ __device__ __forceinline__ float block_scale(const float (&x)[8]) {
     return s < kLeast ? kLeast : s;
 }
 
-// Eight values over their block's scale, each rounded once to e4m3 (to
-// nearest, even). The reciprocal and the product are f32 (2^-23 of a value
-// before a rounding of 2^-4). An infinity (0 times infinity here, so the
-// smaller of NaN and 448) is 448 of its sign.
+// Eight values over their block's scale, each quotient rounded to f32 and then to
+// e4m3 (to nearest, even). A product with the reciprocal alone may be a step off,
+// which takes a quotient at the middle of two e4m3 values (common: f16 values
+// over a scale of few bits) to either; its remainder, exact in an FMA, corrects it
+// (4096 rows of silu of 11008 44.4 -> 44.8 us). An infinity (0 times infinity
+// here, so the smaller of NaN and 448) is 448 of its sign.
 __device__ __forceinline__ u32x2 to_e4m3(const float (&x)[8], float scale) {
-    const float inv = __builtin_amdgcn_rcpf(scale);
+    const float d = scale < __builtin_inff() ? scale : 0.0f;  // (no remainders where the quotients are 0 or NaN)
+    float inv = __builtin_amdgcn_rcpf(scale);
+    inv = fmaf(fmaf(-d, inv, 1.0f), inv, inv);
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = copysignf(fminf(fabsf(x[i] * inv), kMost), x[i]);
+    for (int i = 0; i < 8; ++i) {
+        const float q = x[i] * inv;
+        v[i] = copysignf(fminf(fabsf(fmaf(fmaf(-d, q, x[i]), inv, q)), kMost), x[i]);
+    }
     u32x2 r;
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
     r.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
