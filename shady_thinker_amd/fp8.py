@@ -78,8 +78,10 @@ class Fp8Rows:
         if scale.shape != (fp8_blocks(k), m) or (m > 1 and scale.stride(1) != 1) or scale.device != data.device:
             raise ValueError(f"Fp8Rows: scale {tuple(scale.shape)}, strides {scale.stride()}, on {scale.device} (need "
                              f"[{fp8_blocks(k)}, {m}], a block's side by side, on {data.device})")
+        self.stride = scale.stride(0) if scale.shape[0] > 1 else m
+        if self.stride < m:
+            raise ValueError(f"Fp8Rows: scale {tuple(scale.shape)}, strides {scale.stride()}: a block's scales overlap the next one's")
         self._data, self._scale, self.M, self.K = data, scale, m, k
-        self.stride = max(scale.stride(0), m) if scale.shape[0] > 1 else m
         self._at, self._scale_at, self._device = data.data_ptr(), scale.data_ptr(), data.get_device()
 
     @property
