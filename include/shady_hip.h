@@ -378,9 +378,10 @@ int st_int8_repack(st_context *ctx, const int8_t *w, int8_t *w_tiled, int K, int
  *   y         y_dtype (ST_F32 or ST_F16) or NULL; it may be x's buffer, or the
  *             residual's where the sum does not go there
  *   *_stride  elements from one row to the next
- * Buffers that are one have one type and stride. f32 arithmetic. M less than
- * 2^22; D a multiple of 16, at most 32768. Pointers and strides in whole 16 bytes
- * (y_scale: 4). */
+ * residual_out may also be x's buffer. Buffers that are one have one type and
+ * stride; otherwise outputs share no element with another argument. f32
+ * arithmetic. M less than 2^22; D a multiple of 16, at most 32768. Pointers and
+ * strides in whole 16 bytes (y_scale: 4). */
 int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dtype, int64_t res_stride, const void *x,
                    int x_dtype, int64_t x_stride, void *residual_out, int64_t out_stride, const float *weight,
                    float eps, void *y, int y_dtype, int64_t y_stride, uint8_t *y8, float *y_scale,

@@ -3,6 +3,8 @@
 // their entry points share.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.hpp"
 
 namespace st {
@@ -119,6 +121,11 @@ __device__ __forceinline__ u32x2 to_e4m3(const float (&x)[8], float scale) {
 }
 
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+inline bool one_of(const void *p, std::initializer_list<const void *> others) {
+    for (const void *o : others)
+        if (p && p == o) return true;
+    return false;
+}
 inline int blocks(int n) { return (n + kBlock - 1) / kBlock; }
 inline bool act_dtype(int d) { return d == ST_F32 || d == ST_F16; }
 inline bool whole16(int64_t elements, int dtype) { return elements % (dtype == ST_F32 ? 4 : 8) == 0; }

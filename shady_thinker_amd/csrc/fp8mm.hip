@@ -614,6 +614,7 @@ extern "C" int st_fp8_gemm(st_context *ctx, const uint8_t *x, const float *x_sca
         return st::fail(ST_ERR_SHAPE, "%s: M=%d, N=%d (each at most 2^28, fewer than 2^22 blocks of 128 x 128)", fn, M, N);
     if (!st::aligned16(x) || !st::aligned16(w) || !st::aligned16(y) || !aligned4(x_scale) || !aligned4(w_scale))
         return st::fail(ST_ERR_ALIGN, "%s: pointers must be 16-byte aligned (scales: 4)", fn);
+    if (one_of(y, {x, x_scale, w, w_scale})) return st::fail(ST_ERR_INVALID, "%s: y in an input's buffer", fn);
     const MmArgs a{x, w, x_scale, w_scale, y, scale_stride, M, K, N, y_dtype == ST_F32};
     const st::OnDevice on(ctx);
     if (on.error != hipSuccess) return st::hip_fail(on.error, fn);

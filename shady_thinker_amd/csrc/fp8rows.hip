@@ -188,6 +188,11 @@ extern "C" int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dty
         return st::fail(ST_ERR_INVALID, "%s: residual_out in residual's buffer with another stride", fn);
     if (y && y == residual_out) return st::fail(ST_ERR_INVALID, "%s: y in residual_out's buffer", fn);
     if ((int64_t)M * 1024 > 0xFFFFFFFF) return st::fail(ST_ERR_SHAPE, "%s: M=%d (fewer than 2^22)", fn, M);
+    if (x && residual_out == x && (res_dtype != x_dtype || out_stride != x_stride))
+        return st::fail(ST_ERR_INVALID, "%s: residual_out in x's buffer with another type or stride", fn);
+    if (weight == y || weight == residual_out || one_of(y8, {residual, x, residual_out, weight, y}) ||
+        one_of(y_scale, {residual, x, residual_out, weight, y, y8}))
+        return st::fail(ST_ERR_INVALID, "%s: an output in another argument's buffer", fn);
     NormArgs a{};
     a.res = residual, a.x = x, a.res_out = residual_out, a.weight = weight, a.y = y, a.y8 = y8, a.scale = y_scale;
     a.res_stride = res_stride, a.x_stride = x_stride, a.out_stride = out_stride, a.y_stride = y_stride, a.scale_stride = scale_stride;
@@ -217,6 +222,7 @@ extern "C" int st_fp8_quant(st_context *ctx, const void *a, const void *b, int d
     q.a = a, q.b = b, q.a_stride = a_stride, q.b_stride = b_stride, q.scale_stride = scale_stride;
     q.y8 = y8, q.scale = y_scale, q.pieces = K / 8, q.units = (K / 8 + 255) / 256;
     if ((int64_t)M * q.units * 256 > 0xFFFFFFFF) return st::fail(ST_ERR_SHAPE, "%s: M=%d rows of %d are too many", fn, M, K);
+    if (one_of(y8, {a, b}) || one_of(y_scale, {a, b, y8})) return st::fail(ST_ERR_INVALID, "%s: an output in another argument's buffer", fn);
     const st::OnDevice on(ctx);
     if (on.error != hipSuccess) return st::hip_fail(on.error, fn);
     const dim3 grid((unsigned)(M * q.units)), block(256);
