@@ -128,7 +128,7 @@ typedef enum {
     ST_TUNE_I4MM_PAIR,         /* f16-MFMA gate/up: 0 gives each wave one source (default 1: both sources of a tile per wave) */
     ST_TUNE_I4MM_PREPASS,      /* f16-MFMA GPTQ decode, f32 x: 1 splits x in a pre-pass launch (default: in the kernel, unless act-order) */
     ST_TUNE_I4MM_SPLIT_TILES,  /* f16-MFMA GPTQ decode on at most one 16-column tile per CU: 0 keeps the limb kernels */
-    ST_TUNE_FP8_TILE,          /* st_fp8_gemm: tokens x columns of a workgroup: 0 the few tokens' kernel (up to 64), 1 64 x 64, 2 64 x 128, 3 128 x 64, 4 128 x 128, 5 128 x 256, 6 256 x 128, 7 256 x 256 (6: not for f16 y of more than 64 tokens; 5, 7: only for it; 7: K of more than 128) */
+    ST_TUNE_FP8_TILE,          /* st_fp8_gemm: tokens x columns of a workgroup: 0 the few tokens' kernel (up to 64), 1 64 x 64, 2 64 x 128, 3 128 x 64, 4 128 x 128, 5 128 x 256, 6 256 x 128, 7 256 x 256 (6: not for f16 y of more than 64 tokens; 5, 7: only for it; 7: K of more than 128; one that is not built for the call, or too small for a launch, gives way to the automatic choice) */
     ST_TUNE_FP8_SPLITS,        /* st_fp8_gemm with a tile set: slices of K (1, 2, 4 or 8) */
     ST_TUNE_COUNT
 } st_tune;

@@ -540,18 +540,23 @@ Plan plan(const st_context *ctx, const MmArgs &a) {
     if (can_mv && (forced == MV || (forced < 0 && a.M <= 48))) return best;
     double least = can_mv ? mv_us(ctx, a) : 1e30;
     const int KB = blocks(a.K);
+    auto tiles_of = [&](const Tile &t) { return (int64_t)((a.M + t.bm - 1) / t.bm) * ((a.N + t.bn - 1) / t.bn); };
+    // (a launch is of fewer than 2^32 threads: of the sizes that the call permits, f32 y in tiles of 64 x 64 can be more)
+    auto fits = [&](const Tile &t, int s) {
+        return tiles_of(t) * s * (t.kind == R64x64 && !exact ? 256 : 512) <= 0xFFFFFFFF && (s == 1 || (int64_t)a.M * a.N < (int64_t)1 << 33);
+    };
     // (the 256 x 256 kernel brings two blocks of K at once)
-    auto built = [&](const Tile &t) { return (exact ? t.by16 : t.by8).all != 0 && (t.kind != R256x256 || KB > 1); };
+    auto built = [&](const Tile &t) { return (exact ? t.by16 : t.by8).all != 0 && (t.kind != R256x256 || KB > 1) && fits(t, 1); };
     bool force = false;
     for (const Tile &t : kTiles) force |= t.kind == forced && built(t);
     if (force) least = 1e30;
     for (const Tile &t : kTiles) {
         if (!built(t) || (force ? t.kind != forced : a.M <= 64 && t.bm != 64)) continue;
         const Rate rate = exact ? t.by16 : t.by8;
-        const int64_t tiles = (int64_t)((a.M + t.bm - 1) / t.bm) * ((a.N + t.bn - 1) / t.bn);
+        const int64_t tiles = tiles_of(t);
         for (int s = 1; s <= 8 && s <= KB; s *= 2) {
             const double sums = 4.0 * s * a.M * a.N;
-            if (s > 1 && (t.kind == R256x256 || sums > (double)ctx->ws_bytes)) break;
+            if (s > 1 && (t.kind == R256x256 || sums > (double)ctx->ws_bytes || !fits(t, s))) break;
             const int64_t rounds = tiles * s / ctx->num_cus;
             const double rest = (double)(tiles * s % ctx->num_cus) / ctx->num_cus;
             const auto round = [&](double on) { return t.ends + (KB + s - 1) / s * std::max(rate.few, rate.all * on); };
@@ -609,7 +614,8 @@ extern "C" int st_fp8_gemm(st_context *ctx, const uint8_t *x, const float *x_sca
     if (M < 1 || N < 1 || K < 16 || K % 16 || K > (1 << 22))
         return st::fail(ST_ERR_SHAPE, "%s: M=%d, K=%d (a multiple of 16, at most 2^22), N=%d", fn, M, K, N);
     if (scale_stride < M) return st::fail(ST_ERR_SHAPE, "%s: a block's scales overlap the next one's", fn);
-    // (a launch is of fewer than 2^32 threads; the smallest tile is 128 x 64 for 512, of at most 64 tokens 32 columns for 256)
+    // (a launch is of fewer than 2^32 threads: of at most 64 tokens 256 for 32 columns, or 512 for 64; of more plan() takes
+    // tiles that fit, and 128 x 128 for 512 always does)
     if (M > kMostRows || N > kMostRows || (int64_t)blocks(M) * blocks(N) >= (1 << 22))
         return st::fail(ST_ERR_SHAPE, "%s: M=%d, N=%d (each at most 2^28, fewer than 2^22 blocks of 128 x 128)", fn, M, N);
     if (!st::aligned16(x) || !st::aligned16(w) || !st::aligned16(y) || !aligned4(x_scale) || !aligned4(w_scale))

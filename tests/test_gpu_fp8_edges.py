@@ -1,9 +1,10 @@
 """Calls of the 8-bit floating point operators that their documentation allows
-at its edges: the sum in x's buffer."""
+at its edges: the sum in the buffer of x, tiles and columns past a launch."""
 import pytest
 import torch
 
 import shady_thinker_amd as sta
+from shady_thinker_amd._lib import launches
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +26,22 @@ def test_sum_in_the_buffer_of_x(gpu, m, d, dtype):
     sta.add_rmsnorm(gpu, r, w, x, rows=again, residual_out=x)
     assert torch.equal(x, want) and torch.equal(rows.scale, again.scale)
     assert torch.equal(rows.data.view(torch.uint8), again.data.view(torch.uint8))
+
+
+def test_tiles_that_do_not_fit_a_launch(gpu, tune):
+    """65 tokens and 2^28 columns, f32 y: 64 x 64 would be 2^32 threads, more than
+    a launch has; the setting gives way to a tile that fits."""
+    m, k, n, b = 65, 16, 1 << 28, 1 << 16
+    tune(FP8_TILE=1)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randint(-8, 9, (m, k), device=DEV, generator=g).float()
+    part = torch.randint(-8, 9, (b, k), device=DEV, generator=g).float()
+    w = part.to(torch.float8_e4m3fn).view(torch.uint8).repeat(n // b, 1).view(torch.float8_e4m3fn)
+    scale = 2.0 ** (torch.arange(n // 128, device=DEV)[:, None] % 3).float()
+    y = torch.empty(m, n, device=DEV)
+    launches()
+    sta.fp8_gemm(gpu, sta.Fp8Rows.of(x.to(torch.float8_e4m3fn), torch.ones(1, m, device=DEV)), sta.Fp8Weight.of(w, scale), y)
+    assert launches() == ["fp8_ring_kernel"]
+    want = x @ part.t()  # (whole numbers: exact)
+    for n0 in (0, n // 2, n - b):
+        assert torch.equal(y[:, n0:n0 + b], want * scale[n0 // 128:(n0 + b) // 128, 0].repeat_interleave(128))
