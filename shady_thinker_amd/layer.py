@@ -59,6 +59,14 @@ def _mv(gpu, name, x, w: GptqWeight, y) -> None:
     M.gptq_matvec(gpu, name, x, w.qweight, w.scales, y, w.K, w.N, w.group_size, w.qzeros, w.perm, w.flags)
 
 
+def _need_gptq(what: str, weights: dict) -> None:
+    """An e4m3 layer is a self-attention one with all of its linears in e4m3
+    (Fp8DecoderLinears): others of its weights are refused by name."""
+    for name, w in weights.items():
+        if isinstance(w, Fp8Weight):
+            raise TypeError(f"{what}: {name} is an e4m3 weight (need GPTQ; e4m3 layers are self-attention, every linear e4m3)")
+
+
 class _Mlp:
     """The MLP shared by both layer kinds: gate, up (one fused call) and
     down, all GptqWeights of one group size."""
@@ -108,6 +116,7 @@ class DecoderLinears(_Mlp):
 
     def __init__(self, q: GptqWeight, k: GptqWeight, v: GptqWeight, o: GptqWeight, gate: GptqWeight,
                  up: GptqWeight, down: GptqWeight):
+        _need_gptq("DecoderLinears", dict(q=q, k=k, v=v, o=o, gate=gate, up=up, down=down))
         if not (q.K == k.K == v.K):
             raise ValueError("q, k and v must read the same hidden size")
         if o.N != q.K:
@@ -130,6 +139,7 @@ class DecoderLinears(_Mlp):
         missing = [n for n in names if n not in linears]
         if missing:
             raise KeyError(f"DecoderLinears.from_linears: no GPTQ linear {missing[0]}")
+        _need_gptq("DecoderLinears", {n: linears[n] for n in names})
         return cls(*(linears[n] for n in names))
 
     def decode(self, gpu, x, attn, qkv_out, o_out, h_out, down_out, xm=None) -> None:
@@ -169,6 +179,7 @@ class DeltaNetLinears(_Mlp):
 
     def __init__(self, in_qkv: GptqWeight, in_z: GptqWeight, out: GptqWeight, gate: GptqWeight, up: GptqWeight,
                  down: GptqWeight):
+        _need_gptq("DeltaNetLinears", dict(in_qkv=in_qkv, in_z=in_z, out=out, gate=gate, up=up, down=down))
         if in_qkv.K != in_z.K:
             raise ValueError("in_proj_qkv and in_proj_z must read the same hidden size")
         if out.K != in_z.N or out.N != in_qkv.K:
@@ -192,6 +203,7 @@ class DeltaNetLinears(_Mlp):
         missing = [n for n in names if n not in linears]
         if missing:
             raise KeyError(f"DeltaNetLinears.from_linears: no GPTQ linear {missing[0]}")
+        _need_gptq("DeltaNetLinears", {n: linears[n] for n in names})
         return cls(*(linears[n] for n in names))
 
     def z_of(self, qkv_out):
@@ -255,6 +267,9 @@ class Fp8DecoderLinears:
     fp8 = True
 
     def __init__(self, q: Fp8Weight, k: Fp8Weight, v: Fp8Weight, o: Fp8Weight, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight):
+        for name, w in dict(q=q, k=k, v=v, o=o, gate=gate, up=up, down=down).items():
+            if not isinstance(w, Fp8Weight):
+                raise TypeError(f"Fp8DecoderLinears: {name} is {type(w).__name__} (need e4m3, Fp8Weight)")
         if not (q.K == k.K == v.K == gate.K == up.K):
             raise ValueError("q, k, v, gate and up must read the same hidden size")
         if o.N != q.K:
@@ -305,7 +320,7 @@ def layer_from_linears(linears: dict, layer: int, layer_prefix: str = "model.lay
     """The layer's linears of whichever kind it is: self-attention when
     `{layer_prefix}.{i}.self_attn.q_proj` was loaded (the reference's test,
     src/weights.rs:247-250; Fp8DecoderLinears when that is an Fp8Weight),
-    DeltaNet otherwise."""
+    DeltaNet otherwise (GPTQ: an e4m3 one is refused)."""
     q = linears.get(f"{layer_prefix}.{layer}.self_attn.q_proj")
     if isinstance(q, Fp8Weight):
         return Fp8DecoderLinears.from_linears(linears, layer, layer_prefix)

@@ -127,7 +127,10 @@ def load_gptq_checkpoint(gpu, model_dir: str, tiled: bool = True) -> tuple[dict,
 
 def load_fp8_checkpoint(gpu, model_dir: str) -> tuple[dict, dict]:
     """Upload every e4m3 linear with block scales (`{prefix: Fp8Weight}`) and
-    the bf16 lm_head / embedding weights (`{name: device int16 tensor [N, K]}`)."""
+    the bf16 lm_head / embedding weights (`{name: device int16 tensor [N, K]}`).
+    Not returned: norm weights (ResidualNorms takes them from the caller) and
+    linears that the file keeps in bf16; a layer one of whose linears is missing
+    is refused when it is put together (layer_from_linears)."""
     import torch
     from safetensors import safe_open
 

@@ -1,13 +1,13 @@
 """Calls of the 8-bit floating point operators that are refused, on the CPU:
-scales that overlap, outputs in the buffers of inputs."""
+scales that overlap, outputs in the buffers of inputs, layers that are not built."""
 import ctypes
 
 import pytest
 import torch
 
 import shady_thinker_amd as sta
-from fp8_util import F8
-from shady_thinker_amd._lib import ST_F16, ST_F32, lib
+from fp8_util import F8, weight_of
+from shady_thinker_amd._lib import ST_F16, ST_F32, ST_FLAG_TILED, lib
 
 ST_ERR_INVALID = 1  # (st_status)
 
@@ -70,3 +70,48 @@ def test_quant_over_inputs(kw):
 @pytest.mark.parametrize("other", ["x", "x_scale", "w", "w_scale"])
 def test_product_over_inputs(other):
     refused("st_fp8_gemm", {**GEMM, "y": GEMM[other]}, "buffer")
+
+
+# --------------------------------------------------- layers that are not built
+def fp8_weight(n, k):
+    return sta.Fp8Weight.of(*weight_of(torch.ones(n, k)))
+
+
+def gptq_weight(n, k):
+    return sta.GptqWeight(torch.zeros(n * k // 8, dtype=torch.int32), torch.zeros(k // 128, n, dtype=torch.float16), None, None, k, n, 128,
+                          ST_FLAG_TILED)
+
+
+DELTA = {"linear_attn.in_proj_qkv": (384, 256), "linear_attn.in_proj_z": (128, 256), "linear_attn.out_proj": (256, 128)}
+MLP = {"mlp.gate_proj": (512, 256), "mlp.up_proj": (512, 256), "mlp.down_proj": (256, 512)}
+ATTENTION = {f"self_attn.{p}_proj": (256, 256) for p in "qkvo"}
+
+
+@pytest.mark.parametrize("e4m3", [{*DELTA, *MLP}, {*DELTA}, {*MLP}, {"linear_attn.out_proj"}, {"mlp.down_proj"}])
+def test_delta_net_layers_in_e4m3(e4m3):
+    """A hybrid model's linear attention in e4m3 is refused by its name."""
+    linears = {f"model.layers.4.{name}": (fp8_weight if name in e4m3 else gptq_weight)(*s) for name, s in {**DELTA, **MLP}.items()}
+    with pytest.raises(TypeError, match=r"DeltaNetLinears: model\.layers\.4\.\S+ is an e4m3 weight"):
+        sta.layer_from_linears(linears, 4)
+
+
+@pytest.mark.parametrize("e4m3", [{*MLP}, {"self_attn.o_proj"}])
+def test_mixed_layers(e4m3):
+    linears = {f"model.layers.0.{name}": (fp8_weight if name in e4m3 else gptq_weight)(*s) for name, s in {**ATTENTION, **MLP}.items()}
+    with pytest.raises(TypeError, match=r"DecoderLinears: model\.layers\.0\.\S+ is an e4m3 weight"):
+        sta.layer_from_linears(linears, 0)
+
+
+def test_layers_of_e4m3_by_hand():
+    g, f = [gptq_weight(*s) for s in (*DELTA.values(), *MLP.values())], [fp8_weight(*s) for s in (*DELTA.values(), *MLP.values())]
+    sta.DeltaNetLinears(*g)
+    for i in range(6):
+        with pytest.raises(TypeError, match="is an e4m3 weight"):
+            sta.DeltaNetLinears(*g[:i], f[i], *g[i + 1:])
+    g, f = [gptq_weight(*s) for s in (*ATTENTION.values(), *MLP.values())], [fp8_weight(*s) for s in (*ATTENTION.values(), *MLP.values())]
+    sta.DecoderLinears(*g)
+    for i in range(7):
+        with pytest.raises(TypeError, match="is an e4m3 weight"):
+            sta.DecoderLinears(*g[:i], f[i], *g[i + 1:])
+        with pytest.raises(TypeError, match="need e4m3"):
+            sta.Fp8DecoderLinears(*f[:i], g[i], *f[i + 1:])
