@@ -240,8 +240,12 @@ def linear(gpu, x, w, y) -> None:
         from .fp8 import Fp8Rows, fp8_gemm, fp8_quant
 
         m = _rows(x, w.K)
+        _need(y, "output", _ACT, m * w.N)
         rows = Fp8Rows(gpu, m, w.K)
-        fp8_quant(gpu, x.view(m, w.K), rows)
-        fp8_gemm(gpu, rows, w, y)
+        if x.shape != (m, w.K):  # (such an x may be a part of wider rows)
+            _need(x, "input", _ACT, m * w.K)
+            x = x.view(m, w.K)
+        fp8_quant(gpu, x, rows)
+        fp8_gemm(gpu, rows, w, y if y.shape == (m, w.N) else y.view(-1)[: m * w.N].view(m, w.N))
     else:
         raise TypeError(type(w))

@@ -1,5 +1,6 @@
 """Calls of the 8-bit floating point operators that are refused, on the CPU:
-scales that overlap, outputs in the buffers of inputs, layers that are not built."""
+scales that overlap, outputs in the buffers of inputs, layers that are not
+built, the shapes that linear() takes."""
 import ctypes
 
 import pytest
@@ -115,3 +116,37 @@ def test_layers_of_e4m3_by_hand():
             sta.DecoderLinears(*g[:i], f[i], *g[i + 1:])
         with pytest.raises(TypeError, match="need e4m3"):
             sta.Fp8DecoderLinears(*f[:i], g[i], *f[i + 1:])
+
+
+# --------------------------------------------------------------------- linear()
+class NoGpu:
+    handle = None
+    device = torch.device("cpu")
+
+    def sync_stream(self):
+        pass
+
+
+@pytest.mark.parametrize("xs,ys", [((144,), (40,)), ((3, 144), (3, 40)), ((2, 3, 144), (2, 3, 40)), ((3, 144), (130,))])
+def test_linear_shapes(monkeypatch, xs, ys):
+    seen = []
+    monkeypatch.setattr(sta.fp8, "call", lambda name, *a: seen.append((name, a[-3:])))
+    sta.linear(NoGpu(), torch.zeros(xs), fp8_weight(40, 144), torch.zeros(ys))
+    m = torch.zeros(xs).numel() // 144
+    assert seen[0][0] == "st_fp8_quant" and seen[0][1][-2:] == (m, 144) and seen[1] == ("st_fp8_gemm", (m, 144, 40))
+
+
+def test_linear_of_a_part_of_wider_rows(monkeypatch):
+    seen = []
+    monkeypatch.setattr(sta.fp8, "call", lambda name, *a: seen.append(a))
+    sta.linear(NoGpu(), torch.zeros(3, 288)[:, :144], fp8_weight(40, 144), torch.zeros(3, 40))
+    assert seen[0][4] == 288  # (a_stride)
+
+
+@pytest.mark.parametrize("x,y", [
+    (torch.zeros(3, 143), torch.zeros(3, 40)), (torch.zeros(3, 144), torch.zeros(3, 39)), (torch.zeros(3, 144).int(), torch.zeros(3, 40)),
+    (torch.zeros(144, 3).t(), torch.zeros(3, 40)), (torch.zeros(2, 2, 288)[..., :144], torch.zeros(4, 40)), (torch.zeros(3, 144), torch.zeros(40, 3).t()), (torch.zeros(3, 144), torch.zeros(3, 40).double())])
+def test_linear_refusals(monkeypatch, x, y):
+    monkeypatch.setattr(sta.fp8, "call", lambda *a: None)
+    with pytest.raises((ValueError, TypeError)):
+        sta.linear(NoGpu(), x, fp8_weight(40, 144), y)

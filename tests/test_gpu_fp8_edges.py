@@ -45,3 +45,18 @@ def test_tiles_that_do_not_fit_a_launch(gpu, tune):
     want = x @ part.t()  # (whole numbers: exact)
     for n0 in (0, n // 2, n - b):
         assert torch.equal(y[:, n0:n0 + b], want * scale[n0 // 128:(n0 + b) // 128, 0].repeat_interleave(128))
+
+
+@pytest.mark.parametrize("xs,ys", [((272,), (150,)), ((2, 3, 272), (2, 3, 150)), ((4, 272), (700,))])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_linear_of_any_shape(gpu, xs, ys, dtype):
+    """linear() takes x and y of any shape that holds the rows, as for the other
+    weights; what lies behind them is left alone."""
+    w8 = (rand(1, 150, 272) * 20).to(torch.float8_e4m3fn)
+    w, x, y = sta.Fp8Weight.of(w8, rand(2, 2, 3).abs()), rand(3, *xs), torch.full(ys, 7.0, dtype=dtype, device=DEV)
+    m = x.numel() // 272
+    rows, want = sta.Fp8Rows(gpu, m, 272), torch.empty(m, 150, dtype=dtype, device=DEV)
+    sta.linear(gpu, x, w, y)
+    sta.fp8_quant(gpu, x.view(m, 272), rows)
+    sta.fp8_gemm(gpu, rows, w, want)
+    assert torch.equal(y.view(-1)[:m * 150], want.view(-1)) and (y.view(-1)[m * 150:] == 7.0).all()
