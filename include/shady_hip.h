@@ -128,8 +128,9 @@ typedef enum {
     ST_TUNE_I4MM_PAIR,         /* f16-MFMA gate/up: 0 gives each wave one source (default 1: both sources of a tile per wave) */
     ST_TUNE_I4MM_PREPASS,      /* f16-MFMA GPTQ decode, f32 x: 1 splits x in a pre-pass launch (default: in the kernel, unless act-order) */
     ST_TUNE_I4MM_SPLIT_TILES,  /* f16-MFMA GPTQ decode on at most one 16-column tile per CU: 0 keeps the limb kernels */
-    ST_TUNE_FP8_TILE,          /* st_fp8_gemm: tokens x columns of a workgroup: 0 the few tokens' kernel (up to 64), 1 64 x 64, 2 64 x 128, 3 128 x 64, 4 128 x 128, 5 128 x 256, 6 256 x 128, 7 256 x 256 (6: not for f16 y of more than 64 tokens; 5, 7: only for it; 7: K of more than 128; one that is not built for the call, or too small for a launch, gives way to the automatic choice) */
+    ST_TUNE_FP8_TILE,          /* st_fp8_gemm: tokens x columns of a workgroup: 0 the few tokens' kernel (up to 64), 1 64 x 64, 2 64 x 128, 3 128 x 64, 4 128 x 128, 5 128 x 256, 6 256 x 128, 7 256 x 256 (6: not for f16 y of more than 64 tokens unless FP8_EXACT; 5, 7: only for it; 7: K of more than 128; one that is not built for the call, or too small for a launch, gives way to the automatic choice) */
     ST_TUNE_FP8_SPLITS,        /* st_fp8_gemm with a tile set: slices of K (1, 2, 4 or 8) */
+    ST_TUNE_FP8_EXACT,         /* st_fp8_gemm, f16 y of more than 64 tokens: 1 keeps products exact there too (default 0: see st_fp8_gemm) */
     ST_TUNE_COUNT
 } st_tune;
 int st_context_set_tune(st_context *ctx, int knob, int value);
@@ -396,11 +397,16 @@ int st_fp8_quant(st_context *ctx, const void *a, const void *b, int dtype, int64
 
 /* y[m][n] = sum_b x_scale[b][m] w_scale[n / 128][b] sum_{k in b} x8[m][k] w[n][k],
  * y [M][N] of y_dtype (ST_F32 or ST_F16), any M and N (at most 2^28, and fewer
- * than 2^22 blocks of 128 x 128 of y). Products are exact; sums are f32, in a
- * fixed order. x8, w and y 16-byte aligned (scales: 4). f32 y keeps f32 sums; so
- * does f16 y of at most 64 tokens. f16 y of more comes from the 8-bit matrix
- * instruction, which keeps a product to 2^-13 of the largest of its eight k
- * (rel-L2 3e-5 to 5e-5, beside 2.1e-4 of f16 itself). */
+ * than 2^22 blocks of 128 x 128 of y). x8, w and y 16-byte aligned (scales: 4).
+ * Sums are f32, in a fixed order for each size. With f32 y, and f16 y of at most
+ * 64 tokens, products are exact. f16 y of more tokens comes from the 8-bit matrix
+ * instruction, which keeps a product to 2^-13 of the power of two of the largest
+ * of its eight neighbouring k, so that sums which cancel lose what lies below,
+ * and a token's row is not quite the same in a batch of 64 and of 65. By rel-L2
+ * that is 1.4e-5 on normal activations, 2.8e-5 with some channels at 16 times the
+ * rest, 6.8e-5 with one at 1000 times (measured, weights normal), beside f16's own
+ * 2.1e-4. ST_TUNE_FP8_EXACT 1 keeps products exact there too, at up to twice the
+ * time. */
 int st_fp8_gemm(st_context *ctx, const uint8_t *x8, const float *x_scale, int64_t scale_stride, const uint8_t *w,
                 const float *w_scale, void *y, int y_dtype, int M, int K, int N);
 

@@ -26,7 +26,7 @@ ST_FLAG_ROPE_PAIRS = 0x8
 TUNE_KNOBS = ("DECODE_KERNEL", "STAGE_MODE", "STAGE_ROUNDS", "WAVES", "NO_COOP", "ONE_TILE", "NO_CHUNK", "NO_KSPLIT",
               "SPLIT_TILES_CU", "TOKEN_BLOCK", "I4MM_MIN_M", "I4MM_MIN_TILES", "I8MM_MIN_M", "GEMM_CB", "GEMM_NO_SPLIT",
               "STREAM_WAVES", "STREAM_TILES_WG", "STREAM_SYNC", "SPLIT_REDUCE_KERNEL", "I4MM_WAVES", "I4MM_PAIR", "I4MM_PREPASS",
-              "I4MM_SPLIT_TILES", "FP8_TILE", "FP8_SPLITS")
+              "I4MM_SPLIT_TILES", "FP8_TILE", "FP8_SPLITS", "FP8_EXACT")
 TUNE = {name: i for i, name in enumerate(TUNE_KNOBS)}
 
 STATUS_NAMES = {

@@ -7,8 +7,11 @@
 //  * v_mfma_f32_16x16x128_f8f6f4 takes the block whole. In each eight k it keeps
 //    a product to 2^-13 of the largest one's power of two (measured: a product
 //    of 2^-14 beside one of 1 is lost, in another eight it counts to 2^-23), so
-//    the sum is off by some 2^-15 of its magnitude: for f16 y, whose own
-//    rounding is 2^-12 at the mean, of more than 64 tokens.
+//    the sum is off by some 2^-15 of its magnitude (rel-L2 1.4e-5 on normal
+//    values, 6.8e-5 where one channel is 1000 times the rest): for f16 y, whose
+//    own rounding is 2.1e-4, of more than 64 tokens, unless the context asks for
+//    exact products (ST_TUNE_FP8_EXACT; 77 x 5120 x 13824 18 -> 30 us, 512 x 11008
+//    x 4096 35 -> 55, 4096 x 4096 x 22016 329 -> 648).
 //  * otherwise e4m3 goes to f16, exactly, and the products of
 //    v_mfma_f32_16x16x32_f16 are exact in its f32 sums. Half the rate.
 // One FMA with the block's factor adds its sum to the accumulator: 4 FMAs beside
@@ -533,15 +536,18 @@ struct Plan {
     int splits;
 };
 
+// Whether the f16 instruction sums, whose products are exact.
+bool exact_sums(const st_context *ctx, const MmArgs &a) { return a.f32 || a.M <= 64 || st::tune(ctx, ST_TUNE_FP8_EXACT, 0) > 0; }
+
 Plan plan(const st_context *ctx, const MmArgs &a) {
     const int forced = st::tune(ctx, ST_TUNE_FP8_TILE, -1), slices = st::tune(ctx, ST_TUNE_FP8_SPLITS, -1);
     Plan best{MV, 1};
-    const bool can_mv = a.M <= 64, exact = a.f32 || a.M <= 64;
+    const bool can_mv = a.M <= 64, exact = exact_sums(ctx, a);
     if (can_mv && (forced == MV || (forced < 0 && a.M <= 48))) return best;
     double least = can_mv ? mv_us(ctx, a) : 1e30;
     const int KB = blocks(a.K);
     auto tiles_of = [&](const Tile &t) { return (int64_t)((a.M + t.bm - 1) / t.bm) * ((a.N + t.bn - 1) / t.bn); };
-    // (a launch is of fewer than 2^32 threads: of the sizes that the call permits, f32 y in tiles of 64 x 64 can be more)
+    // (a launch is of fewer than 2^32 threads: of the sizes that the call permits, exact sums in tiles of 64 x 64 can be more)
     auto fits = [&](const Tile &t, int s) {
         return tiles_of(t) * s * (t.kind == R64x64 && !exact ? 256 : 512) <= 0xFFFFFFFF && (s == 1 || (int64_t)a.M * a.N < (int64_t)1 << 33);
     };
@@ -574,7 +580,7 @@ void run_ring(st_context *ctx, const MmArgs &a, int splits) {
 }
 
 int run(st_context *ctx, const MmArgs &a, Plan p) {
-    const bool exact = a.f32 || a.M <= 64;
+    const bool exact = exact_sums(ctx, a);
     const char *name = "fp8_ring_kernel";
     switch (p.kind) {
         case MV: return mv(ctx, a);

@@ -178,7 +178,10 @@ def fp8_quant(gpu, a, rows: Fp8Rows, b=None) -> None:
 
 
 def fp8_gemm(gpu, rows: Fp8Rows, w: Fp8Weight, y) -> None:
-    """y [M, N] (float32 or float16) = rows . w^T, M of any size."""
+    """y [M, N] (float32 or float16) = rows . w^T, M of any size. float16 y of
+    more than 64 tokens: the 8-bit matrix instruction cuts small products beside
+    large ones (st_fp8_gemm in the header says how far), unless
+    gpu.set_tune("FP8_EXACT", 1), at up to twice the time."""
     m, k, n, dev = rows.M, w.K, w.N, rows._device
     d = _DT.get(y.dtype)
     if (d is None or rows.K != k or y.shape != (m, n) or not y.is_contiguous() or y.get_device() != dev or w._device != dev

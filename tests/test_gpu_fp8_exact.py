@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import shady_thinker_amd as sta
-from fp8_util import B, F8, blocks, spread
+from fp8_util import B, F8, blocks, check_product, rows_of, spread, weight_of
 from shady_thinker_amd._lib import launches
 
 pytestmark = pytest.mark.gpu
@@ -134,3 +134,28 @@ def test_not_finite(gpu, tune, m, n, tile):
     fine_c = torch.ones(n, dtype=torch.bool, device=DEV)
     fine_r[rows], fine_c[cols] = False, False
     assert torch.equal(y[fine_r][:, fine_c], want[fine_r][:, fine_c])
+
+
+# ----------------------------------------------- exact products for f16 y, by choice
+@pytest.mark.parametrize("m,k,n", [(65, 2752, 515), (300, 1040, 260), (1030, 272, 776)])
+@pytest.mark.parametrize("tile,splits", [(-1, -1), (1, 1), (2, 4), (3, 1), (4, 4), (6, 1), (6, 4), (5, -1), (7, -1)])
+def test_exact_products(gpu, tune, m, k, n, tile, splits):
+    """FP8_EXACT: f16 y within the bound of f32 sums, whatever the batch; tiles of
+    the 8-bit instruction alone (5, 7) give way."""
+    tune(FP8_EXACT=1, FP8_TILE=tile, FP8_SPLITS=splits)
+    x8, sx = rows_of(torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(DEV) * (1.0 + 999.0 * (torch.arange(k, device=DEV) % 128 == 5)))
+    w8, sw = weight_of(torch.randn(n, k, generator=torch.Generator().manual_seed(n)).to(DEV))
+    y, ran = gemm(gpu, (x8, sx, w8, sw), F16)
+    assert ran[0] == "fp8_ring_kernel"
+    check_product(y, x8, sx, w8, sw, many=False)
+
+
+@pytest.mark.parametrize("m", [1, 64, 65, 300])
+@pytest.mark.parametrize("tile", [-1, 1, 2, 3, 4, 6])
+def test_exact_products_that_cancel(gpu, tune, m, tile):
+    """1 - 1 + 2^-14 of neighbouring k is 2^-14."""
+    tune(FP8_EXACT=1, FP8_TILE=tile)
+    x, w = torch.zeros(m, 272, device=DEV), torch.zeros(200, 272, device=DEV)
+    x[:, 160:163], w[:, 160:163] = torch.tensor([1.0, -1.0, 2.0**-7], device=DEV), torch.tensor([1.0, 1.0, 2.0**-7], device=DEV)
+    y, _ = gemm(gpu, (x.to(F8), torch.ones(3, m, device=DEV), w.to(F8), torch.ones(2, 3, device=DEV)), F16)
+    assert (y == 2.0**-14).all()
