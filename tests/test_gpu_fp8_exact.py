@@ -4,6 +4,7 @@ instruction cuts none, and every sum is a multiple of 1/2 below 2^23: f32 holds
 it whatever the order, and f16 y is its one rounding. A product, scale, row or
 column out of its place shows, however long K is."""
 import math
+import random
 
 import pytest
 import torch
@@ -159,3 +160,18 @@ def test_exact_products_that_cancel(gpu, tune, m, tile):
     x[:, 160:163], w[:, 160:163] = torch.tensor([1.0, -1.0, 2.0**-7], device=DEV), torch.tensor([1.0, 1.0, 2.0**-7], device=DEV)
     y, _ = gemm(gpu, (x.to(F8), torch.ones(3, m, device=DEV), w.to(F8), torch.ones(2, 3, device=DEV)), F16)
     assert (y == 2.0**-14).all()
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn(gpu, seed):
+    """Sizes spread over the range, tile and slices by the estimates; a part of
+    a larger batch's rows."""
+    rng = random.Random(seed)
+    spread_over = lambda lo, hi, step=1: max(lo, int(math.exp(rng.uniform(math.log(lo), math.log(hi)))) // step * step)
+    m, k, n = rng.choice([spread_over(1, 64), spread_over(65, 4096)]), spread_over(16, 12000, 16), spread_over(1, 12000)
+    dtype, skip = rng.choice([F16, F32]), rng.randint(0, 5)
+    x8, sx, w8, sw = case(seed, m + skip, k, n)
+    y = torch.full((m + 1, n), 7.0, dtype=dtype, device=DEV)
+    with gpu.tuning(FP8_EXACT=rng.choice([0, 1])):
+        sta.fp8_gemm(gpu, sta.Fp8Rows.of(x8, sx)[skip:], sta.Fp8Weight.of(w8, sw), y[:m])
+    assert torch.equal(y[:m], exact(x8[skip:], sx[:, skip:], w8, sw).to(dtype)) and (y[m] == 7.0).all()
