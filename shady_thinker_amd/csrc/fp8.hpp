@@ -98,19 +98,25 @@ __device__ __forceinline__ float block_scale(const float (&x)[8]) {
 
 // Eight values over their block's scale, each quotient rounded to f32 and then to
 // e4m3 (to nearest, even). A product with the reciprocal alone may be a step off,
-// which takes a quotient at the middle of two e4m3 values (common: f16 values
-// over a scale of few bits) to either; its remainder, exact in an FMA, corrects it
-// (4096 rows of silu of 11008 44.4 -> 44.8 us). An infinity (0 times infinity
-// here, so the smaller of NaN and 448) is 448 of its sign.
+// which takes a quotient at the middle of two e4m3 values to either (16 of a
+// million f16 values); its remainder, exact in an FMA, corrects it (0 keeps its
+// sign: -0 is added to it). 4096 f16 rows of silu of 11008 43.5 -> 43.8 us, without
+// silu 28.4, f32 77.7 and 43.4 as before. The largest is 448 within two steps, which rounds to
+// 448. Where the scale is not finite: 448 of its sign for an infinity (0 times
+// infinity, so the smaller of NaN and 448), 0 beside it, and 448 beside a NaN.
 __device__ __forceinline__ u32x2 to_e4m3(const float (&x)[8], float scale) {
-    const float d = scale < __builtin_inff() ? scale : 0.0f;  // (no remainders where the quotients are 0 or NaN)
     float inv = __builtin_amdgcn_rcpf(scale);
-    inv = fmaf(fmaf(-d, inv, 1.0f), inv, inv);
+    inv = fmaf(-fmaf(scale, inv, -1.0f), inv, inv);
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float q = x[i] * inv;
-        v[i] = copysignf(fminf(fabsf(fmaf(fmaf(-d, q, x[i]), inv, q)), kMost), x[i]);
+        v[i] = fmaf(-fmaf(scale, q, -x[i]), inv, q);
+    }
+    if (!(scale < __builtin_inff())) {
+        inv = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = copysignf(fminf(fabsf(x[i] * inv), kMost), x[i]);
     }
     u32x2 r;
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);

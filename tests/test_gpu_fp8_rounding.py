@@ -34,6 +34,7 @@ def values(kind, m, k, dtype):
         x = torch.randint(-200, 201, (m, k), generator=g).float()
     else:
         x = torch.randn(m, k, generator=g) * 2.0 ** torch.randint(-6, 7, (m, 1), generator=g)
+    x[:, 3::7] *= 0.0  # (zeros of both signs)
     if kind == "tiny" and dtype is F32:
         x = x * 2.0**-122  # (scales about the least one, subnormal values)
     return x.to(dtype)
