@@ -94,8 +94,10 @@ __device__ __forceinline__ void turned(i32x4 *s, const f32x4 (&v)[NT], T *y, int
 // BM x BN of y by WM x WN waves, S stages of LDS, K in slices where the tiles
 // alone leave CUs idle (f32 partial sums in the workspace, added in order by
 // reduce_kernel). Block b + S - 1 comes while b is multiplied. What bounds it is
-// the DMAs' way from the L2s (14 to 17 TB/s of all CUs; without the products and
-// their reads 512 x 11008 x 4096 takes 28 us of 33).
+// its loads: without the products and their reads it took 80 % of its time. DMAs
+// alone reach 14 to 17 TB/s from the L2s; the tiles bring 9 to 12 (512 x 11008 x
+// 4096 in 128 x 256, four slices: 270 MB in 30 us; 77 x 5120 x 13824 in 64 x 128:
+// 212 MB in 17.5, an eighth of it rows past the last), and why not more is open.
 template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN >= 8 ? 2 : 1) void ring_kernel(MmArgs a, float *part, int splits) {
     constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, STEPS = MT * NT;

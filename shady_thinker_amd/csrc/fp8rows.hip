@@ -5,8 +5,8 @@
 //   r = residual + x,  y = r (mean r^2 + eps)^-1/2 (weight + 0 or 1)
 //   s_b = max |y_k| / 448 over the block b,  q_k = e4m3(y_k / s_b)
 // Bound by HBM: every value is read and written once, in registers between. 4096
-// rows: norms of 4096 dims, f32 43.0 us (5.1 TB/s), f16 25.2 (4.7), of 8192 f32
-// 80.6 (5.4), silu of 11008 46.4 (4.9); a copy of 1 GiB runs at 5.1. A row is a
+// rows: norms of 4096 dims, f32 43.2 us (5.05 TB/s), f16 25.4 (4.6), of 8192 f32
+// 81.1 (5.4), silu of f16 11008 44.5 (5.1); a copy of 1 GiB runs at 5.1. A row is a
 // workgroup of the norm (its sum goes through LDS once), 256 threads of 2048 dims
 // one of the quantising. Few rows are a launch and a chain of latencies: one row
 // of 4096 3.2 us, one of silu of 11008 2.4. f32 arithmetic; a value is rounded
@@ -143,7 +143,8 @@ __global__ __launch_bounds__(256) void quant_kernel(QuantArgs a) {
 template <bool RF32, bool XF32>
 void launch_norm(st_context *ctx, const NormArgs &a, int M) {
     // One piece a thread up to 8192 dims (4095 rows of 4096, f32: 42.2 us; two 43.3, four 46.2; one row 2.9, 3.1, 3.7), but two
-    // of many f16 rows whose workgroups are large for what they load (4095 of 5120: 31.9 us, one 35.7, four 32.6)
+    // of many f16 rows whose workgroups are large for what they load (4095 rows, us of two and one: of 4112 27.3, 28.1; 4608
+    // 28.8, 29.6; 5120 31.8, 33.8; 6144 37.4, 37.2; 7168 42.5, 44.2; 8192 46.7, 47.7; 256 to 1024 rows 0 to 10 % less or equal)
     const bool two = !RF32 && a.pieces > 512 && M >= ctx->num_cus;
     const int per = a.pieces <= 1024 ? 1 + two : a.pieces <= 2048 ? 2 : 4;
     const dim3 block((unsigned)(((a.pieces + per - 1) / per + 63) / 64 * 64));

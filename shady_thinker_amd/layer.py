@@ -393,7 +393,8 @@ class DecoderStack:
     :749-756 and out_proj :786-791, gate/up/down :803-812, lm_head :824-834).
     Layers are DecoderLinears, DeltaNetLinears or Fp8DecoderLinears, in any mix
     (the reference's hybrid models); the lm_head is a GptqWeight, an Fp8Weight
-    or bf16.
+    or bf16. A step has at most 32 rows, of any kind of layer; more tokens (a
+    prompt) go through the layers' prefill.
 
     Between the projections a model runs its own ops (norms, attention or the
     DeltaNet core, residual adds: src/model.rs:685-690, 715-726, 758-784,
