@@ -391,13 +391,15 @@ int st_add_rmsnorm(st_context *ctx, const void *residual, int res_dtype, int64_t
 /* Rows of e4m3 of M rows a [K], or of silu(a) * b where b is given (the input
  * of a down projection), silu(v) = v / (1 + exp(-v)); dtype ST_F32 or ST_F16,
  * *_stride elements from one row to the next. Less than 2^24 units of a row's
- * 2048 dims. Pointers and strides in whole 16 bytes (y_scale: 4). */
+ * 2048 dims. Pointers and strides in whole 16 bytes (y_scale: 4). Outputs share
+ * no element with inputs. */
 int st_fp8_quant(st_context *ctx, const void *a, const void *b, int dtype, int64_t a_stride, int64_t b_stride,
                  uint8_t *y8, float *y_scale, int64_t scale_stride, int M, int K);
 
 /* y[m][n] = sum_b x_scale[b][m] w_scale[n / 128][b] sum_{k in b} x8[m][k] w[n][k],
  * y [M][N] of y_dtype (ST_F32 or ST_F16), any M and N (at most 2^28, and fewer
- * than 2^22 blocks of 128 x 128 of y). x8, w and y 16-byte aligned (scales: 4).
+ * than 2^22 blocks of 128 x 128 of y), in memory of its own. x8, w and y 16-byte
+ * aligned (scales: 4).
  * Sums are f32, in a fixed order for each size. With f32 y, and f16 y of at most
  * 64 tokens, products are exact. f16 y of more tokens comes from the 8-bit matrix
  * instruction, which keeps a product to 2^-13 of the power of two of the largest

@@ -54,7 +54,9 @@ def _row_stride(gpu, t, name: str, m: int, k: int) -> int:
 class Fp8Rows:
     """M quantised rows of K dims: data e4m3 [M, K], scale f32 [ceil(K / 128),
     M] (the scales of one block of dims side by side by token; a part of
-    wider rows will do). Row m's dim k is data[m, k] * scale[k // 128, m]."""
+    wider rows will do). Row m's dim k is data[m, k] * scale[k // 128, m].
+    Calls use the memory that both have when the rows are made: it is theirs as
+    long as the rows are used (no set_, resize_ or other .data)."""
 
     def __init__(self, gpu, m: int, k: int):
         """Allocates rows on the context's device; what they hold is undefined."""

@@ -241,7 +241,9 @@ def fp8_blocks(n: int) -> int:
 class Fp8Weight:
     """e4m3 weight of a block-scaled checkpoint: w float8_e4m3fn [N, K]
     row-major, scale f32 [ceil(N / 128), ceil(K / 128)] (what such files call
-    weight_scale_inv): the weight's value is w times its block's scale."""
+    weight_scale_inv): the weight's value is w times its block's scale. Calls use
+    the memory that both have when the weight is made: it is theirs as long as
+    the weight is used (no set_, resize_ or other .data)."""
 
     w: object
     scale: object
